@@ -11,7 +11,10 @@ LIB = os.path.join(PKG, 'libigcn_hip.so')
 ROOF_LIB = os.path.join(PKG, 'libigcn_roof.so')
 SOURCES = [f for f in ('spmm.hip', 'bpr.hip', 'score_topk.hip', 'topk_order.hip', 'sampler.hip', 'csr_util.hip')
            if os.path.exists(os.path.join(CSRC, f))]
+# -packed-fp32-ops: no packed fp32 arithmetic (v_pk_fma_f32 and its like, which hipcc forms from ordinary float code by itself): some of
+# its forms have given wrong results on this hardware now and then (the host pass does not know the feature and says so)
 FLAGS = ['-O3', '-std=c++17', '--offload-arch=gfx950', '-fPIC', '-Wall', '-Wno-unused-function',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC]
 # per source: the d = 128 candidate sweep runs one wave per SIMD with 396 registers; with MFMA results in VGPRs (this option)
 # the selection reads the accumulators where they are, the item tiles and user planes spill over into AGPRs instead
@@ -159,11 +162,11 @@ def scratch_report(lib_path=None):
 def build(force=False, verbose=True):
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
-    headers.append(os.path.join(ROOT, 'include', 'igcn_hip.h'))
+    headers += [os.path.join(ROOT, 'include', 'igcn_hip.h'), os.path.abspath(__file__)]         # (this file holds the flags)
     srcs = [os.path.join(CSRC, name) for name in SOURCES]
     # The shipped library is current (the GPU box gets the .so but not the objects: *.o is in .gpurunignore): nothing to do there
     main_current = not force and not _newer(srcs + headers, LIB)
-    objs = []
+    objs, running = [], []                                # (one hipcc per stale source, side by side)
     for name in ([] if main_current else SOURCES):
         src = os.path.join(CSRC, name)
         if not os.path.exists(src):
@@ -173,8 +176,11 @@ def build(force=False, verbose=True):
             cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(name, []) + ['-c', src, '-o', obj]
             if verbose:
                 print(' '.join(cmd), flush=True)
-            subprocess.check_call(cmd)
+            running.append((cmd, subprocess.Popen(cmd)))
         objs.append(obj)
+    failed = [cmd for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
     if not main_current and (force or _newer(objs, LIB)):
         cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs
         if verbose:
@@ -185,8 +191,8 @@ def build(force=False, verbose=True):
         raise RuntimeError('kernels with a private segment in %s (none is allowed: HIP-graph replays fault on them): %s' % (LIB, bad))
     # measurement kernels of bench.py (the in-run gather roof): a library of their own, never loaded by the product
     roof_src = os.path.join(CSRC, 'roof_probe.hip')
-    if os.path.exists(roof_src) and (force or _newer([roof_src], ROOF_LIB)):
-        cmd = [hipcc, '-O3', '-std=c++17', '--offload-arch=gfx950', '-fPIC', '-shared', '-o', ROOF_LIB, roof_src]
+    if os.path.exists(roof_src) and (force or _newer([roof_src, os.path.abspath(__file__)], ROOF_LIB)):
+        cmd = [hipcc] + FLAGS + ['-shared', '-o', ROOF_LIB, roof_src]
         if verbose:
             print(' '.join(cmd), flush=True)
         subprocess.check_call(cmd)

@@ -1131,7 +1131,7 @@ __global__ __launch_bounds__(kWave, ((MODE == 2 && D == 128 && NG == 2) || D == 
             float ureach[NG];                                  // s_u |u| of this lane's users: what a unit row can score at most
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                ureach[g] = A.tile_bound && user_ok[g] ? sqrtf(A.unorm2[group * UPW + g * 32 + j]) * ldexpf(1.f, -scale_exp(__uint_as_float(A.stats[2]))) : 0.f;
+                ureach[g] = A.tile_bound && user_ok[g] ? sqrtf(A.unorm2[group * UPW + g * 32 + cold(j)]) * ldexpf(1.f, -scale_exp(__uint_as_float(A.stats[2]))) : 0.f;
 #ifdef IGCN_X_TURN6
             constexpr int kTurn = 6;
 #else
