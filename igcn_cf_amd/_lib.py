@@ -91,6 +91,13 @@ SIGNATURES = {
     'igcn_bpr_loss_bwd_f32': (C.c_int, [vp, vp, vp, C.c_int64, vp, vp, vp, C.c_int64, vp, vp, vp,
                                         C.c_int64, C.c_int32, vp, vp, vp, C.c_float,
                                         vp, vp, vp, vp, vp, vp, vp, vp]),
+    'igcn_adamw_workspace_bytes': (C.c_int64, [vp, C.c_int64]),
+    'igcn_adamw_step': (C.c_int, [vp, C.c_int64, C.c_int32, C.c_double, vp, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp,
+                                  C.c_uint64, vp, vp]),
+    'igcn_grad_norm': (C.c_int, [vp, C.c_int64, vp, vp, vp]),
+    'igcn_quantize_rows_i8': (C.c_int, [vp, C.c_int32, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int64, vp, vp]),
+    'igcn_dequantize_rows_i8': (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64, vp]),
+    'igcn_matmul_i8': (C.c_int, [vp, C.c_int64, vp, vp, C.c_int64, vp, vp, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64, vp]),
     'igcn_bpr_loss_bwd_scaled_f32': (C.c_int, [vp, vp, vp, C.c_int64, vp, vp, vp, C.c_int64, vp, vp, vp,
                                                C.c_int64, C.c_int32, vp, vp, vp, C.c_float, C.c_float,
                                                vp, vp, vp, vp, vp, vp, vp, vp]),

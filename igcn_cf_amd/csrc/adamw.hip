@@ -1,0 +1,416 @@
+// AdamW over many tensors in one call, moments in float32 or in 8 bits, with the gradient norm over all tensors and clipping by it.
+//
+//   g' = c g,  c = min(1, max_norm / (|g| + 1e-6)) or 1;   m = b1 m + (1 - b1) g';   v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Nothing is used twice: the step is bound by the bytes of p, g, m, v (28 a float32 element, 16.1 with 8-bit moments), a small call by
+// its launches.  So: one launch for up to kTensors tensors, their pointers in the launch arguments (nothing is copied to the device,
+// a captured step replays with the addresses it was captured with), and one small launch before it that counts the steps, forms the
+// bias corrections once per tensor in 64 bits and adds the norm's partial sums up in a fixed order.
+//
+// 8-bit moments: blocks of 128 consecutive elements share s_m = max |m| / 448 and s_v = max v / 57344 (float32); m / s_m is held as
+// e4m3, v / s_v as e5m2.  An average that moves by 0.1 % a step would stand still under a code step of 12-25 % rounded to nearest, so
+// the codes are rounded stochastically: code = floor(x + u), u of 16 bits from a hash of (seed, tensor, step, element) — right in the
+// mean, the same on every replay and every machine.  v > 0 is never held as 0 (m / sqrt(0)).  The averages and codes are formed in
+// float32 with every operation rounded once, in the order written (no fused multiply-add): elementary float32 operations in any other
+// program give the same codes, bit for bit.
+#include "dtypes.h"
+#include <cmath>
+
+namespace igcn {
+
+constexpr int kTensors = 56;             // of one launch: 64 bytes each in at most 4 KiB of launch arguments
+constexpr int kPer = 8;                  // elements of a thread: 16 lanes (a DPP row) hold a block of 128
+constexpr int kChunk = kBlock * kPer;    // elements of a workgroup
+constexpr int kNormBlocks = 512;         // partial sums of a norm launch
+static_assert(IGCN_ADAMW_BLOCK == 16 * kPer, "a block of the 8-bit moments is a DPP row's elements");
+
+struct TensorTable {
+    igcn_adamw_tensor t[kTensors];
+    int first[kTensors + 1];             // first chunk of each tensor; [n] = all chunks of the launch
+    int n;
+};
+// what the small launch leaves for the others, per tensor of the call
+struct Prepared { float factor, step_size, inv_sqrt_c2, keep; uint32_t key, pad[3]; };      // keep = 1 - lr wd
+
+struct Hyper {
+    double beta1, beta2, log_beta1, log_beta2, lr, weight_decay, max_norm;
+    const float *lr_dev;
+    float eps;
+    uint32_t seed_lo, seed_hi;
+};
+
+// 8 consecutive values of src at element i; `whole`: all 8 are there and src is aligned to 8 of them (16 bytes at most)
+template <typename T> __device__ __forceinline__ void load8(const T *__restrict__ src, int64_t i, int64_t n, bool whole, T (&x)[kPer])
+{
+    if (whole) {
+        struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) V { T v[kPer]; };
+        const V w = *reinterpret_cast<const V *>(src + i);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) x[k] = w.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) x[k] = i + k < n ? src[i + k] : T(0.f);
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T *__restrict__ dst, int64_t i, int64_t n, bool whole, const T (&x)[kPer])
+{
+    if (whole) {
+        struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) V { T v[kPer]; } w;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) w.v[k] = x[k];
+        *reinterpret_cast<V *>(dst + i) = w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) if (i + k < n) dst[i + k] = x[k];
+    }
+}
+
+__device__ __forceinline__ int tensor_of_chunk(const TensorTable &T, int chunk)
+{
+    int lo = 0, hi = T.n - 1;                                   // the last tensor whose first chunk is not behind this one
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (T.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// ---- the norm ------------------------------------------------------------------------------------------------------------------
+template <typename G> __device__ __forceinline__ double chunk_squares(const G *__restrict__ g, int64_t i, int64_t n)
+{
+    if (i >= n) return 0.0;
+    G x[kPer];
+    load8(g, i, n, i + kPer <= n && aligned(g, sizeof(G) * kPer < 16 ? sizeof(G) * kPer : 16), x);
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) { const double y = to_float(x[k]); s = fma(y, y, s); }
+    return s;
+}
+
+__device__ __forceinline__ double block_sum(double s, double *lds)
+{
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = lds[0] + lds[1] + lds[2] + lds[3];
+    __syncthreads();
+    return s;
+}
+
+// partial[blockIdx.x] = squares of the chunks blockIdx.x, + gridDim.x, ...: sums in float64, in an order that depends on the sizes alone
+__global__ __launch_bounds__(kBlock) void grad_squares_kernel(const TensorTable T, double *__restrict__ partial)
+{
+    __shared__ double lds[kBlock / kWave];
+    double s = 0.0;
+    for (int chunk = blockIdx.x; chunk < T.first[T.n]; chunk += gridDim.x) {
+        const int at = tensor_of_chunk(T, chunk);
+        const igcn_adamw_tensor &t = T.t[at];
+        const int64_t i = (int64_t)(chunk - T.first[at]) * kChunk + threadIdx.x * kPer;
+        if (t.grad_dtype == IGCN_DTYPE_F32) s += chunk_squares(static_cast<const float *>(t.grad), i, t.n);
+        else if (t.grad_dtype == IGCN_DTYPE_BF16) s += chunk_squares(static_cast<const __hip_bfloat16 *>(t.grad), i, t.n);
+        else s += chunk_squares(static_cast<const __half *>(t.grad), i, t.n);
+    }
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ double norm_of(const double *__restrict__ partial, int n, double *lds)
+{
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += kBlock) s += partial[i];
+    return sqrt(block_sum(s, lds));
+}
+
+__global__ __launch_bounds__(kBlock) void grad_norm_kernel(const double *__restrict__ partial, int n, float *__restrict__ out)
+{
+    __shared__ double lds[kBlock / kWave];
+    const double norm = norm_of(partial, n, lds);
+    if (threadIdx.x == 0) *out = (float)norm;
+}
+
+// ---- before the step: steps counted, bias corrections, the clipping factor ------------------------------------------------------
+__global__ __launch_bounds__(kBlock) void adamw_prepare_kernel(const TensorTable T, int index0, const Hyper H, const double *__restrict__ partial,
+                                                               int n_partial, const float *norm_in, float *norm_out, Prepared *__restrict__ prep)
+{
+    __shared__ double lds[kBlock / kWave];
+    double factor = 1.0;
+    if (H.max_norm > 0.0) {
+        const double norm = norm_in ? (double)*norm_in : norm_of(partial, n_partial, lds);
+        if (!norm_in && norm_out && index0 == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+        factor = H.max_norm / (norm + 1e-6);
+        factor = factor > 1.0 ? 1.0 : factor;                    // (a NaN norm stays one: the parameters show it)
+    }
+    const int i = threadIdx.x;
+    if (i >= T.n) return;
+    const float step = *T.t[i].step + 1.f;
+    *T.t[i].step = step;
+    const double lr = H.lr_dev ? (double)*H.lr_dev : H.lr;
+    Prepared q;
+    q.factor = (float)factor;
+    q.step_size = (float)(lr / -expm1((double)step * H.log_beta1));          // 1 - b^t without cancellation
+    q.inv_sqrt_c2 = (float)(1.0 / sqrt(-expm1((double)step * H.log_beta2)));
+    q.key = mix32(mix32((uint32_t)(int64_t)step ^ H.seed_lo) ^ (H.seed_hi + (uint32_t)(index0 + i) * 0x9e3779b9u));
+    q.keep = (float)(1.0 - lr * H.weight_decay);
+    q.pad[0] = q.pad[1] = q.pad[2] = 0u;
+    prep[index0 + i] = q;
+}
+
+// ---- the step --------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float stepped(float p, float m, float v, const Prepared &q, float eps)
+{
+    const float denom = fmaf(__builtin_amdgcn_sqrtf(v), q.inv_sqrt_c2, eps);          // 1 ulp each: the update is far below the parameter
+    return fmaf(-q.step_size, m * __builtin_amdgcn_rcpf(denom), p * q.keep);
+}
+
+template <typename P, typename G>
+__device__ __forceinline__ void step32(const igcn_adamw_tensor &t, int64_t i, const Hyper &H, const Prepared &q)
+{
+    const bool ok = i + kPer <= t.n && aligned(t.param, 16) && aligned(t.grad, 16) && aligned(t.exp_avg, 16) && aligned(t.exp_avg_sq, 16);
+    P p[kPer]; G g[kPer]; float m[kPer], v[kPer];
+    load8(static_cast<const G *>(t.grad), i, t.n, ok, g);
+    load8(static_cast<const float *>(t.exp_avg), i, t.n, ok, m);
+    load8(static_cast<const float *>(t.exp_avg_sq), i, t.n, ok, v);
+    load8(static_cast<const P *>(t.param), i, t.n, ok, p);
+    const float factor = q.factor, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const float x = to_float(g[k]) * factor;
+        m[k] = fmaf(a1, x - m[k], m[k]);
+        v[k] = fmaf(a2, fmaf(x, x, -v[k]), v[k]);
+        p[k] = from_float<P>(stepped(to_float(p[k]), m[k], v[k], q, H.eps));
+    }
+    store8(static_cast<float *>(t.exp_avg), i, t.n, ok, m);
+    store8(static_cast<float *>(t.exp_avg_sq), i, t.n, ok, v);
+    store8(static_cast<P *>(t.param), i, t.n, ok, p);
+}
+
+template <int ROR> __device__ __forceinline__ float row_ror(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 | ROR, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row_max(float x)               // the largest of 16 lanes, in all of them
+{
+    x = fmaxf(x, row_ror<8>(x)); x = fmaxf(x, row_ror<4>(x)); x = fmaxf(x, row_ror<2>(x)); return fmaxf(x, row_ror<1>(x));
+}
+
+// t >= 0 as an 8-bit floating code of MANT binary digits, smallest normal 2^EMIN, rounded up where its cut-off part and
+// u = (r16 + 0.5) / 2^16 make one
+template <int MANT, int EMIN> __device__ __forceinline__ uint32_t code_of(float t, uint32_t r16)
+{
+    const int e = max(__float_as_int(t) >> 23, 127 + EMIN);
+    const float u = ((float)r16 + 0.5f) * 0x1p-16f;
+    return ((uint32_t)(e - (127 + EMIN)) << MANT) + (uint32_t)(__builtin_amdgcn_ldexpf(t, MANT + 127 - e) + u);
+}
+
+template <typename P, typename G>
+__device__ __forceinline__ void step8(const igcn_adamw_tensor &t, int64_t i, const Hyper &H, const Prepared &q)
+{
+#pragma clang fp contract(off)
+    const bool ok = i + kPer <= t.n && aligned(t.param, 16) && aligned(t.grad, 16) && aligned(t.exp_avg, 8) && aligned(t.exp_avg_sq, 8);
+    P p[kPer]; G g[kPer]; uint8_t mc[kPer], vc[kPer];
+    load8(static_cast<const G *>(t.grad), i, t.n, ok, g);
+    load8(static_cast<const uint8_t *>(t.exp_avg), i, t.n, ok, mc);
+    load8(static_cast<const uint8_t *>(t.exp_avg_sq), i, t.n, ok, vc);
+    load8(static_cast<const P *>(t.param), i, t.n, ok, p);
+    const int64_t block = i / IGCN_ADAMW_BLOCK;
+    const bool there = i < t.n;                                  // (lanes behind the end stay for their row's maximum)
+    const float sm = there ? t.scales[2 * block] : 0.f, sv = there ? t.scales[2 * block + 1] : 0.f;
+    const float b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2);
+    float m[kPer], v[kPer], big_m = 0.f, big_v = 0.f;
+    float all = fabsf(sm) + fabsf(sv);                           // finite where every input of these averages is
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const float x = to_float(g[k]) * q.factor;
+        all += fabsf(x);
+        m[k] = b1 * (__builtin_amdgcn_cvt_f32_fp8(mc[k], 0) * sm) + a1 * x;
+        v[k] = b2 * (__builtin_amdgcn_cvt_f32_bf8(vc[k], 0) * sv) + a2 * x * x;
+        big_m = fmaxf(big_m, fabsf(m[k]));
+        big_v = fmaxf(big_v, v[k]);
+        p[k] = from_float<P>(stepped(to_float(p[k]), m[k], v[k], q, H.eps));
+    }
+    const bool bad = !(all < INFINITY);
+    if (bad) big_m = big_v = INFINITY;
+    big_m = row_max(big_m);
+    big_v = row_max(big_v);
+    constexpr float kSmallest = 0x1p-100f;                       // below: held as zero (the reciprocal stays finite)
+    const float inv_m = big_m >= kSmallest && big_m < INFINITY ? 1.f / big_m * 448.f : 0.f;
+    const float inv_v = big_v >= kSmallest && big_v < INFINITY ? 1.f / big_v * 57344.f : 0.f;
+    const uint32_t base = mix32(q.key ^ (uint32_t)((uint64_t)i >> 32));
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const uint32_t h = mix32((uint32_t)(i + k) ^ base);
+        const float tm = fabsf(m[k]) * inv_m, tv = v[k] * inv_v;
+        uint32_t cm = bad ? 0u : code_of<3, -6>(tm, h & 0xffffu), cv = bad ? 0u : code_of<2, -14>(tv, h >> 16);
+        cv = max(cv, tv > 0.f ? 1u : 0u);
+        cm |= cm && m[k] < 0.f ? 0x80u : 0u;
+        mc[k] = (uint8_t)cm;
+        vc[k] = (uint8_t)cv;
+    }
+    if (!there) return;
+    store8(static_cast<uint8_t *>(t.exp_avg), i, t.n, ok, mc);
+    store8(static_cast<uint8_t *>(t.exp_avg_sq), i, t.n, ok, vc);
+    store8(static_cast<P *>(t.param), i, t.n, ok, p);
+    if ((threadIdx.x & 15) == 0) {
+        t.scales[2 * block] = big_m < INFINITY ? (inv_m == 0.f ? 0.f : big_m * (1.f / 448.f)) : NAN;
+        t.scales[2 * block + 1] = big_v < INFINITY ? (inv_v == 0.f ? 0.f : big_v * (1.f / 57344.f)) : NAN;
+    }
+}
+
+template <int BITS, typename P, typename G>
+__device__ __forceinline__ void step_any(const igcn_adamw_tensor &t, int64_t i, const Hyper &H, const Prepared &q)
+{
+    if constexpr (BITS == 8) step8<P, G>(t, i, H, q);
+    else if (i < t.n) step32<P, G>(t, i, H, q);
+}
+
+template <int BITS>
+__global__ __launch_bounds__(kBlock) void adamw_step_kernel(const TensorTable T, const Hyper H, const Prepared *__restrict__ prep)
+{
+    const int chunk = blockIdx.x;
+    const int k = tensor_of_chunk(T, chunk);
+    const igcn_adamw_tensor &t = T.t[k];
+    const Prepared q = prep[k];
+    const int64_t i = (int64_t)(chunk - T.first[k]) * kChunk + threadIdx.x * kPer;
+    if (t.dtype == IGCN_DTYPE_F32) step_any<BITS, float, float>(t, i, H, q);
+    else if (t.dtype == IGCN_DTYPE_BF16) {
+        if (t.grad_dtype == IGCN_DTYPE_F32) step_any<BITS, __hip_bfloat16, float>(t, i, H, q);
+        else step_any<BITS, __hip_bfloat16, __hip_bfloat16>(t, i, H, q);
+    } else {
+        if (t.grad_dtype == IGCN_DTYPE_F32) step_any<BITS, __half, float>(t, i, H, q);
+        else step_any<BITS, __half, __half>(t, i, H, q);
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------
+static int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+// Calls fn(table, index of its first tensor) for every launch the tensors need; empty tensors keep their place (no chunk of their own).
+template <typename F> static int for_tables(const igcn_adamw_tensor *tensors, int64_t n, F fn)
+{
+    for (int64_t at = 0; at < n;) {
+        TensorTable T;
+        T.n = 0;
+        int64_t chunks = 0;
+        const int64_t from = at;
+        for (; at < n && T.n < kTensors; ++at) {
+            const int64_t c = chunks_of(tensors[at].n);
+            if (chunks + c > 0x7fffffff) { if (T.n) break; return IGCN_E_SHAPE; }
+            T.t[T.n] = tensors[at];
+            T.first[T.n++] = (int)chunks;
+            chunks += c;
+        }
+        for (int i = T.n; i <= kTensors; ++i) T.first[i] = (int)chunks;
+        const int rc = fn(T, (int)from);
+        if (rc != IGCN_OK) return rc;
+    }
+    return IGCN_OK;
+}
+
+static int grad_squares(const igcn_adamw_tensor *tensors, int64_t n, double *partial, int *n_partial, hipStream_t st)
+{
+    *n_partial = 0;
+    return for_tables(tensors, n, [&](const TensorTable &T, int) {
+        const int chunks = T.first[T.n];
+        if (chunks == 0) return (int)IGCN_OK;
+        const int blocks = chunks < kNormBlocks ? chunks : kNormBlocks;
+        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, T, partial + *n_partial);
+        *n_partial += blocks;
+        return launch_status();
+    });
+}
+
+// moment_bits 0: only the gradients are looked at
+static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment_bits)
+{
+    if (n < 0 || n > 0x7fffffff) return IGCN_E_SHAPE;
+    if (n > 0 && !tensors) return IGCN_E_NULL;
+    const bool eight = moment_bits == 8;
+    for (int64_t i = 0; i < n; ++i) {
+        const igcn_adamw_tensor &t = tensors[i];
+        if (t.n < 0) return IGCN_E_SHAPE;
+        if (!dtype_ok(t.grad_dtype)) return IGCN_E_RANGE;
+        if (t.n > 0 && !t.grad) return IGCN_E_NULL;
+        if (misaligned(t.grad, t.grad_dtype)) return IGCN_E_ALIGN;
+        if (moment_bits == 0) continue;
+        if (!dtype_ok(t.dtype) || (t.grad_dtype != t.dtype && t.grad_dtype != IGCN_DTYPE_F32)) return IGCN_E_RANGE;
+        if (!t.step || (t.n > 0 && (!t.param || !t.exp_avg || !t.exp_avg_sq))) return IGCN_E_NULL;
+        if (eight && t.n > 0 && !t.scales) return IGCN_E_NULL;
+        if (misaligned(t.param, t.dtype)) return IGCN_E_ALIGN;
+        if (!eight && ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & 3)) return IGCN_E_ALIGN;
+        if ((reinterpret_cast<uintptr_t>(t.scales) | reinterpret_cast<uintptr_t>(t.step)) & 3) return IGCN_E_ALIGN;
+    }
+    return IGCN_OK;
+}
+
+}  // namespace igcn
+
+using namespace igcn;
+
+extern "C" int64_t igcn_adamw_workspace_bytes(const igcn_adamw_tensor *tensors_host, int64_t n_tensors)
+{
+    if (check_tensors(tensors_host, n_tensors, 0) != IGCN_OK) return -1;
+    int64_t partials = 0;
+    if (for_tables(tensors_host, n_tensors, [&](const TensorTable &T, int) { partials += T.first[T.n] < kNormBlocks ? T.first[T.n] : kNormBlocks; return (int)IGCN_OK; }) != IGCN_OK)
+        return -1;
+    return n_tensors * (int64_t)sizeof(Prepared) + partials * 8 + 16;
+}
+
+extern "C" int igcn_grad_norm(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, float *norm, void *workspace, void *stream)
+{
+    const int rc = check_tensors(tensors_host, n_tensors, 0);
+    if (rc != IGCN_OK) return rc;
+    if (!norm || !workspace) return IGCN_E_NULL;
+    if ((reinterpret_cast<uintptr_t>(norm) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 15)) return IGCN_E_ALIGN;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    double *partial = static_cast<double *>(workspace);
+    int n_partial = 0;
+    const int rs = grad_squares(tensors_host, n_tensors, partial, &n_partial, st);
+    if (rs != IGCN_OK) return rs;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, st, partial, n_partial, norm);
+    return launch_status();
+}
+
+extern "C" int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, int32_t moment_bits, double lr, const float *lr_dev, double beta1, double beta2,
+                               double eps, double weight_decay, double max_norm, const float *norm_in, float *norm_out, uint64_t seed,
+                               void *workspace, void *stream)
+{
+    if (moment_bits != 8 && moment_bits != 32) return IGCN_E_RANGE;
+    const int rc = check_tensors(tensors_host, n_tensors, moment_bits);
+    if (rc != IGCN_OK) return rc;
+    if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(max_norm >= 0.0))
+        return IGCN_E_RANGE;
+    if (n_tensors > 0 && !workspace) return IGCN_E_NULL;
+    if (max_norm > 0.0 && !norm_in && !norm_out) return IGCN_E_NULL;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) || ((reinterpret_cast<uintptr_t>(norm_in) | reinterpret_cast<uintptr_t>(norm_out) | reinterpret_cast<uintptr_t>(lr_dev)) & 3))
+        return IGCN_E_ALIGN;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    Prepared *prep = static_cast<Prepared *>(workspace);
+    double *partial = reinterpret_cast<double *>(prep + n_tensors);
+    int n_partial = 0;
+    if (max_norm > 0.0 && !norm_in) {
+        const int rs = grad_squares(tensors_host, n_tensors, partial, &n_partial, st);
+        if (rs != IGCN_OK) return rs;
+        if (n_tensors == 0) {
+            hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, st, partial, 0, norm_out);
+            return launch_status();
+        }
+    }
+    Hyper H;
+    H.beta1 = beta1; H.beta2 = beta2; H.log_beta1 = std::log(beta1); H.log_beta2 = std::log(beta2);
+    H.lr = lr; H.lr_dev = lr_dev;
+    H.weight_decay = weight_decay; H.max_norm = max_norm; H.eps = (float)eps;
+    H.seed_lo = (uint32_t)seed; H.seed_hi = (uint32_t)(seed >> 32);
+    return for_tables(tensors_host, n_tensors, [&](const TensorTable &T, int index0) {
+        hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(kBlock), 0, st, T, index0, H, partial, n_partial, norm_in, norm_out, prep);
+        int rs = launch_status();
+        if (rs != IGCN_OK || T.first[T.n] == 0) return rs;
+        const dim3 grid((unsigned)T.first[T.n]);
+        if (moment_bits == 8) hipLaunchKernelGGL(adamw_step_kernel<8>, grid, dim3(kBlock), 0, st, T, H, prep + index0);
+        else hipLaunchKernelGGL(adamw_step_kernel<32>, grid, dim3(kBlock), 0, st, T, H, prep + index0);
+        return launch_status();
+    });
+}

@@ -98,6 +98,20 @@ class BasicModel(nn.Module):
                                 excl_col=excl_col, banned=banned, mode=mode)
         return idx
 
+    # ---- the dense score block from 8-bit rows -------------------------------------
+    def quantized_items(self):
+        """(codes int8 [n_items, d], scale float32 [n_items]): the item rows scores are made from, laid out once for predict_i8
+        (a quarter of the float32 table); stale after the parameters change."""
+        with torch.no_grad():
+            return ops.quantize_rows_i8(self.score_tables()[1])
+
+    def predict_i8(self, users, items=None, dtype=torch.float32):
+        """predict(users) from 8-bit integers: user rows made 8-bit on the way, item rows from `items` = quantized_items() (None:
+        made here); every row has a scale of its own, so a score is off by at most 0.4 % of max|u| |i|_1 + |u|_1 max|i|."""
+        with torch.no_grad():
+            codes, scale = items if items is not None else self.quantized_items()
+            return ops.linear_i8(self.score_tables()[0][users], codes, scale, dtype=dtype)
+
     def _cached_rep(self, key, compute):
         if self.training or torch.is_grad_enabled():
             return compute()

@@ -4,6 +4,7 @@ PyTorch is plumbing here: it owns device memory, the current HIP stream and the
 autograd graph.  All arithmetic of the hot path runs in libigcn_hip.so; there is
 no eager/PyTorch fallback — a missing library or a non-GPU tensor raises.
 """
+import array
 import ctypes as C
 
 import torch
@@ -770,3 +771,220 @@ def bpr_sample(train_rowptr, train_col, nonempty_users, n_items, batch, seed, ou
                                           nonempty_users.numel(), n_items, batch, int(seed) & 0xFFFFFFFFFFFFFFFF,
                                           out.data_ptr(), _lib.current_stream()), 'igcn_bpr_sample')
     return out
+
+
+# ---- the optimizer step over many tensors (csrc/adamw.hip) ----------------------------------------------------------------------
+_DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # IGCN_DTYPE_*
+ADAMW_BLOCK = 128                  # IGCN_ADAMW_BLOCK: consecutive elements that share a scale in the 8-bit moments
+MOMENT_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)                        # of exp_avg and exp_avg_sq in 8 bits
+
+
+class _on:
+    """The device of a tensor as the current one, for a call's launches and workspaces (nothing to do where it is already)."""
+
+    def __init__(self, device):
+        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _dense(t):
+    """Whether the elements of t fill one stretch of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _same_order(a, b):
+    return a.shape == b.shape and (a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous()))
+
+
+def _check_grads(grads):
+    """The one device the gradients are on."""
+    device = grads[0].device if grads else None
+    for g in grads:
+        if not (isinstance(g, torch.Tensor) and g.is_cuda and g.layout == torch.strided and g.dtype in _DTYPE_CODES):
+            raise _lib.IgcnError('gradients must be dense float32, bfloat16 or float16 tensors on the GPU (no CPU path)')
+        if g.device != device:
+            raise _lib.IgcnError('the tensors of a call must be on one device')
+        if not _dense(g):
+            raise _lib.IgcnError('gradients must fill a stretch of memory (a view with gaps or repeats does not)')
+    return device
+
+
+def grad_norm(grads):
+    """float32 scalar on the GPU: the L2 norm over all elements of all tensors of the list (igcn_grad_norm), added up in float64 in
+    an order that depends on the sizes alone.  What torch.nn.utils.clip_grad_norm_ returns, without touching the gradients:
+    adamw_step(..., max_grad_norm=..., grad_norm=...) clips by it on the way."""
+    grads = list(grads)
+    device = _check_grads(grads)
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device='cuda')
+    rows = array.array('q')
+    for g in grads:
+        rows.extend((0, g.data_ptr(), 0, 0, 0, 0, g.numel(), _DTYPE_CODES[g.dtype] << 32))
+    with _on(device):
+        L, table = _lib.lib(), rows.buffer_info()[0]
+        ws = torch.empty(L.igcn_adamw_workspace_bytes(table, len(grads)), dtype=torch.uint8, device=device)
+        out = torch.empty((), dtype=torch.float32, device=device)
+        _lib.check(L.igcn_grad_norm(table, len(grads), out.data_ptr(), ws.data_ptr(), _lib.current_stream()), 'igcn_grad_norm')
+    return out
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None,
+               scales=None, seed=0, grad_norm=None):
+    """One AdamW step over all tensors of the lists, in place (igcn_adamw_step; optim.AdamW is the optimizer around it).
+
+    params: float32, bfloat16 or float16, any shapes, dense in memory; grads: the same shape and order in memory, dtype of the
+    parameter or float32; steps: one float32 number each on the GPU, the steps taken so far (the call adds 1).
+    scales None: exp_avgs / exp_avg_sqs are float32.  scales given: moments in 8 bits — exp_avgs float8_e4m3fn, exp_avg_sqs
+    float8_e5m2, scales float32 [ceil(numel / 128), 2] (the scales of a block of 128 consecutive elements in memory order: a moment is
+    its code times its block's scale), rounded stochastically from (seed, place in the list, step, element); zeros to start with.
+    lr: a number, or a one-element float32 tensor on the GPU (read by the kernel: HIP-graph replays see its current value).
+    max_grad_norm: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) on the way; norm = L2 norm over all of them, computed
+    here or given as `grad_norm` (a one-element float32 tensor, for several calls clipped by one norm).  Returns the norm, or None."""
+    params, grads, exp_avgs, exp_avg_sqs, steps = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps)
+    n, eight = len(params), scales is not None
+    scales = list(scales) if eight else [None] * n
+    if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps) == len(scales) == n:
+        raise _lib.IgcnError('adamw_step takes as many gradients, moments, steps (and scales) as parameters')
+    if max_grad_norm is not None and not max_grad_norm > 0.:
+        raise _lib.IgcnError('max_grad_norm must be positive')
+    if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and weight_decay >= 0.):
+        raise _lib.IgcnError('betas must be in [0, 1), eps and weight_decay not negative')
+    device = _check_grads(grads)
+    want_m, want_v = MOMENT_DTYPES if eight else (torch.float32, torch.float32)
+    rows, written = array.array('q'), []
+    for p, g, m, v, t, s in zip(params, grads, exp_avgs, exp_avg_sqs, steps, scales):
+        if p.device != device or m.device != device or v.device != device or t.device != device or (eight and s.device != device):
+            raise _lib.IgcnError('the tensors of a call must be on one device')
+        if p.dtype not in _DTYPE_CODES or (g.dtype != p.dtype and g.dtype != torch.float32) or m.dtype != want_m or v.dtype != want_v:
+            raise _lib.IgcnError('parameters: float32, bfloat16 or float16; gradients: the same or float32; moments: float32, or with scales '
+                                 'float8_e4m3fn and float8_e5m2 (got %s, %s, %s, %s)' % (p.dtype, g.dtype, m.dtype, v.dtype))
+        if not (_same_order(p, g) and _same_order(p, m) and _same_order(p, v)):
+            raise _lib.IgcnError('gradient and moments must have the shape and the order in memory of their parameter')
+        if t.dtype != torch.float32 or t.numel() != 1:
+            raise _lib.IgcnError('steps must be one-element float32 tensors')
+        k = p.numel()
+        if eight and (s.dtype != torch.float32 or s.shape != ((k + ADAMW_BLOCK - 1) // ADAMW_BLOCK, 2) or not s.is_contiguous()):
+            raise _lib.IgcnError('scales must be contiguous float32 [ceil(numel / %d), 2]' % ADAMW_BLOCK)
+        ptrs = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), s.data_ptr() if eight else 0, t.data_ptr())
+        rows.extend(ptrs)
+        rows.extend((k, _DTYPE_CODES[p.dtype] | _DTYPE_CODES[g.dtype] << 32))
+        written += [ptrs[0], ptrs[2], ptrs[3], ptrs[5]] if k else [ptrs[5]]
+    if len(set(written)) != len(written):
+        raise _lib.IgcnError('a tensor stands in the lists twice: every parameter, moment and step is rewritten by one place only')
+    lr_dev = norm_in = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or (n and lr.device != device):
+            raise _lib.IgcnError('a device learning rate must be a one-element float32 tensor on the GPU')
+        lr_dev, lr = lr, 0.
+    elif not lr >= 0.:
+        raise _lib.IgcnError('lr must not be negative')
+    if max_grad_norm is not None and grad_norm is not None:
+        if not isinstance(grad_norm, torch.Tensor) or grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or (n and grad_norm.device != device):
+            raise _lib.IgcnError('grad_norm must be a one-element float32 tensor on the GPU')
+        norm_in = grad_norm
+    if n == 0:
+        return None if max_grad_norm is None else norm_in if norm_in is not None else torch.zeros((), dtype=torch.float32, device='cuda')
+    with _on(device):
+        L, table = _lib.lib(), rows.buffer_info()[0]
+        ws = torch.empty(L.igcn_adamw_workspace_bytes(table, n), dtype=torch.uint8, device=device)
+        norm = norm_in
+        if max_grad_norm is not None and norm is None:
+            norm = torch.empty((), dtype=torch.float32, device=device)
+        _lib.check(L.igcn_adamw_step(table, n, 8 if eight else 32, float(lr), _lib.ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
+                                     float(weight_decay), 0. if max_grad_norm is None else float(max_grad_norm), _lib.ptr(norm_in),
+                                     _lib.ptr(norm) if norm_in is None else None, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(),
+                                     _lib.current_stream()), 'igcn_adamw_step')
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    return norm
+
+
+# ---- rows in 8-bit integers and their product (csrc/gemm_i8.hip) ------------------------------------------------------------------
+MAX_I8_DEPTH = 131071              # IGCN_MAX_I8_DEPTH: the longest sum of 8-bit products that int32 holds
+
+
+def _require_rows(t, name, dtypes):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+        raise _lib.IgcnError('%s must be a %s tensor on the GPU (no CPU path)' % (name, ' / '.join(str(d).replace('torch.', '') for d in dtypes)))
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise _lib.IgcnError('%s must be 2-D, its rows contiguous and apart' % name)
+
+
+def _ld(t):
+    """Leading dimension of 2-D rows (a single row has whatever stride)."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _require_vector(t, name, n, device):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.device == device):
+        raise _lib.IgcnError('%s must be contiguous float32 [%d] on the device of the rows' % (name, n))
+
+
+def quantize_rows_i8(x):
+    """(codes int8 [M, K], scale float32 [M]) of the rows of x (float32, bfloat16 or float16 [M, K], rows contiguous): scale =
+    max|row| / 127, codes = row / scale to the nearest whole number, ties to even (igcn_quantize_rows_i8).  A row of zeros has scale 0;
+    one with a NaN or an infinity has scale NaN, so that what is computed from it shows it."""
+    _require_rows(x, 'x', tuple(_DTYPE_CODES))
+    m, k = x.shape
+    with _on(x.device):
+        q = torch.empty((m, k), dtype=torch.int8, device=x.device)
+        scale = torch.empty(m, dtype=torch.float32, device=x.device)
+        _lib.check(_lib.lib().igcn_quantize_rows_i8(x.data_ptr(), _DTYPE_CODES[x.dtype], _ld(x), m, k, q.data_ptr(), k, scale.data_ptr(),
+                                                    _lib.current_stream()), 'igcn_quantize_rows_i8')
+    return q, scale
+
+
+def dequantize_rows_i8(codes, scale, dtype=torch.float32):
+    """[M, K] of `dtype`: the values that rows of codes stand for, codes[m, k] * scale[m] (igcn_dequantize_rows_i8)."""
+    _require_rows(codes, 'codes', (torch.int8,))
+    if dtype not in _DTYPE_CODES:
+        raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
+    m, k = codes.shape
+    _require_vector(scale, 'scale', m, codes.device)
+    with _on(codes.device):
+        y = torch.empty((m, k), dtype=dtype, device=codes.device)
+        _lib.check(_lib.lib().igcn_dequantize_rows_i8(codes.data_ptr(), _ld(codes), scale.data_ptr(), m, k, y.data_ptr(), _DTYPE_CODES[dtype], k,
+                                                      _lib.current_stream()), 'igcn_dequantize_rows_i8')
+    return y
+
+
+def matmul_i8(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
+    """[M, N] of `dtype`: (a @ b.T) * a_scale[:, None] * b_scale (+ bias) for 8-bit integer rows a [M, K] and b [N, K] with a float32
+    scale each (igcn_matmul_i8).  The sums are exact, K <= 131071."""
+    _require_rows(a, 'a', (torch.int8,))
+    _require_rows(b, 'b', (torch.int8,))
+    (m, k), n = a.shape, b.shape[0]
+    if b.shape[1] != k or b.device != a.device:
+        raise _lib.IgcnError('a [M, K] and b [N, K] must agree in K and be on one device (got %s on %s, %s on %s)' % (tuple(a.shape), a.device, tuple(b.shape), b.device))
+    if k > MAX_I8_DEPTH:
+        raise _lib.IgcnError('K must be at most %d: a longer sum could pass 32 bits' % MAX_I8_DEPTH)
+    if dtype not in _DTYPE_CODES:
+        raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
+    _require_vector(a_scale, 'a_scale', m, a.device)
+    _require_vector(b_scale, 'b_scale', n, a.device)
+    if bias is not None:
+        _require_vector(bias, 'bias', n, a.device)
+    with _on(a.device):
+        y = torch.empty((m, n), dtype=dtype, device=a.device)
+        _lib.check(_lib.lib().igcn_matmul_i8(a.data_ptr(), _ld(a), a_scale.data_ptr(), b.data_ptr(), _ld(b), b_scale.data_ptr(), _lib.ptr(bias),
+                                             m, n, k, y.data_ptr(), _DTYPE_CODES[dtype], n, _lib.current_stream()), 'igcn_matmul_i8')
+    return y
+
+
+def linear_i8(x, b, b_scale, bias=None, dtype=None):
+    """[M, N] of `dtype` (None: that of x): the rows of x made 8-bit (quantize_rows_i8) and multiplied with those of b (matmul_i8)."""
+    q, scale = quantize_rows_i8(x)
+    return matmul_i8(q, scale, b, b_scale, bias=bias, dtype=x.dtype if dtype is None else dtype)

@@ -1,0 +1,86 @@
+"""AdamW on the HIP kernels (ops.adamw_step): all parameters of a group in one call, moments in float32 or in 8 bits.
+
+The reference trains with torch's Adam, by name (trainer.py:43-45); config key 'optimizer': 'AdamW' takes this one instead."""
+import torch
+
+from . import _lib, ops
+
+
+class AdamW(torch.optim.Optimizer):
+    """Adam with decoupled weight decay.  state_bits 32: moments in float32 (state names and meaning of torch.optim.AdamW, whose
+    state_dict it takes).  state_bits 8: exp_avg as float8_e4m3fn and exp_avg_sq as float8_e5m2 codes with two float32 scales a block
+    of 128 elements ('scales') — 2.06 bytes a parameter instead of 8; a moment is codes.float() * its block's scale.
+    max_grad_norm: clip by the norm over the gradients of ALL groups; the last step's norm is `grad_norm` (a tensor on the GPU).
+    seed: of the 8-bit moments' stochastic rounding.  The step count lives on the device and lr may be a one-element float32 tensor
+    there: the step can sit in a HIP graph."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, seed=0):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.:
+            raise ValueError('lr must not be negative')
+        if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1.) or not eps >= 0. or not weight_decay >= 0.:
+            raise ValueError('betas must be in [0, 1), eps and weight_decay not negative')
+        if state_bits not in (8, 32):
+            raise ValueError('state_bits must be 8 or 32')
+        if max_grad_norm is not None and not max_grad_norm > 0.:
+            raise ValueError('max_grad_norm must be positive')
+        self.max_grad_norm, self.seed, self.grad_norm = max_grad_norm, int(seed), None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def _state_of(self, p, bits):
+        state = self.state[p]
+        if not state:
+            state['step'] = torch.zeros((), dtype=torch.float32, device=p.device)
+            for name, dtype in zip(('exp_avg', 'exp_avg_sq'), ops.MOMENT_DTYPES):
+                state[name] = torch.zeros_like(p, dtype=torch.float32) if bits == 32 else torch.zeros_like(p, dtype=torch.uint8).view(dtype)
+            if bits == 8:
+                state['scales'] = torch.zeros(((p.numel() + ops.ADAMW_BLOCK - 1) // ops.ADAMW_BLOCK, 2), dtype=torch.float32, device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls = []
+        for gi, group in enumerate(self.param_groups):
+            ps = [p for p in group['params'] if p.grad is not None]
+            for p in ps:
+                if not p.is_cuda or p.grad.is_sparse:
+                    raise _lib.IgcnError('AdamW takes parameters on the GPU with dense gradients')
+            gs = [p.grad if ops._same_order(p, p.grad) else torch.empty_like(p, dtype=p.grad.dtype).copy_(p.grad) for p in ps]
+            if ps:
+                calls.append((gi, group, ps, gs))
+        norm = None
+        if self.max_grad_norm is not None and len(calls) > 1:              # one norm over all groups
+            norm = ops.grad_norm([g for call in calls for g in call[3]])
+        for gi, group, ps, gs in calls:
+            states = [self._state_of(p, group['state_bits']) for p in ps]
+            got = ops.adamw_step(ps, gs, [s['exp_avg'] for s in states], [s['exp_avg_sq'] for s in states], [s['step'] for s in states],
+                                 lr=group['lr'], betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'],
+                                 max_grad_norm=self.max_grad_norm, scales=[s['scales'] for s in states] if group['state_bits'] == 8 else None,
+                                 seed=self.seed + (gi << 32), grad_norm=norm)
+            self.grad_norm = got
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the state keeps its own types (torch's casts every floating state to its parameter's).  Takes the state of
+        torch.optim.AdamW too; a group's state_bits then follow from what the state holds."""
+        if any(g.get('amsgrad') or g.get('maximize') for g in state_dict['param_groups']):
+            raise ValueError('a state with amsgrad or maximize is another optimizer\'s')
+        super().load_state_dict(state_dict)
+        for saved, group in zip(state_dict['param_groups'], self.param_groups):
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+            held = {8 if 'scales' in state_dict['state'][i] else 32 for i in saved['params'] if i in state_dict['state']}
+            if len(held) > 1:
+                raise ValueError('a group holds its moments in one form')
+            group['state_bits'] = held.pop() if held else group['state_bits']
+        saved = [i for g in state_dict['param_groups'] for i in g['params']]
+        mine = [p for g in self.param_groups for p in g['params']]
+        for i, p in zip(saved, mine):
+            for name, value in state_dict['state'].get(i, {}).items():
+                if name == 'step':
+                    value = torch.as_tensor(value, dtype=torch.float32).reshape(())
+                if torch.is_tensor(value):
+                    self.state[p][name] = value.to(device=p.device, copy=True)

@@ -28,6 +28,7 @@ from torch.optim import SGD, Adam  # noqa: F401  (resolved by name, trainer.py:4
 from . import ops
 from ._lib import MAX_METRIC_CUTS, MAX_TOPK
 from .dataset import AuxiliaryDataset
+from .optim import AdamW
 
 
 def get_trainer(config, dataset, model):
@@ -177,6 +178,8 @@ class BasicTrainer:
             kw['fused'] = True             # same update rule, one kernel over all parameters
             if self.config.get('hip_graph', True):
                 kw['capturable'] = True    # the step count lives on the device, so the step can sit in a HIP graph
+        elif opt is AdamW:                 # the HIP step: its own settings under its own names
+            kw = {k: self.config[k] for k in ('betas', 'eps', 'weight_decay', 'state_bits', 'max_grad_norm', 'seed') if k in self.config}
         self.opt = opt(self.model.parameters(), lr=self.config['lr'], **kw)
 
     # ---- one optimisation step as ONE captured HIP graph (config key 'hip_graph', default True) -----------------
@@ -188,7 +191,7 @@ class BasicTrainer:
             return False
         if isinstance(self.opt, Adam):
             return all(g.get('capturable', False) for g in self.opt.param_groups)
-        return isinstance(self.opt, SGD)
+        return isinstance(self.opt, (SGD, AdamW))          # (AdamW counts its steps on the device)
 
     _tokens = iter(range(1, 1 << 62))
 
@@ -209,7 +212,9 @@ class BasicTrainer:
         m = self.model
         return (self._token(getattr(m, 'norm_adj', None)), self._token(getattr(m, 'feat_mat', None)), self._token(self.opt),
                 self.batch_size, getattr(m, 'dropout', None), bool(m.training), getattr(self, 'l2_reg', None),
-                getattr(self, 'aux_reg', None), tuple(float(g['lr']) for g in self.opt.param_groups))
+                getattr(self, 'aux_reg', None), tuple(float(g['lr']) for g in self.opt.param_groups)) + \
+            ((self.opt.max_grad_norm,) + tuple((*g['betas'], g['eps'], g['weight_decay']) for g in self.opt.param_groups)
+             if isinstance(self.opt, AdamW) else ())
 
     def _graph_step(self, inputs, loss_fn, kind='nodes'):
         """Replays the captured step on `inputs` (tensors copied into the static buffers the graph reads); captures

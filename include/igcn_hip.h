@@ -476,6 +476,55 @@ int igcn_owned_rows_scatter_add_f32(const int64_t *ids, int64_t n, int64_t n_use
                                     int64_t ilo, int64_t ihi, const float *g, int64_t ld_g, int32_t d,
                                     float *gu, int64_t ld_gu, float *gi, int64_t ld_gi, void *stream);
 
+/* ---- optimizer step and 8-bit rows (no counterpart in the reference, whose optimizer is torch's Adam, trainer.py:43-45, and whose
+ * dense score block is torch.mm over float32 tables, model.py:71, :122) ---- */
+#define IGCN_DTYPE_F32   0
+#define IGCN_DTYPE_BF16  1
+#define IGCN_DTYPE_F16   2
+#define IGCN_ADAMW_BLOCK 128        /* consecutive elements that share a scale in the 8-bit moments */
+#define IGCN_MAX_I8_DEPTH 131071    /* 131071 * 128 * 128 < 2^31: the longest sum of 8-bit products that int32 holds */
+
+/* One tensor of an optimizer step: n elements in any order that param, grad and both moments have in common. */
+typedef struct igcn_adamw_tensor {
+    void *param;                    /* rewritten; `dtype` */
+    const void *grad;               /* `grad_dtype`: that of param, or float32 */
+    void *exp_avg, *exp_avg_sq;     /* rewritten: float32, or (8-bit moments) e4m3 and e5m2 codes, one byte each */
+    float *scales;                  /* rewritten: [ceil(n / IGCN_ADAMW_BLOCK)][2] = (exp_avg's, exp_avg_sq's); float32 moments: not used */
+    float *step;                    /* one number: the steps taken so far; the call adds 1 */
+    int64_t n;
+    int32_t dtype, grad_dtype;      /* IGCN_DTYPE_* */
+} igcn_adamw_tensor;
+
+/* One AdamW step over n_tensors tensors (host array; the pointers in it are device pointers):
+ *   t = ++step;  g' = c g;  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * c = 1 (max_norm 0) or min(1, max_norm / (norm + 1e-6)) with norm = the L2 norm over the gradients of ALL tensors, which goes to
+ * *norm_out (device) — or is read from *norm_in where the caller has it (several calls clipped by one norm; norm_out is not used then).
+ * lr_dev: NULL, or a device float read instead of lr (a captured step whose rate changes).
+ * moment_bits 32: float32 moments.  8: a block of IGCN_ADAMW_BLOCK elements is held as e4m3 codes of m / s_m and e5m2 codes of v / s_v,
+ * s_m = max|m| / 448, s_v = max v / 57344, rounded stochastically with 16 bits of a hash of (seed, tensor's place in the list, step,
+ * element); v > 0 is never held as 0; a block below 2^-100 is held as zeros, one with a NaN or an infinity gets a NaN scale.
+ * The averages themselves are formed unrounded before the parameter is updated.
+ * workspace: igcn_adamw_workspace_bytes(...) bytes, 16-byte aligned; one call's own.  No two tensors of a call may overlap. */
+int64_t igcn_adamw_workspace_bytes(const igcn_adamw_tensor *tensors_host, int64_t n_tensors);
+int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, int32_t moment_bits, double lr, const float *lr_dev,
+                    double beta1, double beta2, double eps, double weight_decay, double max_norm, const float *norm_in, float *norm_out,
+                    uint64_t seed, void *workspace, void *stream);
+
+/* *norm (device) = the L2 norm over the grad of every tensor (n and grad_dtype are the only other fields read); workspace as above. */
+int igcn_grad_norm(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, float *norm, void *workspace, void *stream);
+
+/* Rows as 8-bit integers: scale[r] = max|x[r]| / 127, q[r, i] = x[r, i] / scale[r] to the nearest whole number (ties to even, decided
+ * exactly).  A row of zeros: scale 0, codes 0.  A row with a NaN or an infinity: scale NaN, codes 0.  x: `dtype`, leading dimension ldx. */
+int igcn_quantize_rows_i8(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int64_t k, int8_t *q, int64_t ldq, float *scale, void *stream);
+/* y[r, i] = q[r, i] * scale[r], rounded to `dtype` */
+int igcn_dequantize_rows_i8(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int64_t k, void *y, int32_t dtype, int64_t ldy, void *stream);
+
+/* y[m, n] = (sum_k a[m, k] b[n, k]) sa[m] sb[n] (+ bias[n]): a [m, k] and b [n, k] 8-bit integers (-128 ... 127) by rows, one scale a
+ * row of either, bias NULL or [n]; the sum is exact (k <= IGCN_MAX_I8_DEPTH), scaled in float32 and rounded once to `dtype`. */
+int igcn_matmul_i8(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias,
+                   int64_t m, int64_t n, int64_t k, void *y, int32_t dtype, int64_t ldy, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,225 @@
+"""Rows in 8-bit integers (ops.quantize_rows_i8 / dequantize_rows_i8) and their product (ops.matmul_i8 / linear_i8) on the GPU: codes
+and sums are exact, so codes are compared one by one and scores to the few float32 roundings behind the sum."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+U = 2.0 ** -24
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _rng(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _codes(shape, g, lo=-128):
+    return torch.randint(lo, 128, shape, device=DEV, generator=g, dtype=torch.int8)
+
+
+def _quantized(x):
+    """(codes, scales) from float64: the quotient of two float32 numbers, rounded to 64 bits, is never on the wrong side of a half."""
+    x = x.double()
+    s = (x.abs().amax(1) / 127).float() if x.shape[1] else torch.zeros(x.shape[0], device=x.device)
+    q = torch.round(x / torch.where(s > 0, s, 1.).double()[:, None]) * (s > 0)[:, None]
+    return q.clamp(-127, 127).to(torch.int8), s
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,k', [(1, 1), (3, 7), (5, 16), (64, 63), (65, 64), (1000, 64), (9, 65), (130, 128), (7, 255), (17, 256), (4, 1000),
+                                    (3, 1024), (2, 2049), (3, 8191), (2, 8192), (1, 70001), (0, 5), (4, 0)])
+def test_codes_and_scales_are_the_nearest(rows, k, dtype):
+    from igcn_cf_amd import ops
+    g = _rng(rows * 1000 + k)
+    x = (torch.randn(rows, k, device=DEV, generator=g) * torch.exp(2 * torch.randn(rows, 1, device=DEV, generator=g))).to(dtype)
+    if rows > 2 and k:
+        x[1] = 0                                                                       # a row of zeros
+        x[2] = x[2].abs().amax() * torch.arange(k, device=DEV).remainder(3).sub(1).to(dtype)      # -max, 0, max
+    q, s = ops.quantize_rows_i8(x)
+    want_q, want_s = _quantized(x)
+    assert q.dtype == torch.int8 and torch.equal(s, want_s) and torch.equal(q, want_q)
+    for out in DTYPES:
+        y = ops.dequantize_rows_i8(q, s, dtype=out)
+        assert y.dtype == out and torch.equal(y, (q.float() * s[:, None]).to(out))
+
+
+def test_ties_go_to_the_even_code_and_small_rows_keep_their_size():
+    """max 254 makes the scale exactly 2: odd values are halves.  Rows of the smallest magnitudes have scales of few digits (or 0, where
+    max / 127 is below float32): codes stay the nearest within -127 ... 127."""
+    from igcn_cf_amd import ops
+    x = torch.arange(-254., 255., device=DEV)[None, :]
+    q, s = ops.quantize_rows_i8(x)
+    assert float(s) == 2. and torch.equal(q[0].long(), torch.round(x[0] / 2).long())
+    for scale in (1e-30, 1e-37, 1e-38, 1e-40, 1e-42, 1e-44, 3e38):
+        x = (torch.linspace(-1, 1, 301, dtype=torch.float64, device=DEV) * scale).float()[None, :]
+        q, s = ops.quantize_rows_i8(x)
+        want_q, want_s = _quantized(x)
+        assert torch.equal(s, want_s) and torch.equal(q, want_q), scale
+
+
+def test_broken_rows_show_and_leave_the_others_alone():
+    from igcn_cf_amd import ops
+    x = torch.randn(6, 200, device=DEV, generator=_rng(1))
+    clean_q, clean_s = ops.quantize_rows_i8(x)
+    x[1, 150], x[3, 0], x[4, 199] = float('nan'), float('inf'), -float('inf')
+    q, s = ops.quantize_rows_i8(x)
+    assert torch.isnan(s).tolist() == [False, True, False, True, True, False] and not q[1].any() and not q[3:5].any()
+    for r in (0, 2, 5):
+        assert torch.equal(q[r], clean_q[r]) and s[r] == clean_s[r]
+    y = ops.linear_i8(x, clean_q, clean_s)
+    assert torch.isnan(y).all(1).tolist() == [False, True, False, True, True, False]
+
+
+def test_rows_apart_and_off_alignment():
+    """Leading dimensions other than the width, every second row, and rows that start at any byte."""
+    from igcn_cf_amd import ops
+    g = _rng(2)
+    for dtype in DTYPES:
+        big = torch.randn(50, 300, device=DEV, generator=g).to(dtype)
+        for x in (big[:, 3:260], big[::2, :64], big[1:, 1:130], big[7:8, 5:6]):
+            q, s = ops.quantize_rows_i8(x)
+            want_q, want_s = _quantized(x)
+            assert torch.equal(q, want_q) and torch.equal(s, want_s)
+    ca, cb = _codes((200, 400), g), _codes((300, 500), g)
+    sa, sb = torch.rand(200, device=DEV, generator=g), torch.rand(300, device=DEV, generator=g)
+    for off in (0, 1, 2, 3, 4, 8, 15):
+        for k in (1, 15, 16, 31, 64, 100, 129, 256, 380):
+            for step in (1, 3):
+                a, b = ca[::step, off:off + k], cb[off % 3::step, 2 * off:2 * off + k]
+                check(a, sa[:a.shape[0]], b, sb[:b.shape[0]])
+    y = ops.dequantize_rows_i8(ca[::3, 5:77], sa[:67])
+    assert torch.equal(y, ca[::3, 5:77].float() * sa[:67, None])
+
+
+def check(a, sa, b, sb, bias=None, dtype=torch.float32):
+    """matmul_i8 against 64 bits: the sum is exact, then it is rounded to float32, multiplied twice, and the bias added: 3 roundings of the
+    product and one of the result, and the output type's own."""
+    from igcn_cf_amd import ops
+    y = ops.matmul_i8(a, sa, b, sb, bias=bias, dtype=dtype)
+    assert y.dtype == dtype and y.shape == (a.shape[0], b.shape[0])
+    prod = (a.double() @ b.double().t()) * sa.double()[:, None] * sb.double()
+    want = prod if bias is None else prod + bias.double()
+    off = 3 * U * prod.abs() + U * want.abs()
+    half = 0. if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    off = off + half * (want.abs() + off) + (2.0 ** -25 if dtype == torch.float16 else 0.)
+    top = torch.finfo(dtype).max
+    want = torch.where(want.abs() > top, torch.sign(want) * float('inf'), want) if dtype == torch.float16 else want
+    same = torch.isinf(want) & (y.double() == want)
+    bad = ~(((y.double() - want).abs() <= off * (1 + 1e-6) + 1e-45) | same)
+    assert not bool(bad.any()), (tuple(a.shape), tuple(b.shape), dtype, int(bad.sum()), bad.nonzero()[:4].tolist())
+    return y
+
+
+SIZES = [(1, 1, 1), (1, 17, 64), (2, 33, 16), (3, 5, 48), (4, 100, 8), (5, 1000, 64), (8, 64, 1024), (13, 77, 129), (16, 129, 100), (17, 300, 64), (31, 31, 31),
+         (32, 200, 4096), (33, 65, 63), (48, 96, 256), (63, 1025, 64), (64, 64, 64), (65, 129, 100), (100, 4097, 128), (127, 127, 255), (128, 256, 512), (129, 257, 65),
+         (255, 255, 1000), (256, 512, 192), (257, 300, 515), (300, 700, 2048), (512, 512, 4096), (513, 1029, 333), (1, 5000, 8191), (7, 3001, 5000), (1000, 1, 777),
+         (0, 5, 3), (5, 0, 3), (6, 7, 0)]
+
+
+@pytest.mark.parametrize('m,n,k', SIZES)
+def test_products_of_all_sizes(m, n, k):
+    g = _rng(m * 31 + n * 7 + k)
+    a, b = _codes((m, k), g), _codes((n, k), g)
+    sa, sb = torch.exp(torch.randn(m, device=DEV, generator=g) - 5), torch.exp(torch.randn(n, device=DEV, generator=g) - 5)
+    bias = torch.randn(n, device=DEV, generator=g)
+    for dtype in DTYPES:
+        check(a, sa, b, sb, None, dtype)
+        check(a, sa, b, sb, bias, dtype)
+
+
+def test_the_longest_sums_and_the_largest_codes():
+    """131 071 products of -128 * -128 are 2 147 467 264 < 2^31; and sums past 2^24 are rounded once."""
+    from igcn_cf_amd import ops
+    for k in (131071, 65536, 40000):
+        for m in (1, 3, 40):
+            a = torch.full((m, k), -128, dtype=torch.int8, device=DEV)
+            b = torch.full((70, k), -128, dtype=torch.int8, device=DEV)
+            b[1::2] = 127
+            one = torch.ones(70, device=DEV)
+            y = check(a, one[:m], b, one)
+            assert float(y[0, 0]) == np.float32(k * 16384) and float(y[0, 1]) == np.float32(-k * 128 * 127)
+    with pytest.raises(ops._lib.IgcnError):
+        ops.matmul_i8(torch.zeros(1, 131072, dtype=torch.int8, device=DEV), torch.ones(1, device=DEV), torch.zeros(1, 131072, dtype=torch.int8, device=DEV), torch.ones(1, device=DEV))
+
+
+@pytest.mark.parametrize('m', [1, 3, 40])
+def test_offsets_past_32_bits(m):
+    """Rows behind the 2^31st byte of b, and outputs behind the 2^32nd byte of y."""
+    g = _rng(3)
+    k, n = 8192, 270000                                                                 # 2.2 GB of codes
+    a, b = _codes((m, k), g), torch.empty((n, k), dtype=torch.int8, device=DEV)
+    for r in range(0, n, 30000):
+        b[r:r + 30000] = _codes((30000, k), g)
+    sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+    from igcn_cf_amd import ops
+    y = ops.matmul_i8(a, sa, b, sb)
+    at = torch.cat([torch.arange(100, device=DEV), torch.arange(n - 9000, n, device=DEV)])
+    want = (a.double() @ b[at].double().t()) * sa.double()[:, None] * sb[at].double()
+    assert bool(((y[:, at].double() - want).abs() <= 4 * U * want.abs() * (1 + 1e-6)).all())
+    if m == 40:
+        del y, b
+        m, n, k = 40000, 30000, 16                                                      # 4.8 GB of scores
+        a, b = _codes((m, k), g), _codes((n, k), g)
+        sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+        y = ops.matmul_i8(a, sa, b, sb)
+        for rows in (slice(0, 64), slice(m - 64, m), slice(17890, 17900)):
+            want = (a[rows].double() @ b.double().t()) * sa[rows].double()[:, None] * sb.double()
+            assert bool(((y[rows].double() - want).abs() <= 4 * U * want.abs() * (1 + 1e-6)).all())
+
+
+@pytest.mark.parametrize('m,n,k,dtype', [(1, 1000, 64, torch.float32), (1, 700, 4096, torch.bfloat16), (4, 333, 8192, torch.float16), (16, 500, 100, torch.float32),
+                                         (20, 500, 1000, torch.bfloat16), (300, 400, 64, torch.float32), (2, 99, 131071, torch.float32), (3, 50, 7, torch.bfloat16)])
+def test_a_linear_is_its_two_parts_and_takes_the_inputs_type(m, n, k, dtype):
+    from igcn_cf_amd import ops
+    g = _rng(k)
+    x = torch.randn(m, k, device=DEV, generator=g).to(dtype)
+    b, sb = _codes((n, k), g), torch.rand(n, device=DEV, generator=g)
+    bias = torch.randn(n, device=DEV, generator=g)
+    q, s = _quantized(x)
+    for out in (None, *DTYPES):
+        y = ops.linear_i8(x, b, sb, bias=bias, dtype=out)
+        assert y.dtype == (out or dtype)
+        assert torch.equal(y, ops.matmul_i8(q, s, b, sb, bias=bias, dtype=out or dtype))
+    x[-1, -1] = float('nan')
+    if m > 1:
+        x[0] = 0
+    y = ops.linear_i8(x, b, sb, bias=bias)
+    assert bool(torch.isnan(y[-1]).all()) and (m == 1 or torch.equal(y[0], bias.to(dtype)))
+
+
+def test_captured_products_follow_new_inputs_and_streams_do_not_meet():
+    """One captured call replayed on changed inputs, twice captured calls replayed in turn, and eager calls on several streams at once."""
+    from igcn_cf_amd import ops
+    g = _rng(9)
+    for m, n, k in ((1, 2000, 4096), (4, 1000, 8192), (70, 300, 500), (300, 600, 256)):
+        x, b = torch.randn(m, k, device=DEV, generator=g), _codes((n, k), g)
+        sb = torch.rand(n, device=DEV, generator=g)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.linear_i8(x, b, sb)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs, outs = [], []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(ops.linear_i8(x, b, sb))
+            graphs.append(graph)
+        for rep in range(4):
+            x.copy_(torch.randn(m, k, device=DEV, generator=g))
+            want = ops.linear_i8(x, b, sb)
+            torch.cuda.synchronize()
+            for graph, out in zip(graphs, outs):
+                out.zero_()
+                graph.replay()
+            torch.cuda.synchronize()
+            for out in outs:
+                assert torch.equal(out, want)
+        streams, got = [torch.cuda.Stream() for _ in range(4)], []
+        torch.cuda.synchronize()
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([ops.linear_i8(x, b, sb) for _ in range(3)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for ys in got for y in ys)

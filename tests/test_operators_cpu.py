@@ -1,0 +1,130 @@
+"""What the optimizer step and the 8-bit operators refuse, without a GPU: the Python entry points on tensors they do not take, the C
+entry points by error code before anything is launched, and the plain forms the GPU tests rest on."""
+import array
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from igcn_cf_amd import _lib, ops
+from igcn_cf_amd.optim import AdamW
+from tests import adamw_oracle as A
+
+
+def test_python_entry_points_refuse_cpu_tensors_and_bad_settings():
+    p = torch.zeros(4, 4)
+    t = torch.zeros(())
+    for call in (lambda: ops.adamw_step([p], [p], [p.clone()], [p.clone()], [t], lr=1e-3), lambda: ops.grad_norm([p]), lambda: ops.quantize_rows_i8(p),
+                 lambda: ops.dequantize_rows_i8(p.to(torch.int8), t), lambda: ops.matmul_i8(p.to(torch.int8), t, p.to(torch.int8), t), lambda: ops.linear_i8(p, p, t),
+                 lambda: ops.adamw_step([p], [], [], [], [], lr=1e-3), lambda: ops.adamw_step([], [], [], [], [], lr=1e-3, max_grad_norm=0.),
+                 lambda: ops.adamw_step([], [], [], [], [], lr=-1.), lambda: ops.adamw_step([], [], [], [], [], lr=1e-3, betas=(0.9, 1.0))):
+        with pytest.raises(_lib.IgcnError):
+            call()
+    assert ops.adamw_step([], [], [], [], [], lr=1e-3) is None
+    w = torch.nn.Parameter(p)
+    for kw in (dict(lr=-1.), dict(betas=(1., 0.9)), dict(eps=-1.), dict(weight_decay=-1.), dict(state_bits=16), dict(max_grad_norm=0.)):
+        with pytest.raises(ValueError):
+            AdamW([w], **kw)
+    w.grad = torch.zeros(4, 4)
+    with pytest.raises(_lib.IgcnError):
+        AdamW([w]).step()
+
+
+def _table(count=1, **kw):
+    """igcn_adamw_tensor rows as int64 words; pointers that are aligned and never followed."""
+    f = dict(param=0x1000, grad=0x2000, m=0x3000, v=0x4000, scales=0x5000, step=0x6000, n=256, dtype=0, grad_dtype=0)
+    f.update(kw)
+    row = [f['param'], f['grad'], f['m'], f['v'], f['scales'], f['step'], f['n'], f['dtype'] | f['grad_dtype'] << 32]
+    return array.array('q', row * count)
+
+
+def test_the_c_step_and_norm_reject_bad_arguments_before_any_launch():
+    L = _lib.lib()
+
+    def step(t, n=1, bits=32, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, mx=0., ni=None, no=None, ws=0x100):
+        return L.igcn_adamw_step(t.buffer_info()[0] if t is not None else None, n, bits, lr, None, b1, b2, eps, wd, mx, ni, no, 0, ws, None)
+    assert step(None) == -1 and step(_table(), n=-1) == -2
+    assert step(_table(), bits=16) == -4
+    for kw in (dict(lr=-1.), dict(lr=float('nan')), dict(b1=1.), dict(b2=-0.1), dict(eps=-1.), dict(wd=-1.), dict(mx=-1.), dict(mx=float('nan'))):
+        assert step(_table(), **kw) == -4, kw
+    assert step(_table(), ws=None) == -1 and step(_table(), ws=0x104) == -3 and step(_table(), mx=1.) == -1 and step(_table(), mx=1., no=0x102) == -3
+    for kw in (dict(param=0), dict(grad=0), dict(m=0), dict(v=0), dict(step=0)):
+        assert step(_table(**kw)) == -1, kw
+    assert step(_table(scales=0), bits=8) == -1
+    assert step(_table(dtype=3)) == -4 and step(_table(dtype=0, grad_dtype=1)) == -4 and step(_table(dtype=1, grad_dtype=2)) == -4
+    for kw in (dict(param=0x1002), dict(grad=0x2001), dict(m=0x3002), dict(step=0x6002), dict(scales=0x5002), dict(dtype=1, param=0x1001, grad_dtype=1)):
+        assert step(_table(**kw)) == -3, kw
+    bad = _table()
+    bad[6] = -5
+    assert step(bad) == -2
+    assert L.igcn_adamw_workspace_bytes(bad.buffer_info()[0], 1) == -1
+    assert step(None, n=0) == 0                                                       # nothing to do
+    one, other, lots = _table(), _table(grad_dtype=7), _table(200)                    # (held: the calls get their addresses)
+    assert L.igcn_grad_norm(None, 0, None, 0x100, None) == -1 and L.igcn_grad_norm(one.buffer_info()[0], 1, 0x102, 0x100, None) == -3
+    assert L.igcn_grad_norm(other.buffer_info()[0], 1, 0x100, 0x100, None) == -4
+    few, many = L.igcn_adamw_workspace_bytes(one.buffer_info()[0], 1), L.igcn_adamw_workspace_bytes(lots.buffer_info()[0], 200)
+    assert 0 < few < many
+
+
+def test_the_struct_of_a_tensor_is_laid_out_as_the_binding_fills_it(tmp_path):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = ['param', 'grad', 'exp_avg', 'exp_avg_sq', 'scales', 'step', 'n', 'dtype', 'grad_dtype']
+    src = tmp_path / 'layout.c'
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "igcn_hip.h"\nint main(void) {\n'
+                   + ''.join('    printf("%%zu ", offsetof(igcn_adamw_tensor, %s));\n' % f for f in names)
+                   + '    printf("%zu %d %d\\n", sizeof(igcn_adamw_tensor), IGCN_ADAMW_BLOCK, IGCN_MAX_I8_DEPTH);\n    return 0;\n}\n')
+    subprocess.run(['gcc', '-std=c99', '-Wall', '-Werror', '-I', os.path.join(root, 'include'), str(src), '-o', str(tmp_path / 'layout')], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / 'layout')], check=True, stdout=subprocess.PIPE).stdout.split()]
+    assert got == [0, 8, 16, 24, 32, 40, 48, 56, 60, 64, ops.ADAMW_BLOCK, ops.MAX_I8_DEPTH]
+
+
+def test_the_c_8_bit_entry_points_reject_bad_arguments_before_any_launch():
+    L = _lib.lib()
+    P = 0x1000
+
+    def quantize(x=P, dtype=0, ldx=64, rows=4, k=64, q=P, ldq=64, s=P):
+        return L.igcn_quantize_rows_i8(x, dtype, ldx, rows, k, q, ldq, s, None)
+
+    def back(q=P, ldq=64, s=P, rows=4, k=64, y=P, dtype=0, ldy=64):
+        return L.igcn_dequantize_rows_i8(q, ldq, s, rows, k, y, dtype, ldy, None)
+
+    def product(a=P, lda=64, sa=P, b=P, ldb=64, sb=P, bias=None, m=4, n=8, k=64, y=P, dtype=0, ldy=8):
+        return L.igcn_matmul_i8(a, lda, sa, b, ldb, sb, bias, m, n, k, y, dtype, ldy, None)
+    assert quantize(dtype=5) == -4 and quantize(rows=-1) == -2 and quantize(ldx=63) == -2 and quantize(ldq=1) == -2 and quantize(k=-1) == -2
+    assert quantize(x=None) == -1 and quantize(q=None) == -1 and quantize(s=None) == -1 and quantize(x=0x1002) == -3 and quantize(x=0x1001, dtype=1) == -3 and quantize(s=0x1001) == -3
+    assert quantize(rows=0, x=None) == 0
+    assert back(dtype=-1) == -4 and back(ldy=3) == -2 and back(q=None) == -1 and back(s=None) == -1 and back(y=None) == -1 and back(y=0x1002) == -3 and back(k=0, q=None) == 0
+    assert product(dtype=3) == -4 and product(m=-1) == -2 and product(lda=1) == -2 and product(ldb=1) == -2 and product(ldy=7) == -2
+    assert product(k=131072, lda=1 << 20, ldb=1 << 20) == -4
+    for kw in (dict(a=None), dict(b=None), dict(sa=None), dict(sb=None), dict(y=None)):
+        assert product(**kw) == -1, kw
+    assert product(y=0x1002) == -3 and product(sa=0x1002) == -3 and product(bias=0x1001) == -3 and product(m=0, a=None) == 0 and product(n=0, ldy=0) == 0
+
+
+def test_the_plain_codes_are_those_torch_reads_and_round_both_ways():
+    """decode() against torch's own float8 types over all finite codes; encode() with u just under 1 and just over 0 gives the neighbours."""
+    codes = np.arange(256, dtype=np.uint8)
+    for dtype, mantissa, bias in ((torch.float8_e4m3fn, 3, 7), (torch.float8_e5m2, 2, 15)):
+        want = torch.from_numpy(codes).view(dtype).float().numpy()
+        fine = np.isfinite(want)
+        assert np.array_equal(A.decode(codes, mantissa, bias)[fine], want[fine]) and fine.sum() >= 248
+    x = np.abs(np.random.default_rng(0).standard_normal(1280)).astype(np.float32)
+    x[::128] = 10.
+    low, s, _ = A.encode(x, np.zeros(1280, np.int64), 3, 7, 448.)
+    high, _, _ = A.encode(x, np.full(1280, 65535), 3, 7, 448.)
+    scale = np.repeat(s, 128).astype(np.float64)
+    down, up = (A.decode(c.astype(np.uint8), 3, 7) * scale for c in (low, high))
+    assert (down <= x * (1 + 1e-6)).all() and (up >= x * (1 - 1e-6)).all() and ((high - low) <= 1).all() and (high[::128] == 126).all()
+    assert len({int(h) for h in A.hashes(1000, 7, 0, 1)}) > 990 and not np.array_equal(A.hashes(8, 7, 0, 1), A.hashes(8, 7, 1, 1))
+
+
+def test_dense_orders_are_told_from_views_with_gaps():
+    x = torch.zeros(6, 8, 10)
+    for t in (x, x.transpose(0, 2), x[2], x[:, :1].squeeze(1)[1], x.reshape(-1)[3:7], torch.zeros(()), torch.zeros(0, 3)):
+        assert ops._dense(t)
+    for t in (x[:, 1], x[..., :3], x[::2], torch.zeros(1).expand(5)):
+        assert not ops._dense(t)
+    assert ops._same_order(x.transpose(0, 1), torch.empty_like(x.transpose(0, 1))) and not ops._same_order(x.transpose(0, 2), torch.zeros(10, 8, 6))

@@ -1,0 +1,452 @@
+"""The AdamW step over many tensors (ops.adamw_step, ops.grad_norm, optim.AdamW) on the GPU against the step in 64 bits, and the
+8-bit moments bit for bit against elementary float32 operations."""
+import numpy as np
+import pytest
+import torch
+
+from tests import adamw_oracle as A
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+HYPER = dict(lr=3e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+HALF_STEP = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+
+
+def _grads(shape, rng, dtype=torch.float32):
+    size = np.exp(1.5 * rng.standard_normal((shape[0],) + (1,) * (len(shape) - 1)) - 4) if shape else 0.1
+    return torch.from_numpy(np.asarray(size * rng.standard_normal(shape), dtype=np.float32)).to(DEV).to(dtype)
+
+
+def _params(shape, rng, dtype=torch.float32):
+    return torch.from_numpy(np.asarray(0.1 * rng.standard_normal(shape), dtype=np.float32)).to(DEV).to(dtype)
+
+
+def _zeros8(p):
+    n = -(-p.numel() // 128)
+    return (torch.zeros_like(p, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros_like(p, dtype=torch.uint8).view(torch.float8_e5m2),
+            torch.zeros(n, 2, device=DEV))
+
+
+def _flat(t):
+    """numpy values of t in memory order (uint8 for 8-bit codes, float64 else)."""
+    t = t.detach()
+    if t.dtype in (torch.float8_e4m3fn, torch.float8_e5m2):
+        t = t.view(torch.uint8)
+    if t.dim() and not t.is_contiguous():
+        order = sorted(range(t.dim()), key=lambda d: -t.stride(d))
+        t = t.permute(order)
+    a = t.cpu()
+    return (a.numpy() if a.dtype == torch.uint8 else a.double().numpy()).reshape(-1)
+
+
+def _check32(p0, g, m0, v0, t, p1, m1, v1, factor=1.0, hyper=HYPER):
+    e = A.step64(_flat(p0), _flat(g), _flat(m0), _flat(v0), t, hyper['lr'], *hyper['betas'], hyper['eps'], hyper['weight_decay'], factor)
+    half = HALF_STEP[p1.dtype]
+    tiny = 2.0 ** -25 if p1.dtype == torch.float16 else 0.                       # half of fp16's smallest step
+    assert (np.abs(_flat(p1) - e[0]) <= e[3] + half * (np.abs(e[0]) + e[3]) + tiny).all()
+    assert (np.abs(_flat(m1) - e[1]) <= e[4]).all() and (np.abs(_flat(v1) - e[2]) <= e[5]).all()
+
+
+SHAPES = [[(1,)], [(7,), (8,), (9,)], [(127,), (128, 1), (3, 43)], [(2047,), (2048,), (2049,), (5, 1000)], [(), (0, 4), (300, 64), (1,)]]
+
+
+@pytest.mark.parametrize('dtype,grad_dtype', [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                              (torch.float16, torch.float16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize('shapes', range(len(SHAPES)))
+def test_float32_moments_follow_the_step_in_64_bits(shapes, dtype, grad_dtype):
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(shapes)
+    ps = [_params(s, rng, dtype) for s in SHAPES[shapes]]
+    ms, vs = [torch.zeros_like(p, dtype=torch.float32) for p in ps], [torch.zeros_like(p, dtype=torch.float32) for p in ps]
+    ts = [torch.full((), float(i), device=DEV) for i in range(len(ps))]            # every tensor counts its own steps
+    for step in range(1, 4):
+        gs = [_grads(s, rng, grad_dtype) for s in SHAPES[shapes]]
+        before = [(p.clone(), m.clone(), v.clone()) for p, m, v in zip(ps, ms, vs)]
+        assert ops.adamw_step(ps, gs, ms, vs, ts, **HYPER) is None
+        for i, (p0, m0, v0) in enumerate(before):
+            assert float(ts[i]) == i + step
+            _check32(p0, gs[i], m0, v0, i + step, ps[i], ms[i], vs[i])
+
+
+@pytest.mark.parametrize('shapes', range(len(SHAPES)))
+@pytest.mark.parametrize('dtype,clip', [(torch.float32, False), (torch.float32, True), (torch.bfloat16, True), (torch.float16, False)])
+def test_8_bit_moments_meet_the_elementary_operations_bit_for_bit(shapes, dtype, clip):
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(100 + shapes)
+    seed = 0x1234567890abcdef
+    ps = [_params(s, rng, dtype) for s in SHAPES[shapes]]
+    state = [_zeros8(p) for p in ps]
+    ts = [torch.zeros((), device=DEV) for _ in ps]
+    b1, b2 = HYPER['betas']
+    for step in range(1, 5):
+        gs = [_grads(s, rng, dtype) for s in SHAPES[shapes]]
+        before = [(p.clone(), _flat(m), _flat(v), s.cpu().numpy()) for p, (m, v, s) in zip(ps, state)]
+        norm = ops.adamw_step(ps, gs, [s[0] for s in state], [s[1] for s in state], ts, scales=[s[2] for s in state], seed=seed,
+                              max_grad_norm=0.05 if clip else None, **HYPER)
+        factor = np.float32(min(1.0, 0.05 / (float(np.sqrt(sum((_flat(g) ** 2).sum() for g in gs))) + 1e-6))) if clip else np.float32(1)
+        assert (norm is not None) == clip
+        for i, (p0, mc0, vc0, s0) in enumerate(before):
+            mc, vc, sc, m, v = A.moments8(_flat(gs[i]).astype(np.float32), mc0, vc0, s0, factor, b1, b2, seed, i, step)
+            assert np.array_equal(_flat(state[i][0]), mc) and np.array_equal(_flat(state[i][1]), vc)
+            assert np.array_equal(state[i][2].cpu().numpy(), sc)
+            m0, v0 = (A.decode(c, k, b).astype(np.float64) * np.repeat(s0[:, j], 128)[:c.size] for j, (c, k, b) in enumerate(((mc0, 3, 7), (vc0, 2, 15))))
+            e = A.step64(_flat(p0), _flat(gs[i]), m0, v0, step, HYPER['lr'], b1, b2, HYPER['eps'], HYPER['weight_decay'], float(factor))
+            assert (np.abs(_flat(ps[i]) - e[0]) <= e[3] + HALF_STEP[dtype] * (np.abs(e[0]) + e[3]) + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
+            # what is held is within one code step of the average: 1/8 of its size (e4m3), 1/4 (e5m2), or the smallest step of the block
+            held_m = A.decode(mc, 3, 7).astype(np.float64) * np.repeat(sc[:, 0], 128)[:mc.size]
+            held_v = A.decode(vc, 2, 15).astype(np.float64) * np.repeat(sc[:, 1], 128)[:vc.size]
+            assert (np.abs(held_m - m) <= np.abs(m) / 8 * (1 + 1e-6) + np.repeat(sc[:, 0], 128)[:mc.size] * 2.0 ** -9).all()
+            assert (np.abs(held_v - v) <= v / 4 * (1 + 1e-6) + np.repeat(sc[:, 1], 128)[:vc.size] * 2.0 ** -16).all()
+            assert ((vc > 0) == (v * np.repeat(sc[:, 1] > 0, 128)[:v.size] > 0)).all()
+
+
+def test_torch_reads_the_codes_as_the_moments_they_stand_for():
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(5)
+    p, g = _params((33, 40), rng), _grads((33, 40), rng)
+    m8, v8, s = _zeros8(p)
+    ops.adamw_step([p], [g], [m8], [v8], [torch.zeros((), device=DEV)], scales=[s], **HYPER)
+    for t, k, b in ((m8, 3, 7), (v8, 2, 15)):
+        assert np.array_equal(t.float().cpu().numpy().reshape(-1), A.decode(t.view(torch.uint8).cpu().numpy().reshape(-1), k, b))
+
+
+def test_stochastic_rounding_is_right_in_the_mean_and_does_not_freeze_the_average():
+    """4 096 seeds round the same averages: the mean of what is held is off by at most 6 standard deviations of such a mean (a rounding
+    to one of two neighbours a step apart varies by at most half a step).  And a second moment that has to rise a thousandfold at 0.1 %
+    of its target a step gets there: rounded to nearest, a step under an eighth of its size would leave it where it was."""
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(6)
+    g = _grads((128,), rng)
+    mean = [0., 0.]
+    n = 4096
+    for seed in range(n):
+        p = torch.zeros(128, device=DEV)
+        m8, v8, s = _zeros8(p)
+        ops.adamw_step([p], [g], [m8], [v8], [torch.zeros((), device=DEV)], scales=[s], seed=seed * 0x9e3779b97f4a7c15, **HYPER)
+        mean[0] = mean[0] + m8.double() * s[0, 0].double() / n
+        mean[1] = mean[1] + v8.double() * s[0, 1].double() / n
+    true = (0.1 * g.double(), 0.001 * g.double() ** 2)
+    for got, want, part, scale, small in zip(mean, true, (8, 4), s[0].double(), (2.0 ** -9, 2.0 ** -16)):
+        step = torch.maximum(want.abs() / part, scale * small)
+        some = want.abs() > 2 * scale * small                                        # (a second moment under the smallest code is held as that code)
+        assert bool(((got - want).abs() <= 6 * step / 2 / n ** 0.5 + 1e-6 * want.abs())[some].all())
+    p = torch.zeros(256, device=DEV)
+    m8, v8, s = _zeros8(p)
+    t = torch.zeros((), device=DEV)
+    small, large = torch.full((256,), 1e-3, device=DEV), torch.full((256,), 1e-3, device=DEV)
+    small[::128] = large[::128] = 1e-1                                               # one large value in each block sets its scale
+    large[1::2] = 3e-2
+    for k in range(6000):
+        ops.adamw_step([p], [small if k < 1000 else large], [m8], [v8], [t], scales=[s], lr=0.)
+    v = (v8.float() * s[:, 1].repeat_interleave(128)).double()
+    want = 9e-4 * (1 - 0.999 ** 5000)
+    # a step moves v by at most 0.1 %, so it lands on the next code (a quarter off at most) with a chance of 0.001 / 0.25 at least: a walk of
+    # variance 0.001 * 0.25 a step, pulled back over 1 000 steps: 0.125, 35 % of v; the mean of 128 such values is within 0.16 (5 sigma)
+    assert abs(float(v[1::2].mean()) / want - 1) < 0.16 and float(v[1::2].min()) > want / 4
+
+
+@pytest.mark.parametrize('eight', [False, True])
+def test_orders_offsets_and_many_tensors(eight):
+    """Transposed parameters (dense, not contiguous), views that start off any alignment, and more tensors than one launch takes give
+    what contiguous, aligned, single calls give."""
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(7)
+    shapes = [((i * 37) % 311 + 1, i % 5 + 1) for i in range(130)]
+    base = [_params((s[0] * s[1] + 3,), rng) for s in shapes]
+    gbase = [_grads((s[0] * s[1] + 3,), rng) for s in shapes]
+    view = [(lambda b, s, o, tr: b[o:o + s[0] * s[1]].view(s[::-1]).t() if tr else b[o:o + s[0] * s[1]].view(s)) for _ in shapes]
+    ps = [f(b, s, i % 4 and 1, i % 3 == 0) for i, (f, b, s) in enumerate(zip(view, [b.clone() for b in base], shapes))]
+    gs = [f(b, s, (i + 1) % 3, i % 3 == 0) for i, (f, b, s) in enumerate(zip(view, gbase, shapes))]
+    if eight:
+        st = [_zeros8(p) for p in ps]
+        ms, vs, sc = [s[0] for s in st], [s[1] for s in st], [s[2] for s in st]
+    else:
+        ms, vs, sc = [torch.zeros_like(p) for p in ps], [torch.zeros_like(p) for p in ps], None
+    ts = [torch.zeros(1, device=DEV) for _ in ps]
+    p0 = [p.clone() for p in ps]
+    norm = ops.adamw_step(ps, gs, ms, vs, ts, scales=sc, max_grad_norm=0.5, seed=3, **HYPER)
+    factor = min(1.0, 0.5 / (float(np.sqrt(sum((_flat(g) ** 2).sum() for g in gs))) + 1e-6))
+    assert abs(float(norm) - float(np.sqrt(sum((_flat(g) ** 2).sum() for g in gs)))) <= 2.0 ** -23 * float(norm)
+    for i in range(len(ps)):
+        n = ps[i].numel()
+        e = A.step64(_flat(p0[i]), _flat(gs[i]), np.zeros(n), np.zeros(n), 1, HYPER['lr'], *HYPER['betas'], HYPER['eps'], HYPER['weight_decay'], factor)
+        assert (np.abs(_flat(ps[i]) - e[0]) <= e[3] + 2.0 ** -24 * np.abs(e[0])).all(), i
+        if eight:
+            mc, vc, s, _, _ = A.moments8(_flat(gs[i]).astype(np.float32), np.zeros(n, np.uint8), np.zeros(n, np.uint8), np.zeros((-(-n // 128), 2), np.float32),
+                                         np.float32(factor), 0.9, 0.999, 3, i, 1)
+            assert np.array_equal(_flat(ms[i]), mc) and np.array_equal(_flat(vs[i]), vc) and np.array_equal(sc[i].cpu().numpy(), s), i
+        else:
+            assert (np.abs(_flat(ms[i]) - e[1]) <= e[4]).all() and (np.abs(_flat(vs[i]) - e[2]) <= e[5]).all(), i
+    for i, b in enumerate(base):                                                     # nothing outside a view is touched
+        whole = ps[i]._base if ps[i]._base is not None else ps[i]
+        o, n = i % 4 and 1, ps[i].numel()
+        assert torch.equal(whole[:o], b[:o]) and torch.equal(whole[o + n:], b[o + n:])
+
+
+def test_norm_over_many_tensors_and_clipping_by_a_given_one():
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(8)
+    for dtypes in ((torch.float32,), (torch.float32, torch.bfloat16, torch.float16)):
+        gs = [_grads(s, rng, dtypes[i % len(dtypes)]) for i, s in enumerate([(1,), (0, 3), (1000003,), (64, 129), ()] * 30)]
+        want = float(np.sqrt(sum((_flat(g) ** 2).sum() for g in gs)))
+        got = ops.grad_norm(gs)
+        assert got.dtype == torch.float32 and got.dim() == 0 and abs(float(got) - want) <= 2.0 ** -23 * want
+        assert torch.equal(ops.grad_norm(gs), got)                                   # same order every time
+    assert float(ops.grad_norm([])) == 0. and float(ops.grad_norm([torch.empty(0, device=DEV)])) == 0.
+    assert not np.isfinite(float(ops.grad_norm([torch.tensor([1., float('nan')], device=DEV)])))
+    p0, g = _params((5, 77), rng), _grads((5, 77), rng)
+    out = []
+    for norm in (None, torch.full((), 4.0, device=DEV)):
+        p, m, v = p0.clone(), torch.zeros_like(p0), torch.zeros_like(p0)
+        got = ops.adamw_step([p], [g], [m], [v], [torch.zeros((), device=DEV)], max_grad_norm=1e-3, grad_norm=norm, **HYPER)
+        assert norm is None or got is norm
+        _check32(p0, g, torch.zeros_like(p0), torch.zeros_like(p0), 1, p, m, v, factor=1e-3 / (float(got) + 1e-6))
+        out.append(m)
+    assert not torch.equal(*out)
+
+
+@pytest.mark.parametrize('eight', [False, True])
+def test_zero_huge_and_broken_gradients(eight):
+    """All-zero gradients from zero moments move nothing but the decay; a NaN or an infinity shows in its own parameter at once and, with
+    8-bit moments, as a NaN scale of its block — never in another block; gradients whose squares leave the codes' range are held as zero."""
+    from igcn_cf_amd import ops
+    for case in ('zero', 'tiny', 'nan', 'inf'):
+        p0 = torch.linspace(-1, 1, 400, device=DEV)
+        g = torch.zeros(400, device=DEV)
+        if case == 'tiny':
+            g.fill_(1e-20)
+        elif case != 'zero':
+            g.fill_(0.01)
+            g[130] = float(case)
+        p = p0.clone()
+        m, v, s = _zeros8(p) if eight else (torch.zeros_like(p), torch.zeros_like(p), None)
+        ops.adamw_step([p], [g], [m], [v], [torch.zeros((), device=DEV)], scales=[s] if eight else None, **HYPER)
+        if case in ('zero', 'tiny'):
+            keep = p0.double() * (1 - HYPER['lr'] * HYPER['weight_decay'])
+            assert bool(((p.double() - keep).abs() <= 4 * 2.0 ** -24 * p0.abs().double() + 1e-13).all())        # (1e-20 / eps * lr / 0.1)
+            if eight:
+                assert not v.view(torch.uint8).any() and bool((s[:, 1] == 0).all())
+                assert case == 'tiny' or not s.any()
+        else:
+            broken = ~torch.isfinite(p)
+            assert broken.nonzero().flatten().tolist() == [130]
+            if eight:
+                assert torch.isnan(s).all(1).tolist() == [False, True, False, False] and not m.view(torch.uint8)[128:256].any()
+
+
+def test_captured_steps_follow_the_eager_ones():
+    """A captured step (clipped, 8-bit and float32 moments, a device learning rate) replayed with the program's own work between replays
+    gives what eager calls give, bit for bit; its steps go on counting."""
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(9)
+    p0 = [_params((300, 64), rng), _params((1000,), rng)]
+    grads = [[_grads((300, 64), rng), _grads((1000,), rng)] for _ in range(6)]
+    for eight in (False, True):
+        ends = []
+        for captured in (False, True):
+            ps = [p.clone() for p in p0]
+            st = [_zeros8(p) if eight else (torch.zeros_like(p), torch.zeros_like(p), None) for p in ps]
+            ts, lr = [torch.zeros((), device=DEV) for _ in ps], torch.full((1,), 1e-2, device=DEV)
+            gs = [g.clone() for g in grads[0]]
+            run = lambda: ops.adamw_step(ps, gs, [s[0] for s in st], [s[1] for s in st], ts, lr=lr, weight_decay=0.01, max_grad_norm=0.1,
+                                         scales=[s[2] for s in st] if eight else None, seed=11)
+            if captured:
+                saved = [[t.clone() for t in (*ps, *ts, *(x for s in st for x in s if x is not None))]]
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    run()
+                torch.cuda.current_stream().wait_stream(side)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    norm = run()
+                for t, o in zip((*ps, *ts, *(x for s in st for x in s if x is not None)), saved[0]):
+                    t.copy_(o)
+            norms = []
+            for k in range(6):
+                for a, b in zip(gs, grads[k]):
+                    a.copy_(b)
+                lr.fill_(1e-2 / (k + 1))
+                if captured:
+                    graph.replay()
+                else:
+                    norm = run()
+                norms.append(float(norm))
+                junk = torch.randn(1 << 16, device=DEV).square().sum()                # the program's own work, and a wait for it
+                torch.cuda.synchronize()
+            assert all(float(t) == 6 for t in ts)
+            ends.append([norms] + [_flat(t) for t in (*ps, *(x for s in st for x in s if x is not None))])
+        assert ends[0][0] == ends[1][0]
+        for a, b in zip(ends[0][1:], ends[1][1:]):
+            assert np.array_equal(a, b)
+
+
+def test_a_step_on_another_stream_and_two_at_once():
+    from igcn_cf_amd import ops
+    rng = np.random.default_rng(10)
+    sets = []
+    for _ in range(4):
+        p, g = _params((200003,), rng), _grads((200003,), rng)
+        sets.append((p, g, _zeros8(p), torch.zeros((), device=DEV)))
+    want = []
+    for p, g, (m, v, s), t in sets:
+        q, st, tt = p.clone(), _zeros8(p), t.clone()
+        for _ in range(3):
+            ops.adamw_step([q], [g], [st[0]], [st[1]], [tt], scales=[st[2]], max_grad_norm=1.0, **HYPER)
+        want.append((q, *st))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        for stream, (p, g, (m, v, s), t) in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                ops.adamw_step([p], [g], [m], [v], [t], scales=[s], max_grad_norm=1.0, **HYPER)
+    torch.cuda.synchronize()
+    for (p, g, (m, v, s), t), w in zip(sets, want):
+        assert torch.equal(p, w[0]) and torch.equal(m.view(torch.uint8), w[1].view(torch.uint8)) and torch.equal(v.view(torch.uint8), w[2].view(torch.uint8)) and torch.equal(s, w[3])
+
+
+# ---- the optimizer -----------------------------------------------------------------------------------------------------------------
+def _model(seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(40, 64), torch.nn.Tanh(), torch.nn.Linear(64, 30)).to(DEV)
+
+
+def _loss(model, k):
+    x = torch.randn(50, 40, generator=torch.Generator().manual_seed(k)).to(DEV)
+    return model(x).square().mean()
+
+
+def test_optimizer_follows_the_formula_and_takes_another_adamws_state():
+    """Against the step in 64 bits, fed the same gradients; and a run continued from a state_dict — torch's own AdamW's among them —
+    goes on as the one it was taken from (float32 moments to one rounding a step of each: 1e-6 over 5 steps)."""
+    from igcn_cf_amd.optim import AdamW
+    model, other = _model(), _model()
+    ours = AdamW(model.parameters(), **HYPER, max_grad_norm=0.05)
+    theirs = torch.optim.AdamW(other.parameters(), **HYPER)
+    for k in range(5):
+        for m, o in ((model, ours), (other, theirs)):
+            o.zero_grad()
+            _loss(m, k).backward()
+        want = torch.nn.utils.clip_grad_norm_(other.parameters(), 0.05)
+        ours.step()
+        theirs.step()
+        assert abs(float(ours.grad_norm) / float(want) - 1) < 1e-5
+    for a, b in zip(model.parameters(), other.parameters()):
+        assert float((a - b).detach().abs().max()) < 1e-5 * 5
+    third = _model()
+    third.load_state_dict(other.state_dict())
+    cont = AdamW(third.parameters(), **HYPER)
+    cont.load_state_dict(theirs.state_dict())
+    for k in range(5, 10):
+        for m, o in ((third, cont), (other, theirs)):
+            o.zero_grad()
+            _loss(m, k).backward()
+            o.step()
+    for a, b in zip(third.parameters(), other.parameters()):
+        assert float((a - b).detach().abs().max()) < 1e-4
+    assert all(float(cont.state[p]['step']) == 10 for p in third.parameters())
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_a_saved_optimizer_goes_on_bit_for_bit(bits, tmp_path):
+    from igcn_cf_amd.optim import AdamW
+    model = _model().to(torch.bfloat16)
+    groups = [{'params': [model[0].weight, model[0].bias]}, {'params': [model[2].weight, model[2].bias], 'lr': 1e-2, 'weight_decay': 0.}]
+    opt = AdamW(groups, **HYPER, state_bits=bits, max_grad_norm=0.1, seed=5)
+
+    def go(m, o, ks):
+        for k in ks:
+            o.zero_grad()
+            x = torch.randn(50, 40, generator=torch.Generator().manual_seed(k)).to(DEV).to(torch.bfloat16)
+            m(x).float().square().mean().backward()
+            o.step()
+    go(model, opt, range(3))
+    torch.save({'model': model.state_dict(), 'opt': opt.state_dict()}, tmp_path / 'c.pt')
+    saved = torch.load(tmp_path / 'c.pt', map_location=DEV, weights_only=True)
+    again = _model(3).to(torch.bfloat16)
+    again.load_state_dict(saved['model'])
+    opt2 = AdamW([{'params': [again[0].weight, again[0].bias]}, {'params': [again[2].weight, again[2].bias]}], **HYPER, state_bits=bits, max_grad_norm=0.1, seed=5)
+    opt2.load_state_dict(saved['opt'])
+    for p, q in zip((q for g in opt.param_groups for q in g['params']), (q for g in opt2.param_groups for q in g['params'])):
+        for name, value in opt.state[p].items():
+            assert opt2.state[q][name].dtype == value.dtype and np.array_equal(_flat(opt2.state[q][name]), _flat(value))
+        assert bits == 32 or opt.state[p]['exp_avg'].dtype == torch.float8_e4m3fn
+    go(model, opt, range(3, 6))
+    go(again, opt2, range(3, 6))
+    for a, b in zip(model.parameters(), again.parameters()):
+        assert torch.equal(a, b)
+    size = sum(t.numel() * t.element_size() for p in model.parameters() for n, t in opt.state[p].items() if n != 'step')
+    assert bits == 32 or size <= sum(2 * p.numel() + 8 * (p.numel() // 128 + 1) for p in model.parameters())
+
+
+def test_parameters_without_gradient_and_gradients_in_another_order():
+    from igcn_cf_amd.optim import AdamW
+    a, b, c = (torch.nn.Parameter(torch.ones(6, 5, device=DEV)) for _ in range(3))
+    opt = AdamW([a, b, c], lr=0.1, weight_decay=0.)
+    a.grad = torch.arange(30., device=DEV).view(5, 6).t() + 1                         # transposed in memory
+    c.grad = torch.ones(6, 5, device=DEV)
+    version = a._version
+    opt.step()
+    assert a._version > version and torch.equal(b, torch.ones_like(b)) and not opt.state[b]
+    assert torch.allclose(a, torch.full_like(a, 0.9), atol=1e-6) and torch.equal(opt.state[a]['exp_avg'].argmax(), a.grad.contiguous().argmax())
+    opt.step(closure=lambda: None)
+    assert float(opt.state[a]['step']) == 2
+
+
+# ---- the trainers ------------------------------------------------------------------------------------------------------------------
+def _trainer(name, hip_graph, bits, **kw):
+    from igcn_cf_amd.dataset import SyntheticDataset
+    from igcn_cf_amd.model import get_model
+    from igcn_cf_amd.trainer import get_trainer
+    torch.manual_seed(1)
+    ds = SyntheticDataset({'name': 'SyntheticDataset', 'n_users': 600, 'n_items': 400, 'n_inter': 12000, 'device': DEV, 'seed': 3})
+    model = get_model({'name': name, 'embedding_size': 64, 'n_layers': 2, 'dropout': 0.1, 'feature_ratio': 1., 'device': DEV}, ds)
+    cfg = {'name': 'IGCNTrainer' if name == 'IGCN' else 'BPRTrainer', 'optimizer': 'AdamW', 'lr': 5e-3, 'l2_reg': 1e-4, 'aux_reg': 0.01, 'device': DEV,
+           'n_epochs': 1, 'batch_size': 1024, 'topks': [20], 'hip_graph': hip_graph, 'state_bits': bits, 'weight_decay': 1e-3, 'max_grad_norm': 0.05, **kw}
+    return ds, model, get_trainer(cfg, ds, model)
+
+
+@pytest.mark.parametrize('name', ['MF', 'LightGCN', 'IGCN'])
+@pytest.mark.parametrize('bits', [8, 32])
+def test_trainers_take_the_step_by_name_captured_or_not(name, bits):
+    """config 'optimizer': 'AdamW': captured and eager steps count and move alike (batch gradients come from float atomics, whose order
+    differs from run to run, so the losses agree to 1e-3 rather than to the bit)."""
+    ends = []
+    for hip_graph in (True, False):
+        ds, model, trainer = _trainer(name, hip_graph, bits)
+        assert type(trainer.opt).__module__ == 'igcn_cf_amd.optim' and trainer._graph_wanted() == hip_graph
+        model.train()
+        losses = [trainer.train_one_epoch() for _ in range(2)]
+        assert all(np.isfinite(losses))
+        assert (trainer._graph is not None) == hip_graph
+        steps = {float(s['step']) for s in trainer.opt.state.values()}
+        assert len(trainer.opt.state) == len(list(model.parameters())) and len(steps) == 1
+        ends.append((losses, steps))
+    assert ends[0][1] == ends[1][1] and min(ends[0][1]) > 2
+    assert all(abs(a - b) < 1e-3 for a, b in zip(ends[0][0], ends[1][0]))
+
+
+def test_train_in_8_bits_clip_quantize_and_answer():
+    """The operators as they are used together: LightGCN trained with 8-bit moments and clipped gradients, its item rows made 8-bit,
+    the dense score block answered from them — every score within the codes' bound of the float32 block's."""
+    ds, model, trainer = _trainer('LightGCN', True, 8)
+    model.train()
+    for _ in range(2):
+        trainer.train_one_epoch()
+    assert 0 < float(trainer.opt.grad_norm) < 1e3
+    model.eval()
+    users = torch.tensor([0, 5, 599, 5, 17], device=DEV)
+    items = model.quantized_items()
+    with torch.no_grad():
+        want = model.predict(users).double()
+        rep = model.get_rep()
+    u, i = rep[users].double(), rep[ds.n_users:].double()
+    eu, ei = u.abs().amax(1, keepdim=True) / 254, i.abs().amax(1, keepdim=True) / 254          # half a code step
+    bound = eu * i.abs().sum(1) + u.abs().sum(1, keepdim=True) * ei.t() + 64 * eu * ei.t()
+    for dtype in (torch.float32, torch.bfloat16):
+        got = model.predict_i8(users, items, dtype=dtype)
+        half = torch.finfo(dtype).eps / 2
+        assert got.dtype == dtype and got.shape == (5, ds.n_items)
+        slack = (half + 8 * 2.0 ** -24) * (want.abs() + bound) + 64 * 2.0 ** -24 * u.abs().sum(1, keepdim=True) * i.abs().amax(1)
+        assert bool(((got.double() - want).abs() <= bound * (1 + 1e-5) + slack).all())
+    assert torch.equal(model.predict_i8(users), model.predict_i8(users, items))
