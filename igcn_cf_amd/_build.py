@@ -9,7 +9,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, 'csrc')
 LIB = os.path.join(PKG, 'libigcn_hip.so')
 ROOF_LIB = os.path.join(PKG, 'libigcn_roof.so')
-SOURCES = [f for f in ('spmm.hip', 'bpr.hip', 'score_topk.hip', 'topk_order.hip', 'sampler.hip', 'csr_util.hip', 'adamw.hip', 'gemm_i8.hip')
+SOURCES = [f for f in ('spmm.hip', 'bpr.hip', 'score_topk.hip', 'topk_order.hip', 'sampler.hip', 'csr_util.hip', 'adamw.hip', 'quant_i8.hip', 'gemm_i8.hip')
            if os.path.exists(os.path.join(CSRC, f))]
 # -packed-fp32-ops: no packed fp32 arithmetic (v_pk_fma_f32 and its like, which hipcc forms from ordinary float code by itself): some of
 # its forms have given wrong results on this hardware now and then (the host pass does not know the feature and says so)

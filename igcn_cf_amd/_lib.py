@@ -98,6 +98,8 @@ SIGNATURES = {
     'igcn_quantize_rows_i8': (C.c_int, [vp, C.c_int32, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int64, vp, vp]),
     'igcn_dequantize_rows_i8': (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64, vp]),
     'igcn_matmul_i8': (C.c_int, [vp, C.c_int64, vp, vp, C.c_int64, vp, vp, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64, vp]),
+    'igcn_linear_i8_workspace_bytes': (C.c_int64, [C.c_int64, C.c_int64]),
+    'igcn_linear_i8': (C.c_int, [vp, C.c_int32, C.c_int64, vp, C.c_int64, vp, vp, C.c_int64, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64, vp, vp]),
     'igcn_bpr_loss_bwd_scaled_f32': (C.c_int, [vp, vp, vp, C.c_int64, vp, vp, vp, C.c_int64, vp, vp, vp,
                                                C.c_int64, C.c_int32, vp, vp, vp, C.c_float, C.c_float,
                                                vp, vp, vp, vp, vp, vp, vp, vp]),
@@ -181,4 +183,4 @@ def ptr(t):
 
 def current_stream():
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())      # (torch.cuda.current_stream().cuda_stream without the Stream object: 2.8 -> 0.3 us a call)

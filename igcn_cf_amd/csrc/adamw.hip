@@ -40,14 +40,11 @@ struct Hyper {
     uint32_t seed_lo, seed_hi;
 };
 
-// 8 consecutive values of src at element i; `whole`: all 8 are there and src is aligned to 8 of them (16 bytes at most)
+// 8 consecutive values of src at element i; `whole`: all 8 are there (at any address: the hardware loads and stores 16 bytes anywhere)
 template <typename T> __device__ __forceinline__ void load8(const T *__restrict__ src, int64_t i, int64_t n, bool whole, T (&x)[kPer])
 {
     if (whole) {
-        struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) V { T v[kPer]; };
-        const V w = *reinterpret_cast<const V *>(src + i);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) x[k] = w.v[k];
+        load_vector(x, src + i);
     } else {
 #pragma unroll
         for (int k = 0; k < kPer; ++k) x[k] = i + k < n ? src[i + k] : T(0.f);
@@ -56,10 +53,7 @@ template <typename T> __device__ __forceinline__ void load8(const T *__restrict_
 template <typename T> __device__ __forceinline__ void store8(T *__restrict__ dst, int64_t i, int64_t n, bool whole, const T (&x)[kPer])
 {
     if (whole) {
-        struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) V { T v[kPer]; } w;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) w.v[k] = x[k];
-        *reinterpret_cast<V *>(dst + i) = w;
+        store_vector(dst + i, x);
     } else {
 #pragma unroll
         for (int k = 0; k < kPer; ++k) if (i + k < n) dst[i + k] = x[k];
@@ -76,14 +70,12 @@ __device__ __forceinline__ int tensor_of_chunk(const TensorTable &T, int chunk)
     return lo;
 }
 
-__device__ __forceinline__ bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-
 // ---- the norm ------------------------------------------------------------------------------------------------------------------
 template <typename G> __device__ __forceinline__ double chunk_squares(const G *__restrict__ g, int64_t i, int64_t n)
 {
     if (i >= n) return 0.0;
     G x[kPer];
-    load8(g, i, n, i + kPer <= n && aligned(g, sizeof(G) * kPer < 16 ? sizeof(G) * kPer : 16), x);
+    load8(g, i, n, i + kPer <= n, x);
     double s = 0.0;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) { const double y = to_float(x[k]); s = fma(y, y, s); }
@@ -169,7 +161,7 @@ __device__ __forceinline__ float stepped(float p, float m, float v, const Prepar
 template <typename P, typename G>
 __device__ __forceinline__ void step32(const igcn_adamw_tensor &t, int64_t i, const Hyper &H, const Prepared &q)
 {
-    const bool ok = i + kPer <= t.n && aligned(t.param, 16) && aligned(t.grad, 16) && aligned(t.exp_avg, 16) && aligned(t.exp_avg_sq, 16);
+    const bool ok = i + kPer <= t.n;
     P p[kPer]; G g[kPer]; float m[kPer], v[kPer];
     load8(static_cast<const G *>(t.grad), i, t.n, ok, g);
     load8(static_cast<const float *>(t.exp_avg), i, t.n, ok, m);
@@ -210,7 +202,7 @@ template <typename P, typename G>
 __device__ __forceinline__ void step8(const igcn_adamw_tensor &t, int64_t i, const Hyper &H, const Prepared &q)
 {
 #pragma clang fp contract(off)
-    const bool ok = i + kPer <= t.n && aligned(t.param, 16) && aligned(t.grad, 16) && aligned(t.exp_avg, 8) && aligned(t.exp_avg_sq, 8);
+    const bool ok = i + kPer <= t.n;
     P p[kPer]; G g[kPer]; uint8_t mc[kPer], vc[kPer];
     load8(static_cast<const G *>(t.grad), i, t.n, ok, g);
     load8(static_cast<const uint8_t *>(t.exp_avg), i, t.n, ok, mc);

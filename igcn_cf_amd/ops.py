@@ -807,7 +807,7 @@ def _dense(t):
 
 
 def _same_order(a, b):
-    return a.shape == b.shape and (a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous()))
+    return a.shape == b.shape and ((a.is_contiguous() and b.is_contiguous()) or a.stride() == b.stride())
 
 
 def _check_grads(grads):
@@ -816,9 +816,9 @@ def _check_grads(grads):
     for g in grads:
         if not (isinstance(g, torch.Tensor) and g.is_cuda and g.layout == torch.strided and g.dtype in _DTYPE_CODES):
             raise _lib.IgcnError('gradients must be dense float32, bfloat16 or float16 tensors on the GPU (no CPU path)')
-        if g.device != device:
+        if g.get_device() != device.index:
             raise _lib.IgcnError('the tensors of a call must be on one device')
-        if not _dense(g):
+        if not (g.is_contiguous() or _dense(g)):
             raise _lib.IgcnError('gradients must fill a stretch of memory (a view with gaps or repeats does not)')
     return device
 
@@ -864,27 +864,27 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and weight_decay >= 0.):
         raise _lib.IgcnError('betas must be in [0, 1), eps and weight_decay not negative')
     device = _check_grads(grads)
-    want_m, want_v = MOMENT_DTYPES if eight else (torch.float32, torch.float32)
-    rows, written = array.array('q'), []
-    for p, g, m, v, t, s in zip(params, grads, exp_avgs, exp_avg_sqs, steps, scales):
-        if p.device != device or m.device != device or v.device != device or t.device != device or (eight and s.device != device):
-            raise _lib.IgcnError('the tensors of a call must be on one device')
-        if p.dtype not in _DTYPE_CODES or (g.dtype != p.dtype and g.dtype != torch.float32) or m.dtype != want_m or v.dtype != want_v:
+    every = params + exp_avgs + exp_avg_sqs + steps + (scales if eight else [])
+    if n and {t.get_device() for t in every} != {device.index}:
+        raise _lib.IgcnError('the tensors of a call must be on one device, a GPU')
+    want = MOMENT_DTYPES if eight else (torch.float32, torch.float32)
+    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+        if p.dtype not in _DTYPE_CODES or (g.dtype != p.dtype and g.dtype != torch.float32) or m.dtype != want[0] or v.dtype != want[1]:
             raise _lib.IgcnError('parameters: float32, bfloat16 or float16; gradients: the same or float32; moments: float32, or with scales '
                                  'float8_e4m3fn and float8_e5m2 (got %s, %s, %s, %s)' % (p.dtype, g.dtype, m.dtype, v.dtype))
         if not (_same_order(p, g) and _same_order(p, m) and _same_order(p, v)):
             raise _lib.IgcnError('gradient and moments must have the shape and the order in memory of their parameter')
-        if t.dtype != torch.float32 or t.numel() != 1:
-            raise _lib.IgcnError('steps must be one-element float32 tensors')
-        k = p.numel()
-        if eight and (s.dtype != torch.float32 or s.shape != ((k + ADAMW_BLOCK - 1) // ADAMW_BLOCK, 2) or not s.is_contiguous()):
-            raise _lib.IgcnError('scales must be contiguous float32 [ceil(numel / %d), 2]' % ADAMW_BLOCK)
-        ptrs = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), s.data_ptr() if eight else 0, t.data_ptr())
-        rows.extend(ptrs)
-        rows.extend((k, _DTYPE_CODES[p.dtype] | _DTYPE_CODES[g.dtype] << 32))
-        written += [ptrs[0], ptrs[2], ptrs[3], ptrs[5]] if k else [ptrs[5]]
+    sizes = [p.numel() for p in params]
+    if any(t.dtype != torch.float32 or t.numel() != 1 for t in steps):
+        raise _lib.IgcnError('steps must be one-element float32 tensors')
+    if eight and any(s.dtype != torch.float32 or s.shape != ((k + ADAMW_BLOCK - 1) // ADAMW_BLOCK, 2) or not s.is_contiguous() for s, k in zip(scales, sizes)):
+        raise _lib.IgcnError('scales must be contiguous float32 [ceil(numel / %d), 2]' % ADAMW_BLOCK)
+    at = [[t.data_ptr() for t in ts] for ts in (params, exp_avgs, exp_avg_sqs, steps)]
+    written = [a for column in at for a in column if a]                                  # (an empty tensor has no address)
     if len(set(written)) != len(written):
         raise _lib.IgcnError('a tensor stands in the lists twice: every parameter, moment and step is rewritten by one place only')
+    rows = array.array('q', [x for p, g, m, v, s, t, k, pt, gt in zip(at[0], grads, at[1], at[2], scales, at[3], sizes, params, grads)
+                             for x in (p, g.data_ptr(), m, v, s.data_ptr() if eight else 0, t, k, _DTYPE_CODES[pt.dtype] | _DTYPE_CODES[gt.dtype] << 32)])
     lr_dev = norm_in = None
     if isinstance(lr, torch.Tensor):
         if lr.dtype != torch.float32 or lr.numel() != 1 or (n and lr.device != device):
@@ -928,8 +928,8 @@ def _ld(t):
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
-def _require_vector(t, name, n, device):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.device == device):
+def _require_vector(t, name, n, like):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous() and t.get_device() == like.get_device()):
         raise _lib.IgcnError('%s must be contiguous float32 [%d] on the device of the rows' % (name, n))
 
 
@@ -953,12 +953,23 @@ def dequantize_rows_i8(codes, scale, dtype=torch.float32):
     if dtype not in _DTYPE_CODES:
         raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
     m, k = codes.shape
-    _require_vector(scale, 'scale', m, codes.device)
+    _require_vector(scale, 'scale', m, codes)
     with _on(codes.device):
         y = torch.empty((m, k), dtype=dtype, device=codes.device)
         _lib.check(_lib.lib().igcn_dequantize_rows_i8(codes.data_ptr(), _ld(codes), scale.data_ptr(), m, k, y.data_ptr(), _DTYPE_CODES[dtype], k,
                                                       _lib.current_stream()), 'igcn_dequantize_rows_i8')
     return y
+
+
+def _check_product(a, name, m, k, b, b_scale, bias):
+    if b.shape[1] != k or b.get_device() != a.get_device():
+        raise _lib.IgcnError('%s [M, K] and b [N, K] must agree in K and be on one device (got %s on %s, %s on %s)'
+                             % (name, tuple(a.shape), a.device, tuple(b.shape), b.device))
+    if k > MAX_I8_DEPTH:
+        raise _lib.IgcnError('K must be at most %d: a longer sum could pass 32 bits' % MAX_I8_DEPTH)
+    _require_vector(b_scale, 'b_scale', b.shape[0], a)
+    if bias is not None:
+        _require_vector(bias, 'bias', b.shape[0], a)
 
 
 def matmul_i8(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
@@ -967,16 +978,10 @@ def matmul_i8(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
     _require_rows(a, 'a', (torch.int8,))
     _require_rows(b, 'b', (torch.int8,))
     (m, k), n = a.shape, b.shape[0]
-    if b.shape[1] != k or b.device != a.device:
-        raise _lib.IgcnError('a [M, K] and b [N, K] must agree in K and be on one device (got %s on %s, %s on %s)' % (tuple(a.shape), a.device, tuple(b.shape), b.device))
-    if k > MAX_I8_DEPTH:
-        raise _lib.IgcnError('K must be at most %d: a longer sum could pass 32 bits' % MAX_I8_DEPTH)
+    _check_product(a, 'a', m, k, b, b_scale, bias)
     if dtype not in _DTYPE_CODES:
         raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
-    _require_vector(a_scale, 'a_scale', m, a.device)
-    _require_vector(b_scale, 'b_scale', n, a.device)
-    if bias is not None:
-        _require_vector(bias, 'bias', n, a.device)
+    _require_vector(a_scale, 'a_scale', m, a)
     with _on(a.device):
         y = torch.empty((m, n), dtype=dtype, device=a.device)
         _lib.check(_lib.lib().igcn_matmul_i8(a.data_ptr(), _ld(a), a_scale.data_ptr(), b.data_ptr(), _ld(b), b_scale.data_ptr(), _lib.ptr(bias),
@@ -985,6 +990,20 @@ def matmul_i8(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
 
 
 def linear_i8(x, b, b_scale, bias=None, dtype=None):
-    """[M, N] of `dtype` (None: that of x): the rows of x made 8-bit (quantize_rows_i8) and multiplied with those of b (matmul_i8)."""
-    q, scale = quantize_rows_i8(x)
-    return matmul_i8(q, scale, b, b_scale, bias=bias, dtype=x.dtype if dtype is None else dtype)
+    """[M, N] of `dtype` (None: that of x): the rows of x made 8-bit, as quantize_rows_i8 makes them, and multiplied with those of b, as
+    matmul_i8 does (igcn_linear_i8: one call, a few short rows in one launch)."""
+    _require_rows(x, 'x', tuple(_DTYPE_CODES))
+    _require_rows(b, 'b', (torch.int8,))
+    (m, k), n = x.shape, b.shape[0]
+    _check_product(x, 'x', m, k, b, b_scale, bias)
+    out = _DTYPE_CODES.get(x.dtype if dtype is None else dtype)
+    if out is None:
+        raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
+    with _on(x.device):
+        L = _lib.lib()
+        y = torch.empty((m, n), dtype=dtype or x.dtype, device=x.device)
+        need = L.igcn_linear_i8_workspace_bytes(m, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        _lib.check(L.igcn_linear_i8(x.data_ptr(), _DTYPE_CODES[x.dtype], _ld(x), b.data_ptr(), _ld(b), b_scale.data_ptr(), _lib.ptr(bias), m, n, k,
+                                    y.data_ptr(), out, n, _lib.ptr(ws), _lib.current_stream()), 'igcn_linear_i8')
+    return y

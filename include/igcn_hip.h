@@ -525,6 +525,12 @@ int igcn_dequantize_rows_i8(const int8_t *q, int64_t ldq, const float *scale, in
 int igcn_matmul_i8(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias,
                    int64_t m, int64_t n, int64_t k, void *y, int32_t dtype, int64_t ldy, void *stream);
 
+/* The same with the rows of a given in floating point (x [m, k], `x_dtype`) and made 8-bit on the way, as igcn_quantize_rows_i8 makes
+ * them.  workspace: igcn_linear_i8_workspace_bytes(m, k) bytes, 16-byte aligned (0: NULL will do); one call's own. */
+int64_t igcn_linear_i8_workspace_bytes(int64_t m, int64_t k);
+int igcn_linear_i8(const void *x, int32_t x_dtype, int64_t ldx, const int8_t *b, int64_t ldb, const float *sb, const float *bias,
+                   int64_t m, int64_t n, int64_t k, void *y, int32_t dtype, int64_t ldy, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
