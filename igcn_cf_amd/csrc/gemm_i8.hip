@@ -19,11 +19,11 @@ struct GemmArgs {
 };
 
 // The sum's way to y, the same in every kernel: each operation rounded once in float32, no fused multiply-add.
-__device__ __forceinline__ float scaled(int acc, float sa, float sb, const float *bias, int64_t c)
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, bool biased, float bias)
 {
 #pragma clang fp contract(off)
     const float v = (float)acc * sa * sb;
-    return bias ? v + bias[c] : v;
+    return biased ? v + bias : v;
 }
 __device__ __forceinline__ void store_out(const GemmArgs &G, int64_t r, int64_t c, float v)
 {
@@ -43,36 +43,178 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int64_t 
     return v;
 }
 
-constexpr int kTile = 64, kDepth = 64;
-// One workgroup = 64 x 64 of y, a wave 32 x 32 of it
-__global__ __launch_bounds__(kBlock) void gemm_i8_kernel(const GemmArgs G)
+// ---- many rows of a -------------------------------------------------------------------------------------------------------------------
+// Bound by the matrix cores (deep sums) or by writing y (shallow ones).  A workgroup makes a TM x TN tile of y, a wave TM / WM x TN / WN of it in
+// 32 x 32 pieces (v_mfma_i32_32x32x32_i8: lane l holds row l % 32, 16 bytes of depth at 16 (l / 32)).  128 codes of depth of either side
+// go to LDS per stage, two stages in turn: the next one is on its way from memory while this one is multiplied, one barrier a stage.
+// DIRECT (rows 16-byte aligned, depth a multiple of 16): memory to LDS without registers (global_load_lds, 1 KiB a wave and
+// instruction, lane after lane); else through registers.  A row's eight 16-byte pieces stand in LDS at piece ^ (row % 8): 8 lanes that read the
+// same piece of 8 neighbouring rows hit different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
+// Depth past the end reads a block of zeros, rows past the end the last row (not stored).
+// Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, 4 tiles of a deep at a time, so that the tiles under way there
+// share their rows in its L2.
+constexpr int kDepth = 128;
+__device__ const i32x4 g_zeros = {0, 0, 0, 0};
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+// memory -> LDS, 16 bytes a lane, lane after lane from byte `lds` on, without the compiler's knowledge: it would wait for it before any
+// later LDS read, the other stage's among them.  The kernel waits itself (wait_for_lds) before the barrier behind which it is read.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"                  // (m0 is a reserved register: saying that it is written is the point)
+__device__ __forceinline__ void to_lds(const void *base, unsigned offset, unsigned lds)
 {
-    __shared__ i32x4 as[kTile * kDepth / 16], bs[kTile * kDepth / 16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-    const int row = threadIdx.x >> 2, piece = threadIdx.x & 3;
-    i32x16 acc = {};
-    for (int64_t k0 = 0; k0 < G.k; k0 += kDepth) {
-        i32x4 zero = {0, 0, 0, 0};
-        as[row * 4 + piece] = m0 + row < G.m ? load16(G.a + (m0 + row) * G.lda, k0 + 16 * piece, G.k) : zero;
-        bs[row * 4 + piece] = n0 + row < G.n ? load16(G.b + (n0 + row) * G.ldb, k0 + 16 * piece, G.k) : zero;
-        __syncthreads();
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds(const void *p, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+constexpr int64_t kMostApart = 1 << 23;                          // bytes between rows: 256 of them fit 31 bits
+struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; };
+
+template <int TM, int TN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArgs T)
+{
+    constexpr int kWaves = WM * WN, RT = TM / WM / 32, CT = TN / WN / 32, NA = TM / 8 / kWaves, NB = TN / 8 / kWaves;
+    constexpr int kStage = (TM + TN) * kDepth;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const GemmArgs &G = T.g;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = (int64_t)(blockIdx.x & 7) * T.per_xcd + (blockIdx.x >> 3);
+    if ((int64_t)(blockIdx.x >> 3) >= T.per_xcd || t >= T.tiles_m * T.tiles_n) return;
+    // runs of 4 tile rows, column after column
+    const int64_t band = t / (4 * T.tiles_n), in = t - band * 4 * T.tiles_n, high = T.tiles_m - 4 * band < 4 ? T.tiles_m - 4 * band : 4;
+    const int64_t m0 = (4 * band + in % high) * TM, n0 = in / high * TN;
+
+    // this lane's pieces: rows 8 (wave NA + i) + lane / 8 of the tile, piece (lane % 8) ^ (row % 8); offsets from the tile's first row fit 32 bits
+    const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+    const int8_t *const base_a = G.a + m0 * G.lda, *const base_b = G.b + n0 * G.ldb;
+    const int last_a = (int)(G.m - m0 < TM ? G.m - m0 : TM) - 1, last_b = (int)(G.n - n0 < TN ? G.n - n0 : TN) - 1;
+    unsigned oa[NA], ob[NB];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const i32x4 av = as[((wave >> 1) * 32 + (lane & 31)) * 4 + 2 * s + (lane >> 5)];
-            const i32x4 bv = bs[((wave & 1) * 32 + (lane & 31)) * 4 + 2 * s + (lane >> 5)];
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, bv, acc, 0, 0, 0);
+    for (int i = 0; i < NA; ++i) oa[i] = (unsigned)min(8 * (wave * NA + i) + (lane >> 3), last_a) * (unsigned)G.lda + piece;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) ob[i] = (unsigned)min(8 * (wave * NB + i) + (lane >> 3), last_b) * (unsigned)G.ldb + piece;
+    const int64_t stages = (G.k + kDepth - 1) / kDepth;
+    i32x4 held[DIRECT ? 1 : NA + NB];
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void *)smem;
+
+    auto fetch = [&](int64_t s) {                                // stage s of both sides: on its way to LDS, or to registers
+        const int64_t k0 = s * kDepth;
+        if constexpr (DIRECT) {
+            const unsigned at = lds0 + (unsigned)(s & 1) * kStage + wave * NA * 1024, bt = lds0 + (unsigned)(s & 1) * kStage + TM * kDepth + wave * NB * 1024;
+            if (k0 + kDepth <= G.k) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) to_lds(base_a + k0, oa[i], at + 1024 * i);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) to_lds(base_b + k0, ob[i], bt + 1024 * i);
+            } else {                                             // (pieces are whole: the depth is a multiple of 16)
+                const bool there = k0 + piece < G.k;
+#pragma unroll
+                for (int i = 0; i < NA; ++i) to_lds(there ? (const void *)(base_a + k0 + oa[i]) : (const void *)&g_zeros, at + 1024 * i);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) to_lds(there ? (const void *)(base_b + k0 + ob[i]) : (const void *)&g_zeros, bt + 1024 * i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NA; ++i) held[i] = load16(base_a + oa[i] - piece, k0 + piece, G.k);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + ob[i] - piece, k0 + piece, G.k);
         }
+    };
+    auto land = [&](int64_t s) {                                 // stage s is in LDS for everyone behind the next barrier
+        if constexpr (DIRECT) wait_for_lds();
+        else {
+            i32x4 *at = reinterpret_cast<i32x4 *>(smem + (s & 1) * kStage);
+#pragma unroll
+            for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = held[i];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
+        }
+    };
+
+    i32x16 acc[RT][CT] = {};
+    const int wm = wave / WN, wn = wave % WN;
+    const int ra = wm * (TM / WM) + (lane & 31), rb = wn * (TN / WN) + (lane & 31), half = lane >> 5, turn = lane & 7;
+    if (stages) { fetch(0); land(0); }
+    __syncthreads();
+    for (int64_t s = 0; s < stages; ++s) {
+        if (s + 1 < stages) fetch(s + 1);
+        const unsigned char *sa = smem + (s & 1) * kStage + ra * kDepth, *sb = smem + (s & 1) * kStage + TM * kDepth + rb * kDepth;
+#pragma unroll
+        for (int j = 0; j < kDepth / 32; ++j) {
+            const int at = ((2 * j + half) ^ turn) * 16;
+            i32x4 av[RT], bv[CT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) av[r] = *reinterpret_cast<const i32x4 *>(sa + r * 32 * kDepth + at);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) bv[c] = *reinterpret_cast<const i32x4 *>(sb + c * 32 * kDepth + at);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[r], bv[c], acc[r][c], 0, 0, 0);
+        }
+        if (s + 1 < stages) land(s + 1);
         __syncthreads();
     }
-    const int64_t c = n0 + (wave & 1) * 32 + (lane & 31);
+
+    // lane l holds column l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4: a wave's store covers two rows' 32 neighbouring columns
+    float *const scales = reinterpret_cast<float *>(smem);       // (the last stage is through with LDS)
+    for (int i = threadIdx.x; i <= last_a; i += 64 * kWaves) scales[i] = G.sa[m0 + i];
+    __syncthreads();
+    auto put = [&](auto *y) {
+        using Y = std::remove_pointer_t<decltype(y)>;
+        float sb[CT], bias[CT];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int64_t r = m0 + (wave >> 1) * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-        if (r < G.m && c < G.n) store_out(G, r, c, scaled(acc[i], G.sa[r], G.sb[c], G.bias, c));
-    }
+        for (int c = 0; c < CT; ++c) {
+            sb[c] = rb + 32 * c <= last_b ? G.sb[n0 + rb + 32 * c] : 0.f;
+            bias[c] = G.bias && rb + 32 * c <= last_b ? G.bias[n0 + rb + 32 * c] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int m1 = wm * (TM / WM) + r * 32 + 4 * half;
+            Y *p = y + (m0 + m1) * G.ldy + n0 + rb;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int m = m1 + 8 * (i >> 2) + (i & 3);
+                if (m <= last_a) {
+                    const float s = scales[m];
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+                        if (rb + 32 * c <= last_b) p[32 * c] = from_float<Y>(scaled(acc[r][c][i], s, sb[c], G.bias != nullptr, bias[c]));
+                }
+                p += (i & 3) == 3 ? 5 * G.ldy : G.ldy;
+            }
+        }
+    };
+    if (G.out == IGCN_DTYPE_F32) put(static_cast<float *>(G.y));
+    else if (G.out == IGCN_DTYPE_BF16) put(static_cast<__hip_bfloat16 *>(G.y));
+    else put(static_cast<__half *>(G.y));
 }
 
+template <int TM, int TN, int WM, int WN> static int tiles_launch(const GemmArgs &G, hipStream_t st)
+{
+    TileArgs T;
+    T.g = G;
+    T.tiles_m = (G.m + TM - 1) / TM;
+    T.tiles_n = (G.n + TN - 1) / TN;
+    if (T.tiles_m > (1 << 28) / T.tiles_n) return IGCN_E_SHAPE;
+    T.per_xcd = (T.tiles_m * T.tiles_n + 7) / 8;
+    const bool direct = ((reinterpret_cast<uintptr_t>(G.a) | reinterpret_cast<uintptr_t>(G.b) | (uintptr_t)G.lda | (uintptr_t)G.ldb | (uintptr_t)G.k) & 15) == 0;
+    const size_t lds = (size_t)(G.k > kDepth ? 2 : 1) * (TM + TN) * kDepth;
+    const void *kernel = direct ? reinterpret_cast<const void *>(tiles_i8_kernel<TM, TN, WM, WN, true>) : reinterpret_cast<const void *>(tiles_i8_kernel<TM, TN, WM, WN, false>);
+    if (lds > 65536) {                                           // (once would do; it is a host call of well under a microsecond)
+        const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return (int)e;
+    }
+    if (direct) hipLaunchKernelGGL((tiles_i8_kernel<TM, TN, WM, WN, true>), dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
+    else hipLaunchKernelGGL((tiles_i8_kernel<TM, TN, WM, WN, false>), dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
+    return launch_status();
+}
 
 // ---- few rows of a --------------------------------------------------------------------------------------------------------------------
 // Bound by the bytes of b, each used once: no tile of b is worth staging.  A wave takes 16 rows of b as the matrix instruction's first
@@ -204,7 +346,7 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
                         int sum = 0;
 #pragma unroll
                         for (int w = 0; w < 4; ++w) sum += sums[(((t * GROUPS + g) * 4 + w) * 16 + r) * 17 + c];
-                        store_out(G, mm, n, scaled(sum, sx[mm], G.sb[n], G.bias, n));
+                        store_out(G, mm, n, scaled(sum, sx[mm], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
                     }
                 }
         } else {
@@ -216,7 +358,7 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
                     const int64_t n0 = (tile0 + t) * 16 + 4 * quarter;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (mm < m && n0 + i < G.n) store_out(G, mm, n0 + i, scaled(acc[t][g][i], sx[mm], G.sb[n0 + i], G.bias, n0 + i));
+                        if (mm < m && n0 + i < G.n) store_out(G, mm, n0 + i, scaled(acc[t][g][i], sx[mm], G.sb[n0 + i], G.bias != nullptr, G.bias ? G.bias[n0 + i] : 0.f));
                 }
         }
     }
@@ -251,15 +393,23 @@ template <typename X> static int few_rows(const FewArgs &F, hipStream_t st)
 
 static int product(const GemmArgs &G, hipStream_t st)
 {
-    if (G.m <= kFewRows) {
-        FewArgs F = {};
-        F.g = G;
-        return few_rows<int8_t>(F, st);
+    if (G.m <= kFewRows || G.lda > kMostApart || G.ldb > kMostApart) {
+        const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
+        for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 64 at a time)
+            FewArgs F = {};
+            F.g = G;
+            F.g.a += at * G.lda;
+            F.g.sa += at;
+            F.g.y = static_cast<char *>(G.y) + at * G.ldy * size;
+            F.g.m = G.m - at < kFewRows ? G.m - at : kFewRows;
+            const int rc = few_rows<int8_t>(F, st);
+            if (rc != IGCN_OK) return rc;
+        }
+        return IGCN_OK;
     }
-    const int64_t gx = (G.n + kTile - 1) / kTile, gy = (G.m + kTile - 1) / kTile;
-    if (gx > 0x7fffffff || gy > 65535) return IGCN_E_SHAPE;
-    hipLaunchKernelGGL(gemm_i8_kernel, dim3((unsigned)gx, (unsigned)gy), dim3(kBlock), 0, st, G);
-    return launch_status();
+    // 256 x 256 tiles read each code half as often as 128 x 128 ones, and there have to be enough of them for 256 CUs
+    const int64_t large = ((G.m + 255) / 256) * ((G.n + 255) / 256);
+    return large >= 200 && G.k >= 512 ? tiles_launch<256, 256, 2, 4>(G, st) : tiles_launch<128, 128, 2, 2>(G, st);
 }
 
 static int check_product(const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias, int64_t m, int64_t n, int64_t k, const void *y,
