@@ -156,38 +156,56 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[r], bv[c], acc[r][c], 0, 0, 0);
+                for (int c = 0; c < CT; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[c], av[r], acc[r][c], 0, 0, 0);
         }
         if (s + 1 < stages) land(s + 1);
         __syncthreads();
     }
 
-    // lane l holds column l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4: a wave's store covers two rows' 32 neighbouring columns
-    float *const scales = reinterpret_cast<float *>(smem);       // (the last stage is through with LDS)
-    for (int i = threadIdx.x; i <= last_a; i += 64 * kWaves) scales[i] = G.sa[m0 + i];
+    // The way out.  b is the matrix instruction's first operand: lane l holds row l % 32 of a and columns 8 (i / 4) + 4 (l / 32) + i % 4, four
+    // neighbours of a row of y at a time.  They cross a strip of LDS of the wave's own (32 rows, its columns) so that a store takes whole
+    // lines: 16 bytes a lane, neighbouring lanes along the row.
+    float *const fa = reinterpret_cast<float *>(smem), *const fb = fa + TM, *const fc = fb + TN;       // (the last stage is through with LDS)
+    for (int i = threadIdx.x; i < TM; i += 64 * kWaves) fa[i] = i <= last_a ? G.sa[m0 + i] : 0.f;
+    for (int i = threadIdx.x; i < TN; i += 64 * kWaves) {
+        fb[i] = i <= last_b ? G.sb[n0 + i] : 0.f;
+        fc[i] = G.bias && i <= last_b ? G.bias[n0 + i] : 0.f;
+    }
     __syncthreads();
     auto put = [&](auto *y) {
         using Y = std::remove_pointer_t<decltype(y)>;
-        float sb[CT], bias[CT];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            sb[c] = rb + 32 * c <= last_b ? G.sb[n0 + rb + 32 * c] : 0.f;
-            bias[c] = G.bias && rb + 32 * c <= last_b ? G.bias[n0 + rb + 32 * c] : 0.f;
-        }
+        constexpr int kCols = CT * 32, kRow = kCols * sizeof(Y) + 16, kLanes = kCols * sizeof(Y) / 16, kE = 16 / sizeof(Y);       // (16 bytes more a row: other banks)
+        unsigned char *const strip = smem + (TM + 2 * TN) * 4 + wave * 32 * (kCols * 4 + 16);
+        const bool biased = G.bias != nullptr;
+        const int n1 = wn * (TN / WN) + lane % kLanes * kE;      // of the tile: this lane's columns on the way out
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const int m1 = wm * (TM / WM) + r * 32 + 4 * half;
-            Y *p = y + (m0 + m1) * G.ldy + n0 + rb;
+            const float s = fa[wm * (TM / WM) + r * 32 + (lane & 31)];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int m = m1 + 8 * (i >> 2) + (i & 3);
-                if (m <= last_a) {
-                    const float s = scales[m];
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        if (rb + 32 * c <= last_b) p[32 * c] = from_float<Y>(scaled(acc[r][c][i], s, sb[c], G.bias != nullptr, bias[c]));
+                for (int q = 0; q < 4; ++q) {
+                    const int at = c * 32 + 8 * q + 4 * half;
+                    const float4 sb4 = *reinterpret_cast<const float4 *>(fb + wn * (TN / WN) + at), bi4 = *reinterpret_cast<const float4 *>(fc + wn * (TN / WN) + at);
+                    Y v[4] = {from_float<Y>(scaled(acc[r][c][4 * q], s, sb4.x, biased, bi4.x)), from_float<Y>(scaled(acc[r][c][4 * q + 1], s, sb4.y, biased, bi4.y)),
+                              from_float<Y>(scaled(acc[r][c][4 * q + 2], s, sb4.z, biased, bi4.z)), from_float<Y>(scaled(acc[r][c][4 * q + 3], s, sb4.w, biased, bi4.w))};
+                    __builtin_memcpy(__builtin_assume_aligned(strip + (lane & 31) * kRow + at * sizeof(Y), 8), v, sizeof(v));
                 }
-                p += (i & 3) == 3 ? 5 * G.ldy : G.ldy;
+            const int m1 = wm * (TM / WM) + r * 32 + lane / kLanes;
+            Y *p = y + (m0 + m1) * G.ldy + n0 + n1;
+#pragma unroll
+            for (int i = 0; i < 32 * kLanes / 64; ++i) {
+                const i32x4 w = *reinterpret_cast<const i32x4 *>(strip + (lane / kLanes + i * (64 / kLanes)) * kRow + lane % kLanes * 16);
+                if (m1 + i * (64 / kLanes) <= last_a) {
+                    if (n1 + kE - 1 <= last_b) *reinterpret_cast<i32x4_any *>(p) = w;
+                    else {
+                        Y v[kE];
+                        __builtin_memcpy(v, &w, 16);
+#pragma unroll
+                        for (int e = 0; e < kE; ++e) if (n1 + e <= last_b) p[e] = v[e];
+                    }
+                }
+                p += (64 / kLanes) * G.ldy;
             }
         }
     };
@@ -205,7 +223,8 @@ template <int TM, int TN, int WM, int WN> static int tiles_launch(const GemmArgs
     if (T.tiles_m > (1 << 28) / T.tiles_n) return IGCN_E_SHAPE;
     T.per_xcd = (T.tiles_m * T.tiles_n + 7) / 8;
     const bool direct = ((reinterpret_cast<uintptr_t>(G.a) | reinterpret_cast<uintptr_t>(G.b) | (uintptr_t)G.lda | (uintptr_t)G.ldb | (uintptr_t)G.k) & 15) == 0;
-    const size_t lds = (size_t)(G.k > kDepth ? 2 : 1) * (TM + TN) * kDepth;
+    const size_t stages = (size_t)(G.k > kDepth ? 2 : 1) * (TM + TN) * kDepth, out = (TM + 2 * TN) * 4 + WM * WN * 32 * (TN / WN * 4 + 16);
+    const size_t lds = stages > out ? stages : out;
     const void *kernel = direct ? reinterpret_cast<const void *>(tiles_i8_kernel<TM, TN, WM, WN, true>) : reinterpret_cast<const void *>(tiles_i8_kernel<TM, TN, WM, WN, false>);
     if (lds > 65536) {                                           // (once would do; it is a host call of well under a microsecond)
         const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
