@@ -22,7 +22,7 @@ namespace igcn {
 constexpr int kTensors = 56;             // of one launch: 64 bytes each in at most 4 KiB of launch arguments
 constexpr int kPer = 8;                  // elements of a thread: 16 lanes (a DPP row) hold a block of 128
 constexpr int kChunk = kBlock * kPer;    // elements of a workgroup
-constexpr int kNormBlocks = 512;         // partial sums of a norm launch
+constexpr int kNormBlocks = 2048;        // partial sums of a norm launch
 static_assert(IGCN_ADAMW_BLOCK == 16 * kPer, "a block of the 8-bit moments is a DPP row's elements");
 
 struct TensorTable {

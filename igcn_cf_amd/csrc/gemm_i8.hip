@@ -71,12 +71,12 @@ __device__ __forceinline__ void to_lds(const void *p, unsigned lds)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
-__device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory"); }      // all but the last LEFT are there
 
 constexpr int64_t kMostApart = 1 << 23;                          // bytes between rows: 256 of them fit 31 bits
 struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; };
 
-template <int TM, int TN, int WM, int WN, bool DIRECT>
+template <int TM, int TN, int WM, int WN, int STAGES, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArgs T)
 {
     constexpr int kWaves = WM * WN, RT = TM / WM / 32, CT = TN / WN / 32, NA = TM / 8 / kWaves, NB = TN / 8 / kWaves;
@@ -87,8 +87,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     const int64_t t = (int64_t)(blockIdx.x & 7) * T.per_xcd + (blockIdx.x >> 3);
     if ((int64_t)(blockIdx.x >> 3) >= T.per_xcd || t >= T.tiles_m * T.tiles_n) return;
     // runs of 4 tile rows, column after column
-    const int64_t band = t / (4 * T.tiles_n), in = t - band * 4 * T.tiles_n, high = T.tiles_m - 4 * band < 4 ? T.tiles_m - 4 * band : 4;
-    const int64_t m0 = (4 * band + in % high) * TM, n0 = in / high * TN;
+    constexpr int bd = 4;
+    const int64_t band = t / (bd * T.tiles_n), in = t - band * bd * T.tiles_n, high = T.tiles_m - bd * band < bd ? T.tiles_m - bd * band : bd;
+    const int64_t m0 = (bd * band + in % high) * TM, n0 = in / high * TN;
 
     // this lane's pieces: rows 8 (wave NA + i) + lane / 8 of the tile, piece (lane % 8) ^ (row % 8); offsets from the tile's first row fit 32 bits
     const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     auto fetch = [&](int64_t s) {                                // stage s of both sides: on its way to LDS, or to registers
         const int64_t k0 = s * kDepth;
         if constexpr (DIRECT) {
-            const unsigned at = lds0 + (unsigned)(s & 1) * kStage + wave * NA * 1024, bt = lds0 + (unsigned)(s & 1) * kStage + TM * kDepth + wave * NB * 1024;
+            const unsigned at = lds0 + (unsigned)(s % STAGES) * kStage + wave * NA * 1024, bt = at + TM * kDepth + wave * (NB - NA) * 1024;
             if (k0 + kDepth <= G.k) {
 #pragma unroll
                 for (int i = 0; i < NA; ++i) to_lds(base_a + k0, oa[i], at + 1024 * i);
@@ -126,25 +127,27 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
             for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + ob[i] - piece, k0 + piece, G.k);
         }
     };
-    auto land = [&](int64_t s) {                                 // stage s is in LDS for everyone behind the next barrier
-        if constexpr (DIRECT) wait_for_lds();
-        else {
-            i32x4 *at = reinterpret_cast<i32x4 *>(smem + (s & 1) * kStage);
+    auto land = [&](int64_t s) {                                 // registers to LDS
+        i32x4 *at = reinterpret_cast<i32x4 *>(smem + (s % STAGES) * kStage);
 #pragma unroll
-            for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = held[i];
+        for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = held[i];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
-        }
+        for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
     };
 
     i32x16 acc[RT][CT] = {};
     const int wm = wave / WN, wn = wave % WN;
     const int ra = wm * (TM / WM) + (lane & 31), rb = wn * (TN / WN) + (lane & 31), half = lane >> 5, turn = lane & 7;
-    if (stages) { fetch(0); land(0); }
-    __syncthreads();
+    if constexpr (DIRECT) {
+        for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s);
+    } else if (stages) { fetch(0); land(0); }
     for (int64_t s = 0; s < stages; ++s) {
-        if (s + 1 < stages) fetch(s + 1);
-        const unsigned char *sa = smem + (s & 1) * kStage + ra * kDepth, *sb = smem + (s & 1) * kStage + TM * kDepth + rb * kDepth;
+        if constexpr (DIRECT) {                                  // stage s is there: all but the STAGES - 2 behind it
+            if (s + STAGES - 2 < stages) wait_for_lds<(STAGES - 2) * (NA + NB)>(); else wait_for_lds<0>();
+        }
+        __syncthreads();                                         // ... for everyone, and everyone is through with the stage before it
+        if (s + STAGES - 1 < stages) fetch(s + STAGES - 1);
+        const unsigned char *sa = smem + (s % STAGES) * kStage + ra * kDepth, *sb = smem + (s % STAGES) * kStage + TM * kDepth + rb * kDepth;
 #pragma unroll
         for (int j = 0; j < kDepth / 32; ++j) {
             const int at = ((2 * j + half) ^ turn) * 16;
@@ -158,9 +161,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
                 for (int c = 0; c < CT; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[c], av[r], acc[r][c], 0, 0, 0);
         }
-        if (s + 1 < stages) land(s + 1);
-        __syncthreads();
+        if constexpr (!DIRECT) if (s + 1 < stages) land(s + 1);
     }
+    __syncthreads();
 
     // The way out.  b is the matrix instruction's first operand: lane l holds row l % 32 of a and columns 8 (i / 4) + 4 (l / 32) + i % 4, four
     // neighbours of a row of y at a time.  They cross a strip of LDS of the wave's own (32 rows, its columns) so that a store takes whole
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     __syncthreads();
     auto put = [&](auto *y) {
         using Y = std::remove_pointer_t<decltype(y)>;
-        constexpr int kCols = CT * 32, kRow = kCols * sizeof(Y) + 16, kLanes = kCols * sizeof(Y) / 16, kE = 16 / sizeof(Y);       // (16 bytes more a row: other banks)
+        constexpr int kCols = CT * 32, kRow = kCols * sizeof(Y) + 16, kLanes = kCols * sizeof(Y) / 16, kRows = 64 / kLanes, kE = 16 / sizeof(Y);       // (16 bytes more a row: other banks)
         unsigned char *const strip = smem + (TM + 2 * TN) * 4 + wave * 32 * (kCols * 4 + 16);
         const bool biased = G.bias != nullptr;
         const int n1 = wn * (TN / WN) + lane % kLanes * kE;      // of the tile: this lane's columns on the way out
@@ -194,9 +197,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
             const int m1 = wm * (TM / WM) + r * 32 + lane / kLanes;
             Y *p = y + (m0 + m1) * G.ldy + n0 + n1;
 #pragma unroll
-            for (int i = 0; i < 32 * kLanes / 64; ++i) {
-                const i32x4 w = *reinterpret_cast<const i32x4 *>(strip + (lane / kLanes + i * (64 / kLanes)) * kRow + lane % kLanes * 16);
-                if (m1 + i * (64 / kLanes) <= last_a) {
+            for (int i = 0; i < 32 / kRows; ++i) {
+                const i32x4 w = *reinterpret_cast<const i32x4 *>(strip + (lane / kLanes + i * kRows) * kRow + lane % kLanes * 16);
+                if (m1 + i * kRows <= last_a) {
                     if (n1 + kE - 1 <= last_b) *reinterpret_cast<i32x4_any *>(p) = w;
                     else {
                         Y v[kE];
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
                         for (int e = 0; e < kE; ++e) if (n1 + e <= last_b) p[e] = v[e];
                     }
                 }
-                p += (64 / kLanes) * G.ldy;
+                p += kRows * G.ldy;
             }
         }
     };
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     else put(static_cast<__half *>(G.y));
 }
 
-template <int TM, int TN, int WM, int WN> static int tiles_launch(const GemmArgs &G, hipStream_t st)
+template <int TM, int TN, int WM, int WN, int STAGES> static int tiles_launch(const GemmArgs &G, hipStream_t st)
 {
     TileArgs T;
     T.g = G;
@@ -223,30 +226,33 @@ template <int TM, int TN, int WM, int WN> static int tiles_launch(const GemmArgs
     if (T.tiles_m > (1 << 28) / T.tiles_n) return IGCN_E_SHAPE;
     T.per_xcd = (T.tiles_m * T.tiles_n + 7) / 8;
     const bool direct = ((reinterpret_cast<uintptr_t>(G.a) | reinterpret_cast<uintptr_t>(G.b) | (uintptr_t)G.lda | (uintptr_t)G.ldb | (uintptr_t)G.k) & 15) == 0;
-    const size_t stages = (size_t)(G.k > kDepth ? 2 : 1) * (TM + TN) * kDepth, out = (TM + 2 * TN) * 4 + WM * WN * 32 * (TN / WN * 4 + 16);
-    const size_t lds = stages > out ? stages : out;
-    const void *kernel = direct ? reinterpret_cast<const void *>(tiles_i8_kernel<TM, TN, WM, WN, true>) : reinterpret_cast<const void *>(tiles_i8_kernel<TM, TN, WM, WN, false>);
-    if (lds > 65536) {                                           // (once would do; it is a host call of well under a microsecond)
-        const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return (int)e;
-    }
-    if (direct) hipLaunchKernelGGL((tiles_i8_kernel<TM, TN, WM, WN, true>), dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
-    else hipLaunchKernelGGL((tiles_i8_kernel<TM, TN, WM, WN, false>), dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
-    return launch_status();
+    auto launch = [&](auto *kernel, int most) {
+        int64_t stages = (G.k + kDepth - 1) / kDepth;
+        stages = stages < most ? stages : most;
+        const size_t in = (size_t)stages * (TM + TN) * kDepth, out = (TM + 2 * TN) * 4 + WM * WN * 32 * (TN / WN * 4 + 16), lds = in > out ? in : out;
+        if (lds > 65536) {                                       // (once would do; it is a host call of well under a microsecond)
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return (int)e;
+        }
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
+        return launch_status();
+    };
+    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false>, 2);
 }
 
-// ---- few rows of a --------------------------------------------------------------------------------------------------------------------
+// ---- up to 16 rows of a ---------------------------------------------------------------------------------------------------------------
 // Bound by the bytes of b, each used once: no tile of b is worth staging.  A wave takes 16 rows of b as the matrix instruction's first
-// operand straight from memory (16x16x64: lane l holds row l % 16, 16 bytes at 16 (l / 16)) and the rows of a, the second operand, from
-// LDS, where a workgroup lays them out once in the order the lanes read them: [64 codes of depth][16 of them][row][16 bytes].  Rows of a are rounded up to a
-// power of two there (lanes past it read another row's bytes; what they compute is not stored).  SHARE: with a long depth the four waves
-// of a workgroup take a quarter of it each and add their sums up in LDS (whole numbers: in any order), which fills the card four
-// times as well where b has few rows; with a short one every wave has tiles of its own.  KEEP loads are in flight before the first use.
+// operand straight from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and the rows of a, the second
+// operand, from LDS, where a workgroup lays them out once in the order the lanes read them: [64 codes of depth][16 of them][row][16 bytes].
+// Rows of a are rounded up to a power of two there (lanes past it read another row's bytes; what they compute is not stored).
+// SHARE: with a long depth the four waves of a workgroup take a quarter of it each and add their sums up in LDS (whole numbers: in any
+// order), which fills the card four times as well where b has few rows; with a short one every wave has TILES of its own.  KEEP loads of
+// a wave are under way at a time, the first ones before the rows of a are laid out: their time hides behind the bytes of b.
 // x in floating point (X is not int8_t): every workgroup makes it 8-bit on the way, with the quantiser's own steps — no launch, no
 // buffer; worth it while that is less work than a launch (kFusedValues).
 constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
-constexpr int kFewRows = 64;                                     // rows of a: 16 GROUPS
-constexpr int kPanelBytes = 32768;                               // of LDS: five workgroups on a CU
+constexpr int kFewRows = 16;
+constexpr int kPanelBytes = 32768;                               // of LDS for the rows of a: four workgroups on a CU
 constexpr int64_t kFusedValues = 8192;
 
 struct FewArgs {
@@ -257,7 +263,7 @@ struct FewArgs {
     int64_t jobs;                                                // of a workgroup at most: tile groups it walks
 };
 
-template <int GROUPS, int TILES, int KEEP, bool SHARE, typename X>
+template <int TILES, int KEEP, bool SHARE, typename X>
 __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -266,81 +272,104 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     i32x4 *const xs = reinterpret_cast<i32x4 *>(smem);           // [step][quarter][row] x 16 bytes
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
     const int rows2 = 1 << F.shift, m = (int)G.m;
-    int *const sums = reinterpret_cast<int *>(smem + (int64_t)F.panel * kStep * rows2);       // SHARE: [tile, group, wave][row of a][17]
-    const int64_t steps = (G.k + kStep - 1) / kStep, tiles = (G.n + 15) / 16;
+    int *const sums = reinterpret_cast<int *>(smem + (int64_t)F.panel * kStep * rows2);       // SHARE: [tile, wave][row of a][17]
+    const int steps = (int)((G.k + kStep - 1) / kStep), whole = (int)(G.k / kStep);
+    const int64_t tiles = (G.n + 15) / 16;
     const int64_t group0 = (int64_t)blockIdx.x * F.jobs * (SHARE ? 1 : 4) + (SHARE ? 0 : wave);
     constexpr bool kFloat = !std::is_same<X, int8_t>::value;
+
+    const int8_t *row[TILES];
+    i32x4 v[KEEP][TILES], acc[TILES];
+    auto rows_of = [&](int64_t tile0) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int64_t r = (tile0 + t) * 16 + (lane & 15);
+            row[t] = G.b + (r < G.n ? r : G.n - 1) * G.ldb + 16 * quarter;
+        }
+    };
+    auto load = [&](int s) {                                     // steps s ... s + KEEP - 1, all of them whole
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u)
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) v[u][t] = *reinterpret_cast<const i32x4_any *>(row[t] + (int64_t)(s + u) * kStep);
+    };
+    auto range = [&](int p0, int &from, int &to) {               // this wave's steps of the panel from p0 on
+        const int p1 = min(p0 + F.panel, steps);
+        from = SHARE ? p0 + (p1 - p0) * wave / 4 : p0;
+        to = SHARE ? p0 + (p1 - p0) * (wave + 1) / 4 : p1;
+        return p1;
+    };
+    int from, to;
+    bool loaded = false;
+    if (group0 * TILES < tiles) {                                // the first loads, before anything else
+        range(0, from, to);
+        rows_of(group0 * TILES);
+        if (from + KEEP <= min(to, whole)) { load(from); loaded = true; }
+    }
 
     if constexpr (kFloat) {                                      // (one panel: the whole depth)
         constexpr int E = Chunk<X>::kValues;
         for (int r = wave; r < m; r += 4) {
-            const X *row = static_cast<const X *>(F.x) + r * F.ldx;
+            const X *from_x = static_cast<const X *>(F.x) + r * F.ldx;
             uint32_t big = 0u;
-            for (int64_t at = lane * E; at < G.k; at += 64 * E) { Chunk<X> c; c.load(row + at, G.k - at); big = c.largest(big); }
+            for (int at = lane * E; at < G.k; at += 64 * E) { Chunk<X> c; c.load(from_x + at, G.k - at); big = c.largest(big); }
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off));
             const RowScale s(big);
             if (lane == 0) sx[r] = s.s;
-            for (int64_t at = lane * E; at < steps * kStep; at += 64 * E) {
+            for (int at = lane * E; at < steps * kStep; at += 64 * E) {
                 Chunk<X> c;
-                c.load(row + at, G.k - at);
-                uint32_t w[E / 4] = {};
-#pragma unroll
-                for (int i = 0; i < E; ++i) w[i >> 2] |= (uint32_t)(s.code(c.v[i]) & 0xff) << (8 * (i & 3));
+                uint32_t w[E / 4];
+                c.load(from_x + at, G.k - at);
+                pack_codes<X>(w, c, s);
                 __builtin_memcpy(smem + ((at >> 4) * rows2 + r) * 16 + (at & 15), w, E);
             }
         }
     } else if (threadIdx.x < m) sx[threadIdx.x] = G.sa[threadIdx.x];
     __syncthreads();
 
-    i32x4 acc[TILES][GROUPS];
     for (int64_t job = 0; job < F.jobs; ++job) {
         const int64_t tile0 = (group0 + job * (SHARE ? 1 : 4)) * TILES;
         if (SHARE ? tile0 >= tiles : tile0 - (int64_t)wave * TILES >= tiles) break;          // (the same for the whole workgroup)
-        const int8_t *row[TILES];
+        if (job) { rows_of(tile0); loaded = false; }
+        else if (tile0 >= tiles) rows_of(tile0);
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const int64_t r = (tile0 + t) * 16 + (lane & 15);
-            row[t] = G.b + (r < G.n ? r : G.n - 1) * G.ldb + 16 * quarter;
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) acc[t][g] = i32x4{0, 0, 0, 0};
-        }
-        for (int64_t p0 = 0; p0 < steps; p0 += F.panel) {
-            const int64_t p1 = p0 + F.panel < steps ? p0 + F.panel : steps;
+        for (int t = 0; t < TILES; ++t) acc[t] = i32x4{0, 0, 0, 0};
+        for (int p0 = 0; p0 < steps; p0 += F.panel) {
+            const int p1 = range(p0, from, to);
             if constexpr (!kFloat) if (job == 0 || F.panel < steps) {
                 __syncthreads();
-                for (int64_t i = threadIdx.x; i < (p1 - p0) * 4 * rows2; i += kBlock) {
-                    const int64_t r = i & (rows2 - 1), piece = i >> F.shift;
-                    xs[i] = r < m ? load16(G.a + r * G.lda, (p0 * 4 + piece) * 16, G.k) : i32x4{0, 0, 0, 0};
+                for (int i = threadIdx.x; i < (p1 - p0) * 4 * rows2; i += kBlock) {
+                    const int r = i & (rows2 - 1), piece = i >> F.shift;
+                    xs[i] = r < m ? load16(G.a + r * G.lda, (int64_t)(p0 * 4 + piece) * 16, G.k) : i32x4{0, 0, 0, 0};
                 }
                 __syncthreads();
             }
-            const int64_t from = SHARE ? p0 + (p1 - p0) * wave / 4 : p0, to = SHARE ? p0 + (p1 - p0) * (wave + 1) / 4 : p1;
-            auto multiply = [&](const i32x4 (&v)[TILES], int64_t s) {
-                const i32x4 *x = xs + ((s - p0) * 4 + quarter) * rows2;
+            auto multiply = [&](const i32x4 (&w)[TILES], int s) {
+                const i32x4 xv = xs[((s - p0) * 4 + quarter) * rows2 + (lane & 15 & (rows2 - 1))];
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const i32x4 xv = x[(g * 16 + (lane & 15)) & (rows2 - 1)];
-#pragma unroll
-                    for (int t = 0; t < TILES; ++t) acc[t][g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[t], xv, acc[t][g], 0, 0, 0);
-                }
+                for (int t = 0; t < TILES; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t], xv, acc[t], 0, 0, 0);
             };
-            const int64_t whole = G.k / kStep < to ? G.k / kStep : to;
-            int64_t s = from;
-            for (; s + KEEP <= whole; s += KEEP) {
-                i32x4 v[KEEP][TILES];
+            const int full = min(to, whole);
+            int s = from;
+            if (s + KEEP <= full && !loaded) load(s);
+            loaded = false;
+            while (s + KEEP <= full) {
+                i32x4 w[KEEP][TILES];
 #pragma unroll
                 for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-                    for (int t = 0; t < TILES; ++t) v[u][t] = *reinterpret_cast<const i32x4_any *>(row[t] + (s + u) * kStep);
+                    for (int t = 0; t < TILES; ++t) w[u][t] = v[u][t];
+                s += KEEP;
+                if (s + KEEP <= full) load(s);                   // the next ones while these are multiplied
 #pragma unroll
-                for (int u = 0; u < KEEP; ++u) multiply(v[u], s + u);
+                for (int u = 0; u < KEEP; ++u) multiply(w[u], s - KEEP + u);
             }
             for (; s < to; ++s) {
-                i32x4 v[TILES];
+                i32x4 w[TILES];
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) v[t] = load16(row[t] - 16 * quarter, s * kStep + 16 * quarter, G.k);
-                multiply(v, s);
+                for (int t = 0; t < TILES; ++t) w[t] = load16(row[t] - 16 * quarter, (int64_t)s * kStep + 16 * quarter, G.k);
+                multiply(w, s);
             }
         }
         if constexpr (SHARE) {                                   // lane l holds rows of b 4 (l / 16) + i, row l % 16 of a
@@ -348,42 +377,33 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const int at = (t * GROUPS + g) * 4 + wave;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sums[(at * 16 + (lane & 15)) * 17 + 4 * quarter + i] = acc[t][g][i];
-                }
+                for (int i = 0; i < 4; ++i) sums[((t * 4 + wave) * 16 + (lane & 15)) * 17 + 4 * quarter + i] = acc[t][i];
             __syncthreads();
             const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
+            for (int t = 0; t < TILES; ++t) {
+                const int64_t n = (tile0 + t) * 16 + c;
+                if (n < G.n && r < m) {
+                    int sum = 0;
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const int64_t n = (tile0 + t) * 16 + c;
-                    const int mm = g * 16 + r;
-                    if (n < G.n && mm < m) {
-                        int sum = 0;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) sum += sums[(((t * GROUPS + g) * 4 + w) * 16 + r) * 17 + c];
-                        store_out(G, mm, n, scaled(sum, sx[mm], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
-                    }
+                    for (int w = 0; w < 4; ++w) sum += sums[((t * 4 + w) * 16 + r) * 17 + c];
+                    store_out(G, r, n, scaled(sum, sx[r], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
                 }
+            }
         } else {
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
+            for (int t = 0; t < TILES; ++t) {
+                const int r = lane & 15;
+                const int64_t n0 = (tile0 + t) * 16 + 4 * quarter;
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const int mm = g * 16 + (lane & 15);
-                    const int64_t n0 = (tile0 + t) * 16 + 4 * quarter;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (mm < m && n0 + i < G.n) store_out(G, mm, n0 + i, scaled(acc[t][g][i], sx[mm], G.sb[n0 + i], G.bias != nullptr, G.bias ? G.bias[n0 + i] : 0.f));
-                }
+                for (int i = 0; i < 4; ++i)
+                    if (r < m && n0 + i < G.n) store_out(G, r, n0 + i, scaled(acc[t][i], sx[r], G.sb[n0 + i], G.bias != nullptr, G.bias ? G.bias[n0 + i] : 0.f));
+            }
         }
     }
 }
 
-template <int GROUPS, typename X> static int few_rows_launch(FewArgs F, hipStream_t st)
+template <typename X> static int few_rows(FewArgs F, hipStream_t st)
 {
     const int64_t steps = (F.g.k + kStep - 1) / kStep, tiles = (F.g.n + 15) / 16;
     F.shift = 0;
@@ -391,30 +411,23 @@ template <int GROUPS, typename X> static int few_rows_launch(FewArgs F, hipStrea
     const int64_t fits = kPanelBytes / (kStep << F.shift);
     F.panel = (int)(steps < fits ? (steps ? steps : 1) : fits);
     const bool share = steps >= 16;                              // a quarter of the depth is a batch of loads at least
-    const bool one_panel = F.panel >= steps;
-    constexpr int kTilesOwn = GROUPS == 1 ? 4 : GROUPS == 2 ? 2 : 1;
-    const int64_t per = share ? 1 : 4 * kTilesOwn, groups = (tiles + per - 1) / per;
+    constexpr int kOwn = 4;
+    const int64_t per = share ? 1 : 4 * kOwn, groups = (tiles + per - 1) / per;
     // a workgroup that lays the rows of a out once and walks several tiles with them: as many as keep 2 048 workgroups busy
-    F.jobs = one_panel ? (groups + 2047) / 2048 : 1;
+    F.jobs = F.panel >= steps ? (groups + 2047) / 2048 : 1;
     const int64_t blocks = (groups + F.jobs - 1) / F.jobs;
     if (blocks > 0x7fffffff) return IGCN_E_SHAPE;
-    const size_t lds = ((size_t)F.panel * kStep << F.shift) + (share ? (size_t)GROUPS * 4 * 16 * 17 * 4 : 0);
-    const dim3 grid((unsigned)blocks);
-    if (share) hipLaunchKernelGGL((few_rows_i8_kernel<GROUPS, 1, 4, true, X>), grid, dim3(kBlock), lds, st, F);
-    else hipLaunchKernelGGL((few_rows_i8_kernel<GROUPS, kTilesOwn, 1, false, X>), grid, dim3(kBlock), lds, st, F);
+    const size_t lds = ((size_t)F.panel * kStep << F.shift) + (share ? 4 * 16 * 17 * 4 : 0);
+    if (share) hipLaunchKernelGGL((few_rows_i8_kernel<1, 4, true, X>), dim3((unsigned)blocks), dim3(kBlock), lds, st, F);
+    else hipLaunchKernelGGL((few_rows_i8_kernel<kOwn, 1, false, X>), dim3((unsigned)blocks), dim3(kBlock), lds, st, F);
     return launch_status();
-}
-
-template <typename X> static int few_rows(const FewArgs &F, hipStream_t st)
-{
-    return F.g.m <= 16 ? few_rows_launch<1, X>(F, st) : F.g.m <= 32 ? few_rows_launch<2, X>(F, st) : few_rows_launch<4, X>(F, st);
 }
 
 static int product(const GemmArgs &G, hipStream_t st)
 {
     if (G.m <= kFewRows || G.lda > kMostApart || G.ldb > kMostApart) {
         const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
-        for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 64 at a time)
+        for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 16 at a time)
             FewArgs F = {};
             F.g = G;
             F.g.a += at * G.lda;
@@ -426,9 +439,12 @@ static int product(const GemmArgs &G, hipStream_t st)
         }
         return IGCN_OK;
     }
-    // 256 x 256 tiles read each code half as often as 128 x 128 ones, and there have to be enough of them for 256 CUs
-    const int64_t large = ((G.m + 255) / 256) * ((G.n + 255) / 256);
-    return large >= 200 && G.k >= 512 ? tiles_launch<256, 256, 2, 4>(G, st) : tiles_launch<128, 128, 2, 2>(G, st);
+    auto tiles = [&](int64_t tm, int64_t tn) { return ((G.m + tm - 1) / tm) * ((G.n + tn - 1) / tn); };
+    if (G.m <= 64) return tiles_launch<64, 64, 2, 2, 4>(G, st);
+    if (G.k <= kDepth && G.out == IGCN_DTYPE_F32) return tiles_launch<64, 128, 2, 4, 2>(G, st);
+    if (G.k > kDepth && tiles(256, 256) >= 200) return tiles_launch<256, 256, 2, 4, 2>(G, st);
+    if (tiles(128, 128) >= 200) return tiles_launch<128, 128, 2, 2, 2>(G, st);
+    return tiles_launch<64, 64, 2, 2, 4>(G, st);
 }
 
 static int check_product(const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias, int64_t m, int64_t n, int64_t k, const void *y,

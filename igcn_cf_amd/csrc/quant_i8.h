@@ -52,12 +52,39 @@ struct RowScale {
     }
 };
 
+// The codes of a piece, packed.  x inv + 1.5 2^23 in one operation leaves the nearest whole number in the low bits; off by at most
+// 127 2^-24 before that rounding, it is the right one unless what was cut off is within 2^-16 of a half: a wave that meets such a
+// value (one in 30 000) takes the exact way for the piece.  5 instructions a value instead of 16: at 16 they took as long as the bytes.
+template <typename T> __device__ __forceinline__ void pack_codes(uint32_t (&w)[Chunk<T>::kValues / 4], const Chunk<T> &c, const RowScale &s)
+{
+    constexpr int E = Chunk<T>::kValues;
+    constexpr float kMagic = 12582912.f, kNear = 0.5f - 0x1p-16f;
+    float near = 0.f;
+    uint32_t b[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float m = fmaf(c.v[i], s.inv, kMagic);
+        near = fmaxf(near, fabsf(fmaf(c.v[i], s.inv, kMagic - m)));
+        b[i] = __float_as_uint(m);
+    }
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {                            // the low bytes of four words
+        const uint32_t lo = __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x04000c0cu);
+        w[i] = s.inv > 0.f ? lo | hi : 0u;                       // (a row of zeros, or one that is broken)
+    }
+    if (__any((near >= kNear || s.s < 0x1p-120f) && s.inv > 0.f)) {
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) w[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i >> 2] |= (uint32_t)(s.code(c.v[i]) & 0xff) << (8 * (i & 3));
+    }
+}
+
 template <typename T> __device__ __forceinline__ void store_codes(int8_t *__restrict__ q, int64_t left, const Chunk<T> &c, const RowScale &s)
 {
     constexpr int E = Chunk<T>::kValues;
-    uint32_t w[E / 4] = {};
-#pragma unroll
-    for (int i = 0; i < E; ++i) w[i >> 2] |= (uint32_t)(s.code(c.v[i]) & 0xff) << (8 * (i & 3));
+    uint32_t w[E / 4];
+    pack_codes<T>(w, c, s);
     if (left >= E) __builtin_memcpy(q, w, E);
     else {
 #pragma unroll

@@ -19,19 +19,21 @@ template <int L> __device__ __forceinline__ uint32_t group_max(uint32_t m, uint3
     if constexpr (L > kWave) {
         if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x >> 6] = m;
         __syncthreads();
-        m = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+        m = lds[0];
+#pragma unroll
+        for (int i = 1; i < L / kWave; ++i) m = max(m, lds[i]);
     }
     return m;
 }
 
 template <typename T, int L, int I, int R>
-__global__ __launch_bounds__(kBlock) void quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int64_t k, int8_t *__restrict__ q,
+__global__ __launch_bounds__(L > kBlock ? L : kBlock) void quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int64_t k, int8_t *__restrict__ q,
                                                                int64_t ldq, float *__restrict__ scale)
 {
-    constexpr int E = Chunk<T>::kValues;
-    __shared__ uint32_t lds[kBlock / kWave];
+    constexpr int E = Chunk<T>::kValues, kThreads = L > kBlock ? L : kBlock;
+    __shared__ uint32_t lds[kThreads / kWave];
     const int lane = threadIdx.x & (L - 1);
-    const int64_t r0 = ((int64_t)blockIdx.x * (kBlock / L) + threadIdx.x / L) * R;
+    const int64_t r0 = ((int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L) * R;
     Chunk<T> c[R][I];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -119,8 +121,9 @@ __global__ __launch_bounds__(kBlock) void dequantize_rows_kernel(const int8_t *_
 template <typename T, int L, int I, int R>
 static int quantize_launch(const T *x, int64_t ldx, int64_t rows, int64_t k, int8_t *q, int64_t ldq, float *scale, hipStream_t st)
 {
-    const int64_t per = (int64_t)(kBlock / L) * R;
-    hipLaunchKernelGGL((quantize_rows_kernel<T, L, I, R>), dim3((unsigned)((rows + per - 1) / per)), dim3(kBlock), 0, st, x, ldx, rows, k, q, ldq, scale);
+    constexpr int kThreads = L > kBlock ? L : kBlock;
+    const int64_t per = (int64_t)(kThreads / L) * R;
+    hipLaunchKernelGGL((quantize_rows_kernel<T, L, I, R>), dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, st, x, ldx, rows, k, q, ldq, scale);
     return launch_status();
 }
 
@@ -135,6 +138,9 @@ template <typename T> static int quantize(const void *xv, int64_t ldx, int64_t r
     if (pieces <= 64) return quantize_launch<T, 64, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 128) return quantize_launch<T, 64, 2, 2>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 256) return quantize_launch<T, 64, 4, 1>(x, ldx, rows, k, q, ldq, scale, st);
+    // few rows: a row's time is what counts, so 1 024 lanes share it (4 rows of 8192 bfloat16: see the figures above)
+    if (pieces > 256 && rows <= 256 && pieces <= 1024) return quantize_launch<T, 1024, 1, 1>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces > 256 && rows <= 256 && pieces <= 2048) return quantize_launch<T, 1024, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 512) return quantize_launch<T, kBlock, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 1024) return quantize_launch<T, kBlock, 4, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= kHeldPieces) return quantize_launch<T, kBlock, 8, 1>(x, ldx, rows, k, q, ldq, scale, st);
