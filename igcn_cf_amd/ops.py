@@ -864,14 +864,17 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and weight_decay >= 0.):
         raise _lib.IgcnError('betas must be in [0, 1), eps and weight_decay not negative')
     device = _check_grads(grads)
-    every = params + exp_avgs + exp_avg_sqs + steps + (scales if eight else [])
-    if n and {t.get_device() for t in every} != {device.index}:
+    if n and {t.get_device() for ts in (params, exp_avgs, exp_avg_sqs, steps, scales if eight else ()) for t in ts} != {device.index}:
         raise _lib.IgcnError('the tensors of a call must be on one device, a GPU')
+    pt, gt = [p.dtype for p in params], [g.dtype for g in grads]
     want = MOMENT_DTYPES if eight else (torch.float32, torch.float32)
+    if not all(p in _DTYPE_CODES for p in pt) or any(g != p and g != torch.float32 for p, g in zip(pt, gt)) \
+            or any(m.dtype != want[0] for m in exp_avgs) or any(v.dtype != want[1] for v in exp_avg_sqs):
+        raise _lib.IgcnError('parameters: float32, bfloat16 or float16; gradients: the same or float32; moments: float32, or with scales '
+                             'float8_e4m3fn and float8_e5m2 (got %s, %s, %s, %s)' % tuple({t.dtype for t in ts} for ts in (params, grads, exp_avgs, exp_avg_sqs)))
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
-        if p.dtype not in _DTYPE_CODES or (g.dtype != p.dtype and g.dtype != torch.float32) or m.dtype != want[0] or v.dtype != want[1]:
-            raise _lib.IgcnError('parameters: float32, bfloat16 or float16; gradients: the same or float32; moments: float32, or with scales '
-                                 'float8_e4m3fn and float8_e5m2 (got %s, %s, %s, %s)' % (p.dtype, g.dtype, m.dtype, v.dtype))
+        if p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous() and p.shape == g.shape == m.shape == v.shape:
+            continue
         if not (_same_order(p, g) and _same_order(p, m) and _same_order(p, v)):
             raise _lib.IgcnError('gradient and moments must have the shape and the order in memory of their parameter')
     sizes = [p.numel() for p in params]
@@ -883,8 +886,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     written = [a for column in at for a in column if a]                                  # (an empty tensor has no address)
     if len(set(written)) != len(written):
         raise _lib.IgcnError('a tensor stands in the lists twice: every parameter, moment and step is rewritten by one place only')
-    rows = array.array('q', [x for p, g, m, v, s, t, k, pt, gt in zip(at[0], grads, at[1], at[2], scales, at[3], sizes, params, grads)
-                             for x in (p, g.data_ptr(), m, v, s.data_ptr() if eight else 0, t, k, _DTYPE_CODES[pt.dtype] | _DTYPE_CODES[gt.dtype] << 32)])
+    at[1:1] = [[g.data_ptr() for g in grads]]
+    at[4:4] = [[s.data_ptr() for s in scales] if eight else [0] * n]
+    rows = array.array('q', [x for row in zip(*at, sizes, [_DTYPE_CODES[p] | _DTYPE_CODES[g] << 32 for p, g in zip(pt, gt)]) for x in row])
     lr_dev = norm_in = None
     if isinstance(lr, torch.Tensor):
         if lr.dtype != torch.float32 or lr.numel() != 1 or (n and lr.device != device):
@@ -901,13 +905,16 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     with _on(device):
         L, table = _lib.lib(), rows.buffer_info()[0]
         ws = torch.empty(L.igcn_adamw_workspace_bytes(table, n), dtype=torch.uint8, device=device)
-        norm = norm_in
-        if max_grad_norm is not None and norm is None:
-            norm = torch.empty((), dtype=torch.float32, device=device)
-        _lib.check(L.igcn_adamw_step(table, n, 8 if eight else 32, float(lr), _lib.ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
-                                     float(weight_decay), 0. if max_grad_norm is None else float(max_grad_norm), _lib.ptr(norm_in),
-                                     _lib.ptr(norm) if norm_in is None else None, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(),
-                                     _lib.current_stream()), 'igcn_adamw_step')
+        norm, max_norm, norm_out = norm_in, 0., None
+        if max_grad_norm is not None:
+            max_norm = max_grad_norm
+            if norm_in is None:
+                norm = torch.empty((), dtype=torch.float32, device=device)
+                norm_out = norm.data_ptr()
+        code = L.igcn_adamw_step(table, n, 8 if eight else 32, lr, _lib.ptr(lr_dev), betas[0], betas[1], eps, weight_decay, max_norm, _lib.ptr(norm_in),
+                                 norm_out, seed & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), _lib.current_stream())
+        if code:
+            _lib.check(code, 'igcn_adamw_step')
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
     return norm
 
