@@ -48,8 +48,8 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int64_t 
 // 32 x 32 pieces (v_mfma_i32_32x32x32_i8: lane l holds row l % 32, 16 bytes of depth at 16 (l / 32)).  128 codes of depth of either side
 // go to LDS per stage, two stages in turn: the next one is on its way from memory while this one is multiplied, one barrier a stage.
 // DIRECT (rows 16-byte aligned, depth a multiple of 16): memory to LDS without registers (global_load_lds, 1 KiB a wave and
-// instruction, lane after lane); else through registers.  A row's eight 16-byte pieces stand in LDS at piece ^ (row % 8): 8 lanes that read the
-// same piece of 8 neighbouring rows hit different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
+// instruction, lane after lane); else through registers.  A row's eight 16-byte pieces stand in LDS at piece ^ (row / 2 % 8): 16 lanes that read the
+// same piece of 16 neighbouring rows hit 64 different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
 // Depth past the end reads a block of zeros, rows past the end the last row (not stored).
 // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, 4 tiles of a deep at a time, so that the tiles under way there
 // share their rows in its L2.
@@ -91,15 +91,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     const int64_t band = t / (bd * T.tiles_n), in = t - band * bd * T.tiles_n, high = T.tiles_m - bd * band < bd ? T.tiles_m - bd * band : bd;
     const int64_t m0 = (bd * band + in % high) * TM, n0 = in / high * TN;
 
-    // this lane's pieces: rows 8 (wave NA + i) + lane / 8 of the tile, piece (lane % 8) ^ (row % 8); offsets from the tile's first row fit 32 bits
-    const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+    // this lane's pieces: rows 8 (wave NA + i) + lane / 8 of the tile, piece (lane % 8) ^ (row / 2 % 8); offsets from the tile's first row fit 32 bits
+    auto piece = [&](int i) { return ((lane & 7) ^ ((4 * i + (lane >> 4)) & 7)) * 16; };       // ... of rows 8 i ... 8 i + 7
     const int8_t *const base_a = G.a + m0 * G.lda, *const base_b = G.b + n0 * G.ldb;
     const int last_a = (int)(G.m - m0 < TM ? G.m - m0 : TM) - 1, last_b = (int)(G.n - n0 < TN ? G.n - n0 : TN) - 1;
     unsigned oa[NA], ob[NB];
 #pragma unroll
-    for (int i = 0; i < NA; ++i) oa[i] = (unsigned)min(8 * (wave * NA + i) + (lane >> 3), last_a) * (unsigned)G.lda + piece;
+    for (int i = 0; i < NA; ++i) oa[i] = (unsigned)min(8 * (wave * NA + i) + (lane >> 3), last_a) * (unsigned)G.lda + piece(wave * NA + i);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) ob[i] = (unsigned)min(8 * (wave * NB + i) + (lane >> 3), last_b) * (unsigned)G.ldb + piece;
+    for (int i = 0; i < NB; ++i) ob[i] = (unsigned)min(8 * (wave * NB + i) + (lane >> 3), last_b) * (unsigned)G.ldb + piece(wave * NB + i);
     const int64_t stages = (G.k + kDepth - 1) / kDepth;
     i32x4 held[DIRECT ? 1 : NA + NB];
     const unsigned lds0 = (unsigned)(uintptr_t)(lds_void *)smem;
@@ -114,17 +114,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
                 for (int i = 0; i < NB; ++i) to_lds(base_b + k0, ob[i], bt + 1024 * i);
             } else {                                             // (pieces are whole: the depth is a multiple of 16)
-                const bool there = k0 + piece < G.k;
 #pragma unroll
-                for (int i = 0; i < NA; ++i) to_lds(there ? (const void *)(base_a + k0 + oa[i]) : (const void *)&g_zeros, at + 1024 * i);
+                for (int i = 0; i < NA; ++i) to_lds(k0 + piece(wave * NA + i) < G.k ? (const void *)(base_a + k0 + oa[i]) : (const void *)&g_zeros, at + 1024 * i);
 #pragma unroll
-                for (int i = 0; i < NB; ++i) to_lds(there ? (const void *)(base_b + k0 + ob[i]) : (const void *)&g_zeros, bt + 1024 * i);
+                for (int i = 0; i < NB; ++i) to_lds(k0 + piece(wave * NB + i) < G.k ? (const void *)(base_b + k0 + ob[i]) : (const void *)&g_zeros, bt + 1024 * i);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NA; ++i) held[i] = load16(base_a + oa[i] - piece, k0 + piece, G.k);
+            for (int i = 0; i < NA; ++i) held[i] = load16(base_a + oa[i] - piece(wave * NA + i), k0 + piece(wave * NA + i), G.k);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + ob[i] - piece, k0 + piece, G.k);
+            for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + ob[i] - piece(wave * NB + i), k0 + piece(wave * NB + i), G.k);
         }
     };
     auto land = [&](int64_t s) {                                 // registers to LDS
@@ -137,7 +136,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 
     i32x16 acc[RT][CT] = {};
     const int wm = wave / WN, wn = wave % WN;
-    const int ra = wm * (TM / WM) + (lane & 31), rb = wn * (TN / WN) + (lane & 31), half = lane >> 5, turn = lane & 7;
+    const int ra = wm * (TM / WM) + (lane & 31), rb = wn * (TN / WN) + (lane & 31), half = lane >> 5, turn = (lane >> 1) & 7;
     if constexpr (DIRECT) {
         for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s);
     } else if (stages) { fetch(0); land(0); }
