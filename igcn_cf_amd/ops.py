@@ -6,6 +6,7 @@ no eager/PyTorch fallback — a missing library or a non-GPU tensor raises.
 """
 import array
 import ctypes as C
+import itertools
 
 import torch
 
@@ -812,15 +813,16 @@ def _same_order(a, b):
 
 def _check_grads(grads):
     """The one device the gradients are on."""
-    device = grads[0].device if grads else None
-    for g in grads:
-        if not (isinstance(g, torch.Tensor) and g.is_cuda and g.layout == torch.strided and g.dtype in _DTYPE_CODES):
-            raise _lib.IgcnError('gradients must be dense float32, bfloat16 or float16 tensors on the GPU (no CPU path)')
-        if g.get_device() != device.index:
-            raise _lib.IgcnError('the tensors of a call must be on one device')
-        if not (g.is_contiguous() or _dense(g)):
-            raise _lib.IgcnError('gradients must fill a stretch of memory (a view with gaps or repeats does not)')
-    return device
+    if not grads:
+        return None
+    if not all(isinstance(g, torch.Tensor) for g in grads) or not all(g.is_cuda for g in grads) or {g.layout for g in grads} != {torch.strided} \
+            or not {g.dtype for g in grads} <= _DTYPE_CODES.keys():
+        raise _lib.IgcnError('gradients must be dense float32, bfloat16 or float16 tensors on the GPU (no CPU path)')
+    if len({g.get_device() for g in grads}) != 1:
+        raise _lib.IgcnError('the tensors of a call must be on one device')
+    if not all(g.is_contiguous() or _dense(g) for g in grads):
+        raise _lib.IgcnError('gradients must fill a stretch of memory (a view with gaps or repeats does not)')
+    return grads[0].device
 
 
 def grad_norm(grads):
@@ -868,8 +870,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
         raise _lib.IgcnError('the tensors of a call must be on one device, a GPU')
     pt, gt = [p.dtype for p in params], [g.dtype for g in grads]
     want = MOMENT_DTYPES if eight else (torch.float32, torch.float32)
-    if not all(p in _DTYPE_CODES for p in pt) or any(g != p and g != torch.float32 for p, g in zip(pt, gt)) \
-            or any(m.dtype != want[0] for m in exp_avgs) or any(v.dtype != want[1] for v in exp_avg_sqs):
+    if n and (not _DTYPE_CODES.keys() >= set(pt) or (pt != gt and any(g != p and g != torch.float32 for p, g in zip(pt, gt)))
+              or {m.dtype for m in exp_avgs} != {want[0]} or {v.dtype for v in exp_avg_sqs} != {want[1]}):
         raise _lib.IgcnError('parameters: float32, bfloat16 or float16; gradients: the same or float32; moments: float32, or with scales '
                              'float8_e4m3fn and float8_e5m2 (got %s, %s, %s, %s)' % tuple({t.dtype for t in ts} for ts in (params, grads, exp_avgs, exp_avg_sqs)))
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
@@ -878,9 +880,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
         if not (_same_order(p, g) and _same_order(p, m) and _same_order(p, v)):
             raise _lib.IgcnError('gradient and moments must have the shape and the order in memory of their parameter')
     sizes = [p.numel() for p in params]
-    if any(t.dtype != torch.float32 or t.numel() != 1 for t in steps):
+    if n and ({t.dtype for t in steps} != {torch.float32} or {t.numel() for t in steps} != {1}):
         raise _lib.IgcnError('steps must be one-element float32 tensors')
-    if eight and any(s.dtype != torch.float32 or s.shape != ((k + ADAMW_BLOCK - 1) // ADAMW_BLOCK, 2) or not s.is_contiguous() for s, k in zip(scales, sizes)):
+    if eight and not all(s.dtype is torch.float32 and s.is_contiguous() and s.shape == ((k + ADAMW_BLOCK - 1) // ADAMW_BLOCK, 2) for s, k in zip(scales, sizes)):
         raise _lib.IgcnError('scales must be contiguous float32 [ceil(numel / %d), 2]' % ADAMW_BLOCK)
     at = [[t.data_ptr() for t in ts] for ts in (params, exp_avgs, exp_avg_sqs, steps)]
     written = [a for column in at for a in column if a]                                  # (an empty tensor has no address)
@@ -888,7 +890,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
         raise _lib.IgcnError('a tensor stands in the lists twice: every parameter, moment and step is rewritten by one place only')
     at[1:1] = [[g.data_ptr() for g in grads]]
     at[4:4] = [[s.data_ptr() for s in scales] if eight else [0] * n]
-    rows = array.array('q', [x for row in zip(*at, sizes, [_DTYPE_CODES[p] | _DTYPE_CODES[g] << 32 for p, g in zip(pt, gt)]) for x in row])
+    rows = array.array('q', itertools.chain.from_iterable(zip(*at, sizes, [_DTYPE_CODES[p] | _DTYPE_CODES[g] << 32 for p, g in zip(pt, gt)])))
     lr_dev = norm_in = None
     if isinstance(lr, torch.Tensor):
         if lr.dtype != torch.float32 or lr.numel() != 1 or (n and lr.device != device):
