@@ -310,8 +310,9 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
         constexpr int E = Chunk<X>::kValues;
         for (int r = wave; r < m; r += 4) {
             const X *from_x = static_cast<const X *>(F.x) + r * F.ldx;
-            uint32_t big = 0u;
-            for (int at = lane * E; at < G.k; at += 64 * E) { Chunk<X> c; c.load(from_x + at, G.k - at); big = c.largest(big); }
+            Largest<X> most;
+            for (int at = lane * E; at < G.k; at += 64 * E) { Chunk<X> c; c.load(from_x + at, G.k - at); most.of(c); }
+            uint32_t big = most.bits();
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off));
             const RowScale s(big);

@@ -27,10 +27,10 @@ template <int L> __device__ __forceinline__ uint32_t group_max(uint32_t m, uint3
 }
 
 template <typename T, int L, int I, int R>
-__global__ __launch_bounds__(L > kBlock ? L : kBlock) void quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int64_t k, int8_t *__restrict__ q,
+__global__ __launch_bounds__(L > kWave ? L : kBlock) void quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int64_t k, int8_t *__restrict__ q,
                                                                int64_t ldq, float *__restrict__ scale)
 {
-    constexpr int E = Chunk<T>::kValues, kThreads = L > kBlock ? L : kBlock;
+    constexpr int E = Chunk<T>::kValues, kThreads = L > kWave ? L : kBlock;
     __shared__ uint32_t lds[kThreads / kWave];
     const int lane = threadIdx.x & (L - 1);
     const int64_t r0 = ((int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L) * R;
@@ -44,10 +44,10 @@ __global__ __launch_bounds__(L > kBlock ? L : kBlock) void quantize_rows_kernel(
         }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        uint32_t big = 0u;
+        Largest<T> big;
 #pragma unroll
-        for (int i = 0; i < I; ++i) big = c[r][i].largest(big);
-        const RowScale s(group_max<L>(big, lds));
+        for (int i = 0; i < I; ++i) big.of(c[r][i]);
+        const RowScale s(group_max<L>(big.bits(), lds));
         if (r0 + r >= rows) return;                              // (L > a wave: R is 1, the whole workgroup leaves)
         if (lane == 0) scale[r0 + r] = s.s;
 #pragma unroll
@@ -65,13 +65,13 @@ __global__ __launch_bounds__(kBlock) void quantize_long_rows_kernel(const T *__r
     constexpr int E = Chunk<T>::kValues;
     __shared__ uint32_t lds[kBlock / kWave];
     const T *row = x + blockIdx.x * ldx;
-    uint32_t big = 0u;
+    Largest<T> big;
     for (int64_t at = (int64_t)threadIdx.x * E; at < k; at += kBlock * E) {
         Chunk<T> c;
         c.load(row + at, k - at);
-        big = c.largest(big);
+        big.of(c);
     }
-    const RowScale s(group_max<kBlock>(big, lds));
+    const RowScale s(group_max<kBlock>(big.bits(), lds));
     if (threadIdx.x == 0) scale[blockIdx.x] = s.s;
     for (int64_t at = (int64_t)threadIdx.x * E; at < k; at += kBlock * E) {
         Chunk<T> c;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kBlock) void dequantize_rows_kernel(const int8_t *_
 template <typename T, int L, int I, int R>
 static int quantize_launch(const T *x, int64_t ldx, int64_t rows, int64_t k, int8_t *q, int64_t ldq, float *scale, hipStream_t st)
 {
-    constexpr int kThreads = L > kBlock ? L : kBlock;
+    constexpr int kThreads = L > kWave ? L : kBlock;
     const int64_t per = (int64_t)(kThreads / L) * R;
     hipLaunchKernelGGL((quantize_rows_kernel<T, L, I, R>), dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, st, x, ldx, rows, k, q, ldq, scale);
     return launch_status();
@@ -133,16 +133,16 @@ template <typename T> static int quantize(const void *xv, int64_t ldx, int64_t r
     const int64_t pieces = (k + Chunk<T>::kValues - 1) / Chunk<T>::kValues;
     if (pieces <= 4) return quantize_launch<T, 4, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 8) return quantize_launch<T, 8, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
-    if (pieces <= 16) return quantize_launch<T, 16, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
-    if (pieces <= 32) return quantize_launch<T, 32, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
-    if (pieces <= 64) return quantize_launch<T, 64, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
-    if (pieces <= 128) return quantize_launch<T, 64, 2, 2>(x, ldx, rows, k, q, ldq, scale, st);
-    if (pieces <= 256) return quantize_launch<T, 64, 4, 1>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces <= 16) return quantize_launch<T, 16, 1, 2>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces <= 32) return quantize_launch<T, 32, 1, 2>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces <= 64) return quantize_launch<T, 64, 1, 2>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces <= 128) return quantize_launch<T, 64, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces <= 256) return quantize_launch<T, 128, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     // few rows: a row's time is what counts, so 1 024 lanes share it (4 rows of 8192 bfloat16: see the figures above)
     if (pieces > 256 && rows <= 256 && pieces <= 1024) return quantize_launch<T, 1024, 1, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces > 256 && rows <= 256 && pieces <= 2048) return quantize_launch<T, 1024, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 512) return quantize_launch<T, kBlock, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
-    if (pieces <= 1024) return quantize_launch<T, kBlock, 4, 1>(x, ldx, rows, k, q, ldq, scale, st);
+    if (pieces <= 1024) return quantize_launch<T, 2 * kBlock, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= kHeldPieces) return quantize_launch<T, kBlock, 8, 1>(x, ldx, rows, k, q, ldq, scale, st);
     hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3((unsigned)rows), dim3(kBlock), 0, st, x, ldx, k, q, ldq, scale);
     return launch_status();
