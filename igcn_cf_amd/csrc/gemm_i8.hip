@@ -82,6 +82,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     constexpr int kWaves = WM * WN, RT = TM / WM / 32, CT = TN / WN / 32, NA = TM / 8 / kWaves, NB = TN / 8 / kWaves;
     constexpr int kStage = (TM + TN) * kDepth;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    unsigned char *const ring = smem + (TM + 2 * TN) * 4;       // the stages; behind them, the strips of the way out
     const GemmArgs &G = T.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t t = (int64_t)(blockIdx.x & 7) * T.per_xcd + (blockIdx.x >> 3);
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     for (int i = 0; i < NB; ++i) ob[i] = (unsigned)min(8 * (wave * NB + i) + (lane >> 3), last_b) * (unsigned)G.ldb + piece(wave * NB + i);
     const int64_t stages = (G.k + kDepth - 1) / kDepth;
     i32x4 held[DIRECT ? 1 : NA + NB];
-    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void *)smem;
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_void *)ring;
 
     auto fetch = [&](int64_t s) {                                // stage s of both sides: on its way to LDS, or to registers
         const int64_t k0 = s * kDepth;
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         }
     };
     auto land = [&](int64_t s) {                                 // registers to LDS
-        i32x4 *at = reinterpret_cast<i32x4 *>(smem + (s % STAGES) * kStage);
+        i32x4 *at = reinterpret_cast<i32x4 *>(ring + (s % STAGES) * kStage);
 #pragma unroll
         for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = held[i];
 #pragma unroll
@@ -137,6 +138,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     i32x16 acc[RT][CT] = {};
     const int wm = wave / WN, wn = wave % WN;
     const int ra = wm * (TM / WM) + (lane & 31), rb = wn * (TN / WN) + (lane & 31), half = lane >> 5, turn = (lane >> 1) & 7;
+    float *const fa = reinterpret_cast<float *>(smem), *const fb = fa + TM, *const fc = fb + TN;       // the tile's scales and bias, for the way out
+    for (int i = threadIdx.x; i < TM; i += 64 * kWaves) fa[i] = i <= last_a ? G.sa[m0 + i] : 0.f;
+    for (int i = threadIdx.x; i < TN; i += 64 * kWaves) {
+        fb[i] = i <= last_b ? G.sb[n0 + i] : 0.f;
+        fc[i] = G.bias && i <= last_b ? G.bias[n0 + i] : 0.f;
+    }
     if constexpr (DIRECT) {
         for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s);
     } else if (stages) { fetch(0); land(0); }
@@ -146,7 +153,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         }
         __syncthreads();                                         // ... for everyone, and everyone is through with the stage before it
         if (s + STAGES - 1 < stages) fetch(s + STAGES - 1);
-        const unsigned char *sa = smem + (s % STAGES) * kStage + ra * kDepth, *sb = smem + (s % STAGES) * kStage + TM * kDepth + rb * kDepth;
+        const unsigned char *sa = ring + (s % STAGES) * kStage + ra * kDepth, *sb = ring + (s % STAGES) * kStage + TM * kDepth + rb * kDepth;
 #pragma unroll
         for (int j = 0; j < kDepth / 32; ++j) {
             const int at = ((2 * j + half) ^ turn) * 16;
@@ -167,17 +174,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     // The way out.  b is the matrix instruction's first operand: lane l holds row l % 32 of a and columns 8 (i / 4) + 4 (l / 32) + i % 4, four
     // neighbours of a row of y at a time.  They cross a strip of LDS of the wave's own (32 rows, its columns) so that a store takes whole
     // lines: 16 bytes a lane, neighbouring lanes along the row.
-    float *const fa = reinterpret_cast<float *>(smem), *const fb = fa + TM, *const fc = fb + TN;       // (the last stage is through with LDS)
-    for (int i = threadIdx.x; i < TM; i += 64 * kWaves) fa[i] = i <= last_a ? G.sa[m0 + i] : 0.f;
-    for (int i = threadIdx.x; i < TN; i += 64 * kWaves) {
-        fb[i] = i <= last_b ? G.sb[n0 + i] : 0.f;
-        fc[i] = G.bias && i <= last_b ? G.bias[n0 + i] : 0.f;
-    }
-    __syncthreads();
     auto put = [&](auto *y) {
         using Y = std::remove_pointer_t<decltype(y)>;
         constexpr int kCols = CT * 32, kRow = kCols * sizeof(Y) + 16, kLanes = kCols * sizeof(Y) / 16, kRows = 64 / kLanes, kE = 16 / sizeof(Y);       // (16 bytes more a row: other banks)
-        unsigned char *const strip = smem + (TM + 2 * TN) * 4 + wave * 32 * (kCols * 4 + 16);
+        unsigned char *const strip = ring + wave * 32 * (kCols * 4 + 16);
         const bool biased = G.bias != nullptr;
         const int n1 = wn * (TN / WN) + lane % kLanes * kE;      // of the tile: this lane's columns on the way out
 #pragma unroll
@@ -228,7 +228,7 @@ template <int TM, int TN, int WM, int WN, int STAGES> static int tiles_launch(co
     auto launch = [&](auto *kernel, int most) {
         int64_t stages = (G.k + kDepth - 1) / kDepth;
         stages = stages < most ? stages : most;
-        const size_t in = (size_t)stages * (TM + TN) * kDepth, out = (TM + 2 * TN) * 4 + WM * WN * 32 * (TN / WN * 4 + 16), lds = in > out ? in : out;
+        const size_t in = (size_t)stages * (TM + TN) * kDepth, out = WM * WN * 32 * (TN / WN * 4 + 16), lds = (TM + 2 * TN) * 4 + (in > out ? in : out);
         if (lds > 65536) {                                       // (once would do; it is a host call of well under a microsecond)
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (e != hipSuccess) return (int)e;
