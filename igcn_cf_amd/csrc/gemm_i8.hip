@@ -51,6 +51,9 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int64_t 
 // instruction, lane after lane); else through registers.  A row's eight 16-byte pieces stand in LDS at piece ^ (row / 2 % 8): 16 lanes that read the
 // same piece of 16 neighbouring rows hit 64 different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
 // Depth past the end reads a block of zeros, rows past the end the last row (not stored).
+// BY_DEPTH (a 64 x 64 tile of four waves): a wave takes a quarter of the stage's depth for the whole tile instead of all of it for its own piece,
+// and they exchange sums in the end: LDS is read half as often and no product waits for the one before it (64 x 1000 x 8192: 23.6 -> 18.1 us;
+// 64 x 96421 x 64: 8.2 -> 11.4, so only where the depth pays for the exchange).
 // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, 4 tiles of a deep at a time, so that the tiles under way there
 // share their rows in its L2.
 constexpr int kDepth = 128;
@@ -76,11 +79,15 @@ template <int LEFT> __device__ __forceinline__ void wait_for_lds() { asm volatil
 constexpr int64_t kMostApart = 1 << 23;                          // bytes between rows: 256 of them fit 31 bits
 struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; };
 
-template <int TM, int TN, int WM, int WN, int STAGES, bool DIRECT>
+constexpr size_t kExchanged = 3 * 4 * 4096;                      // of LDS: three waves' sums of four pieces
+
+template <int TM, int TN, int WM, int WN, int STAGES, bool DIRECT, bool BY_DEPTH>
 __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArgs T)
 {
     constexpr int kWaves = WM * WN, RT = TM / WM / 32, CT = TN / WN / 32, NA = TM / 8 / kWaves, NB = TN / 8 / kWaves;
     constexpr int kStage = (TM + TN) * kDepth;
+    static_assert(!BY_DEPTH || (RT == 1 && CT == 1 && kWaves == kDepth / 32), "a quarter of the depth for each of four waves");
+    constexpr int AR = BY_DEPTH ? WM : RT, AC = BY_DEPTH ? WN : CT;       // pieces whose sums a wave holds
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     unsigned char *const ring = smem + (TM + 2 * TN) * 4;       // the stages; behind them, the strips of the way out
     const GemmArgs &G = T.g;
@@ -135,9 +142,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
     };
 
-    i32x16 acc[RT][CT] = {};
+    i32x16 acc[AR][AC] = {};
     const int wm = wave / WN, wn = wave % WN;
-    const int ra = wm * (TM / WM) + (lane & 31), rb = wn * (TN / WN) + (lane & 31), half = lane >> 5, turn = (lane >> 1) & 7;
+    const int ra = (BY_DEPTH ? 0 : wm * (TM / WM)) + (lane & 31), rb = (BY_DEPTH ? 0 : wn * (TN / WN)) + (lane & 31), half = lane >> 5, turn = (lane >> 1) & 7;
     float *const fa = reinterpret_cast<float *>(smem), *const fb = fa + TM, *const fc = fb + TN;       // the tile's scales and bias, for the way out
     for (int i = threadIdx.x; i < TM; i += 64 * kWaves) fa[i] = i <= last_a ? G.sa[m0 + i] : 0.f;
     for (int i = threadIdx.x; i < TN; i += 64 * kWaves) {
@@ -152,24 +159,53 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
             if (s + STAGES - 2 < stages) wait_for_lds<(STAGES - 2) * (NA + NB)>(); else wait_for_lds<0>();
         }
         __syncthreads();                                         // ... for everyone, and everyone is through with the stage before it
-        if (s + STAGES - 1 < stages) fetch(s + STAGES - 1);
         const unsigned char *sa = ring + (s % STAGES) * kStage + ra * kDepth, *sb = ring + (s % STAGES) * kStage + TM * kDepth + rb * kDepth;
-#pragma unroll
-        for (int j = 0; j < kDepth / 32; ++j) {
+        i32x4 av[AR], bv[AC];
+        auto read = [&](int j) {
             const int at = ((2 * j + half) ^ turn) * 16;
-            i32x4 av[RT], bv[CT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) av[r] = *reinterpret_cast<const i32x4 *>(sa + r * 32 * kDepth + at);
+            for (int r = 0; r < AR; ++r) av[r] = *reinterpret_cast<const i32x4 *>(sa + r * 32 * kDepth + at);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) bv[c] = *reinterpret_cast<const i32x4 *>(sb + c * 32 * kDepth + at);
+            for (int c = 0; c < AC; ++c) bv[c] = *reinterpret_cast<const i32x4 *>(sb + c * 32 * kDepth + at);
+        };
+        read(BY_DEPTH ? wave : 0);                               // (before the next stage is sent for: its addresses take a while)
+        if (s + STAGES - 1 < stages) fetch(s + STAGES - 1);
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+        for (int j = 0; j < (BY_DEPTH ? 1 : kDepth / 32); ++j) {
+            if (j) read(j);
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[c], av[r], acc[r][c], 0, 0, 0);
+            for (int r = 0; r < AR; ++r)
+#pragma unroll
+                for (int c = 0; c < AC; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[c], av[r], acc[r][c], 0, 0, 0);
         }
         if constexpr (!DIRECT) if (s + 1 < stages) land(s + 1);
     }
     __syncthreads();
+    if constexpr (BY_DEPTH) {                                    // piece q of the tile goes to wave q: [piece][the three other waves][4 sums a lane and quarter]
+        i32x4 *const sums = reinterpret_cast<i32x4 *>(ring);
+#pragma unroll
+        for (int q = 0; q < kWaves; ++q)
+            if (q != wave) {
+                i32x4 *to = sums + ((q * 3 + (wave - (wave > q))) * 4) * 64 + lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[64 * i] = i32x4{acc[q / WN][q % WN][4 * i], acc[q / WN][q % WN][4 * i + 1], acc[q / WN][q % WN][4 * i + 2], acc[q / WN][q % WN][4 * i + 3]};
+            }
+        __syncthreads();
+        i32x16 all = acc[0][0];
+#pragma unroll
+        for (int q = 1; q < kWaves; ++q)
+            if (q == wave) all = acc[q / WN][q % WN];
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const i32x4 x = sums[((wave * 3 + k) * 4 + i) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) all[4 * i + e] += x[e];
+            }
+        acc[0][0] = all;
+        __syncthreads();                                         // (the strips stand where the sums stood)
+    }
 
     // The way out.  b is the matrix instruction's first operand: lane l holds row l % 32 of a and columns 8 (i / 4) + 4 (l / 32) + i % 4, four
     // neighbours of a row of y at a time.  They cross a strip of LDS of the wave's own (32 rows, its columns) so that a store takes whole
@@ -216,7 +252,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     else put(static_cast<__half *>(G.y));
 }
 
-template <int TM, int TN, int WM, int WN, int STAGES> static int tiles_launch(const GemmArgs &G, hipStream_t st)
+template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> static int tiles_launch(const GemmArgs &G, hipStream_t st)
 {
     TileArgs T;
     T.g = G;
@@ -228,7 +264,11 @@ template <int TM, int TN, int WM, int WN, int STAGES> static int tiles_launch(co
     auto launch = [&](auto *kernel, int most) {
         int64_t stages = (G.k + kDepth - 1) / kDepth;
         stages = stages < most ? stages : most;
-        const size_t in = (size_t)stages * (TM + TN) * kDepth, out = WM * WN * 32 * (TN / WN * 4 + 16), lds = (TM + 2 * TN) * 4 + (in > out ? in : out);
+        size_t ring = (size_t)stages * (TM + TN) * kDepth;
+        const size_t strips = WM * WN * 32 * (TN / WN * 4 + 16);
+        if (ring < strips) ring = strips;
+        if (direct && BY_DEPTH && ring < kExchanged) ring = kExchanged;
+        const size_t lds = (TM + 2 * TN) * 4 + ring;
         if (lds > 65536) {                                       // (once would do; it is a host call of well under a microsecond)
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (e != hipSuccess) return (int)e;
@@ -236,10 +276,10 @@ template <int TM, int TN, int WM, int WN, int STAGES> static int tiles_launch(co
         hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
         return launch_status();
     };
-    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false>, 2);
+    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true, BY_DEPTH>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false, false>, 2);
 }
 
-// ---- up to 16 rows of a ---------------------------------------------------------------------------------------------------------------
+// ---- up to 8 rows of a ----------------------------------------------------------------------------------------------------------------
 // Bound by the bytes of b, each used once: no tile of b is worth staging.  A wave takes 16 rows of b as the matrix instruction's first
 // operand straight from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and the rows of a, the second
 // operand, from LDS, where a workgroup lays them out once in the order the lanes read them: [64 codes of depth][16 of them][row][16 bytes].
@@ -250,7 +290,7 @@ template <int TM, int TN, int WM, int WN, int STAGES> static int tiles_launch(co
 // x in floating point (X is not int8_t): every workgroup makes it 8-bit on the way, with the quantiser's own steps — no launch, no
 // buffer; worth it while that is less work than a launch (kFusedValues).
 constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 8;                                      // (12 rows against 16384 x 8192: 40 us, 34 in tiles; 8 rows: 32 and 34)
 constexpr int kPanelBytes = 32768;                               // of LDS for the rows of a: four workgroups on a CU
 constexpr int64_t kFusedValues = 8192;
 
@@ -427,7 +467,7 @@ static int product(const GemmArgs &G, hipStream_t st)
 {
     if (G.m <= kFewRows || G.lda > kMostApart || G.ldb > kMostApart) {
         const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
-        for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 16 at a time)
+        for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 8 at a time)
             FewArgs F = {};
             F.g = G;
             F.g.a += at * G.lda;
@@ -440,11 +480,16 @@ static int product(const GemmArgs &G, hipStream_t st)
         return IGCN_OK;
     }
     auto tiles = [&](int64_t tm, int64_t tn) { return ((G.m + tm - 1) / tm) * ((G.n + tn - 1) / tn); };
-    if (G.m <= 64) return tiles_launch<64, 64, 2, 2, 4>(G, st);
-    if (G.k <= kDepth && G.out == IGCN_DTYPE_F32) return tiles_launch<64, 128, 2, 4, 2>(G, st);
-    if (G.k > kDepth && tiles(256, 256) >= 200) return tiles_launch<256, 256, 2, 4, 2>(G, st);
-    if (tiles(128, 128) >= 200) return tiles_launch<128, 128, 2, 2, 2>(G, st);
-    return tiles_launch<64, 64, 2, 2, 4>(G, st);
+    // The largest tile that still makes nearly a workgroup for each of 256 CUs: 256 x 256 reads each code half as often as 128 x 128 (8192 x 8192 x
+    // 4096: 258 against 298 us), which with 64 tiles would leave three of four CUs idle (512 x 8192 x 8192: 90 against 47 us; 64 x 64: 57).
+    // One stage of depth: writing y is all there is, and many small waves hide it best (512 x 96421 x 64 to float32: 48 us; 128 x 128 57,
+    // 256 x 256 55; to bfloat16 128 x 128 30, 64 x 128 38).
+    if (G.m > 64) {
+        if (G.k <= kDepth && G.out == IGCN_DTYPE_F32) return tiles_launch<64, 128, 2, 4, 2>(G, st);
+        if (G.k > kDepth && tiles(256, 256) >= 200) return tiles_launch<256, 256, 2, 4, 2>(G, st);
+        if (tiles(128, 128) >= 200) return tiles_launch<128, 128, 2, 2, 2>(G, st);
+    }
+    return G.k >= 512 ? tiles_launch<64, 64, 2, 2, 4, true>(G, st) : tiles_launch<64, 64, 2, 2, 4>(G, st);
 }
 
 static int check_product(const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias, int64_t m, int64_t n, int64_t k, const void *y,
