@@ -15,7 +15,10 @@
 // float32 with every operation rounded once, in the order written (no fused multiply-add): elementary float32 operations in any other
 // program give the same codes, bit for bit.
 #include "dtypes.h"
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 namespace igcn {
 
@@ -23,6 +26,7 @@ constexpr int kTensors = 56;             // of one launch: 64 bytes each in at m
 constexpr int kPer = 8;                  // elements of a thread: 16 lanes (a DPP row) hold a block of 128
 constexpr int kChunk = kBlock * kPer;    // elements of a workgroup
 constexpr int kNormBlocks = 2048;        // partial sums of a norm launch
+constexpr int64_t kMostChunks = (1 << 24) - 1;      // of a launch: 2^32 threads at most
 static_assert(IGCN_ADAMW_BLOCK == 16 * kPer, "a block of the 8-bit moments is a DPP row's elements");
 
 struct TensorTable {
@@ -340,7 +344,7 @@ template <typename F> static int for_tables(const igcn_adamw_tensor *tensors, in
         const int64_t from = at;
         for (; at < n && T.n < kTensors; ++at) {
             const int64_t c = chunks_of(tensors[at].n);
-            if (chunks + c > 0x7fffffff) { if (T.n) break; return IGCN_E_SHAPE; }
+            if (chunks + c > kMostChunks) break;                // (one tensor alone is at most that: check_tensors)
             T.t[T.n] = tensors[at];
             T.first[T.n++] = (int)chunks;
             chunks += c;
@@ -365,6 +369,35 @@ static int grad_squares(const igcn_adamw_tensor *tensors, int64_t n, double *par
     });
 }
 
+// Whether memory that the step writes is shared between two of its tensors, or with a gradient (gradients may share theirs).
+static int check_overlap(const igcn_adamw_tensor *tensors, int64_t n, bool eight)
+{
+    struct Stretch { uintptr_t begin, end; bool written; };
+    const std::unique_ptr<Stretch[]> all(new (std::nothrow) Stretch[6 * n]);
+    if (!all) return (int)hipErrorOutOfMemory;
+    int64_t count = 0;
+    auto add = [&](const void *p, int64_t bytes, bool written) {
+        if (bytes) all[count++] = Stretch{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, written};
+    };
+    for (int64_t i = 0; i < n; ++i) {
+        const igcn_adamw_tensor &t = tensors[i];
+        add(t.param, t.n * (t.dtype == IGCN_DTYPE_F32 ? 4 : 2), true);
+        add(t.exp_avg, t.n * (eight ? 1 : 4), true);
+        add(t.exp_avg_sq, t.n * (eight ? 1 : 4), true);
+        if (eight) add(t.scales, (t.n + IGCN_ADAMW_BLOCK - 1) / IGCN_ADAMW_BLOCK * 8, true);
+        add(t.step, 4, true);
+        add(t.grad, t.n * (t.grad_dtype == IGCN_DTYPE_F32 ? 4 : 2), false);
+    }
+    std::sort(all.get(), all.get() + count, [](const Stretch &a, const Stretch &b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;                              // the furthest end so far
+    for (int64_t i = 0; i < count; ++i) {
+        if (all[i].begin < (all[i].written ? any : written)) return IGCN_E_OVERLAP;
+        any = std::max(any, all[i].end);
+        if (all[i].written) written = std::max(written, all[i].end);
+    }
+    return IGCN_OK;
+}
+
 // moment_bits 0: only the gradients are looked at
 static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment_bits)
 {
@@ -373,7 +406,7 @@ static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment
     const bool eight = moment_bits == 8;
     for (int64_t i = 0; i < n; ++i) {
         const igcn_adamw_tensor &t = tensors[i];
-        if (t.n < 0) return IGCN_E_SHAPE;
+        if (t.n < 0 || t.n > kMostChunks * kChunk) return IGCN_E_SHAPE;
         if (!dtype_ok(t.grad_dtype)) return IGCN_E_RANGE;
         if (t.n > 0 && !t.grad) return IGCN_E_NULL;
         if (misaligned(t.grad, t.grad_dtype)) return IGCN_E_ALIGN;
@@ -385,7 +418,7 @@ static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment
         if (!eight && ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & 3)) return IGCN_E_ALIGN;
         if ((reinterpret_cast<uintptr_t>(t.scales) | reinterpret_cast<uintptr_t>(t.step)) & 3) return IGCN_E_ALIGN;
     }
-    return IGCN_OK;
+    return moment_bits ? check_overlap(tensors, n, eight) : (int)IGCN_OK;
 }
 
 }  // namespace igcn

@@ -258,7 +258,8 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
     T.g = G;
     T.tiles_m = (G.m + TM - 1) / TM;
     T.tiles_n = (G.n + TN - 1) / TN;
-    if (T.tiles_m > (1 << 28) / T.tiles_n) return IGCN_E_SHAPE;
+    constexpr int64_t kMostTiles = ((int64_t)1 << 32) / (64 * WM * WN) - 8;      // a launch has fewer than 2^32 threads
+    if (T.tiles_m > kMostTiles / T.tiles_n) return IGCN_E_SHAPE;
     T.per_xcd = (T.tiles_m * T.tiles_n + 7) / 8;
     const bool direct = ((reinterpret_cast<uintptr_t>(G.a) | reinterpret_cast<uintptr_t>(G.b) | (uintptr_t)G.lda | (uintptr_t)G.ldb | (uintptr_t)G.k) & 15) == 0;
     auto launch = [&](auto *kernel, int most) {
@@ -288,11 +289,12 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
 // order), which fills the card four times as well where b has few rows; with a short one every wave has TILES of its own.  KEEP loads of
 // a wave are under way at a time, the first ones before the rows of a are laid out: their time hides behind the bytes of b.
 // x in floating point (X is not int8_t): every workgroup makes it 8-bit on the way, with the quantiser's own steps — no launch, no
-// buffer; worth it while that is less work than a launch (kFusedValues).
+// buffer; worth it while that is less work than a launch (against 16384 rows of b: 1 x 2048 10.9 us this way and 12.4 in two launches,
+// 1 x 4096 19.5 and 16.1; 4 x 512 against 96421 rows 16.7 and 19.4, 4 x 2048 against 16384 13.1 and 12.3).
 constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
 constexpr int kFewRows = 8;                                      // (12 rows against 16384 x 8192: 40 us, 34 in tiles; 8 rows: 32 and 34)
 constexpr int kPanelBytes = 32768;                               // of LDS for the rows of a: four workgroups on a CU
-constexpr int64_t kFusedValues = 8192;
+constexpr int64_t kFusedValues = 2048;
 
 struct FewArgs {
     GemmArgs g;
@@ -456,7 +458,7 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     // a workgroup that lays the rows of a out once and walks several tiles with them: as many as keep 2 048 workgroups busy
     F.jobs = F.panel >= steps ? (groups + 2047) / 2048 : 1;
     const int64_t blocks = (groups + F.jobs - 1) / F.jobs;
-    if (blocks > 0x7fffffff) return IGCN_E_SHAPE;
+    if (blocks >= ((int64_t)1 << 32) / kBlock) return IGCN_E_SHAPE;              // (2^32 threads of a launch)
     const size_t lds = ((size_t)F.panel * kStep << F.shift) + (share ? 4 * 16 * 17 * 4 : 0);
     if (share) hipLaunchKernelGGL((few_rows_i8_kernel<1, 4, true, X>), dim3((unsigned)blocks), dim3(kBlock), lds, st, F);
     else hipLaunchKernelGGL((few_rows_i8_kernel<kOwn, 1, false, X>), dim3((unsigned)blocks), dim3(kBlock), lds, st, F);
@@ -504,7 +506,7 @@ static int check_product(const float *sa, const int8_t *b, int64_t ldb, const fl
     return IGCN_OK;
 }
 
-static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && m * k <= kFusedValues && m * ((k + kStep - 1) / kStep) * kStep <= kPanelBytes / 2; }
+static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && m * k <= kFusedValues; }      // (as steps of up to 8 rows well under kPanelBytes)
 static int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 
 }  // namespace igcn

@@ -4,8 +4,9 @@
 //
 // Bound by the bytes: x read once, q written once.  A row's values stay in registers between its maximum and its codes: L lanes hold a
 // row in I pieces of 16 bytes each (adjacent lanes, adjacent pieces: every load and store of a wave covers whole lines), L the smallest
-// power of two that makes I one, up to a wave; from 1 024 pieces on a workgroup holds the row.  Short rows: each lane group takes R rows
-// at once, R loads in flight before the first maximum.  Rows over kHeld bytes do not fit: they are read a second time (from L2).
+// power of two that makes I one, up to a wave; from 129 pieces on more waves share the row, at most two pieces a lane until it is long
+// (2048 rows of 8192 bfloat16: two pieces on 512 lanes 13.7 us, four on 256 16.7).  Short rows: each lane group takes R rows at once, R loads
+// in flight before the first maximum.  Rows over kHeldPieces do not fit: they are read a second time (from L2).
 #include "quant_i8.h"
 
 namespace igcn {
@@ -127,9 +128,8 @@ static int quantize_launch(const T *x, int64_t ldx, int64_t rows, int64_t k, int
     return launch_status();
 }
 
-template <typename T> static int quantize(const void *xv, int64_t ldx, int64_t rows, int64_t k, int8_t *q, int64_t ldq, float *scale, hipStream_t st)
+template <typename T> static int quantize(const T *x, int64_t ldx, int64_t rows, int64_t k, int8_t *q, int64_t ldq, float *scale, hipStream_t st)
 {
-    const T *x = static_cast<const T *>(xv);
     const int64_t pieces = (k + Chunk<T>::kValues - 1) / Chunk<T>::kValues;
     if (pieces <= 4) return quantize_launch<T, 4, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 8) return quantize_launch<T, 8, 1, 4>(x, ldx, rows, k, q, ldq, scale, st);
@@ -138,7 +138,7 @@ template <typename T> static int quantize(const void *xv, int64_t ldx, int64_t r
     if (pieces <= 64) return quantize_launch<T, 64, 1, 2>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 128) return quantize_launch<T, 64, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 256) return quantize_launch<T, 128, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
-    // few rows: a row's time is what counts, so 1 024 lanes share it (4 rows of 8192 bfloat16: see the figures above)
+    // no more rows than CUs: a row's own time is what counts, so 1 024 lanes share it (4 rows of 8192 bfloat16: 5.0 us; 512 lanes 7.4)
     if (pieces > 256 && rows <= 256 && pieces <= 1024) return quantize_launch<T, 1024, 1, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces > 256 && rows <= 256 && pieces <= 2048) return quantize_launch<T, 1024, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
     if (pieces <= 512) return quantize_launch<T, kBlock, 2, 1>(x, ldx, rows, k, q, ldq, scale, st);
@@ -152,14 +152,12 @@ template <typename T, int L, int R>
 static int dequantize_launch(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int64_t k, int64_t pieces, T *y, int64_t ldy, hipStream_t st)
 {
     const int64_t per = (int64_t)(kBlock / L) * R, gy = (pieces + L - 1) / L;
-    if (gy > 65535) return IGCN_E_SHAPE;
     hipLaunchKernelGGL((dequantize_rows_kernel<T, L, R>), dim3((unsigned)((rows + per - 1) / per), (unsigned)gy), dim3(kBlock), 0, st, q, ldq, scale, rows, k, y, ldy);
     return launch_status();
 }
 
-template <typename T> static int dequantize(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int64_t k, void *yv, int64_t ldy, hipStream_t st)
+template <typename T> static int dequantize(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int64_t k, T *y, int64_t ldy, hipStream_t st)
 {
-    T *y = static_cast<T *>(yv);
     const int64_t pieces = (k + Chunk<T>::kValues - 1) / Chunk<T>::kValues;
     if (pieces <= 4) return dequantize_launch<T, 4, 4>(q, ldq, scale, rows, k, pieces, y, ldy, st);
     if (pieces <= 8) return dequantize_launch<T, 8, 4>(q, ldq, scale, rows, k, pieces, y, ldy, st);
@@ -173,6 +171,8 @@ template <typename T> static int dequantize(const int8_t *q, int64_t ldq, const 
 using namespace igcn;
 
 constexpr int64_t kMostRows = 0x7fffffff;
+// A launch has fewer than 2^32 threads and 65536 x 64 pieces of a row: larger arrays go in slabs, a gigabyte each and more
+constexpr int64_t kSlabRows = 1 << 22, kSlabColumns = 1 << 23;
 
 extern "C" int igcn_quantize_rows_i8(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int64_t k, int8_t *q, int64_t ldq, float *scale, void *stream)
 {
@@ -182,9 +182,14 @@ extern "C" int igcn_quantize_rows_i8(const void *x, int32_t dtype, int64_t ldx, 
     if (!scale || (k > 0 && (!x || !q))) return IGCN_E_NULL;
     if (misaligned(x, dtype) || (reinterpret_cast<uintptr_t>(scale) & 3)) return IGCN_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == IGCN_DTYPE_F32) return quantize<float>(x, ldx, rows, k, q, ldq, scale, st);
-    if (dtype == IGCN_DTYPE_BF16) return quantize<__hip_bfloat16>(x, ldx, rows, k, q, ldq, scale, st);
-    return quantize<__half>(x, ldx, rows, k, q, ldq, scale, st);
+    int rc = IGCN_OK;
+    for (int64_t r = 0; r < rows && rc == IGCN_OK; r += kSlabRows) {
+        const int64_t n = rows - r < kSlabRows ? rows - r : kSlabRows;
+        if (dtype == IGCN_DTYPE_F32) rc = quantize(static_cast<const float *>(x) + r * ldx, ldx, n, k, q + r * ldq, ldq, scale + r, st);
+        else if (dtype == IGCN_DTYPE_BF16) rc = quantize(static_cast<const __hip_bfloat16 *>(x) + r * ldx, ldx, n, k, q + r * ldq, ldq, scale + r, st);
+        else rc = quantize(static_cast<const __half *>(x) + r * ldx, ldx, n, k, q + r * ldq, ldq, scale + r, st);
+    }
+    return rc;
 }
 
 extern "C" int igcn_dequantize_rows_i8(const int8_t *q, int64_t ldq, const float *scale, int64_t rows, int64_t k, void *y, int32_t dtype, int64_t ldy, void *stream)
@@ -195,7 +200,14 @@ extern "C" int igcn_dequantize_rows_i8(const int8_t *q, int64_t ldq, const float
     if (!q || !scale || !y) return IGCN_E_NULL;
     if (misaligned(y, dtype) || (reinterpret_cast<uintptr_t>(scale) & 3)) return IGCN_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == IGCN_DTYPE_F32) return dequantize<float>(q, ldq, scale, rows, k, y, ldy, st);
-    if (dtype == IGCN_DTYPE_BF16) return dequantize<__hip_bfloat16>(q, ldq, scale, rows, k, y, ldy, st);
-    return dequantize<__half>(q, ldq, scale, rows, k, y, ldy, st);
+    int rc = IGCN_OK;
+    for (int64_t r = 0; r < rows; r += kSlabRows)
+        for (int64_t c = 0; c < k && rc == IGCN_OK; c += kSlabColumns) {
+            const int64_t n = rows - r < kSlabRows ? rows - r : kSlabRows, w = k - c < kSlabColumns ? k - c : kSlabColumns, at = r * ldy + c;
+            const int8_t *from = q + r * ldq + c;
+            if (dtype == IGCN_DTYPE_F32) rc = dequantize(from, ldq, scale + r, n, w, static_cast<float *>(y) + at, ldy, st);
+            else if (dtype == IGCN_DTYPE_BF16) rc = dequantize(from, ldq, scale + r, n, w, static_cast<__hip_bfloat16 *>(y) + at, ldy, st);
+            else rc = dequantize(from, ldq, scale + r, n, w, static_cast<__half *>(y) + at, ldy, st);
+        }
+    return rc;
 }

@@ -107,7 +107,8 @@ class BasicModel(nn.Module):
 
     def predict_i8(self, users, items=None, dtype=torch.float32):
         """predict(users) from 8-bit integers: user rows made 8-bit on the way, item rows from `items` = quantized_items() (None:
-        made here); every row has a scale of its own, so a score is off by at most 0.4 % of max|u| |i|_1 + |u|_1 max|i|."""
+        made here); every row has a scale of its own, so a score is off by at most about 0.4 % (1 / 254) of
+        max|u| |i|_1 + |u|_1 max|i|."""
         with torch.no_grad():
             codes, scale = items if items is not None else self.quantized_items()
             return ops.linear_i8(self.score_tables()[0][users], codes, scale, dtype=dtype)

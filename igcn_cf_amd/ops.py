@@ -855,7 +855,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     its code times its block's scale), rounded stochastically from (seed, place in the list, step, element); zeros to start with.
     lr: a number, or a one-element float32 tensor on the GPU (read by the kernel: HIP-graph replays see its current value).
     max_grad_norm: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) on the way; norm = L2 norm over all of them, computed
-    here or given as `grad_norm` (a one-element float32 tensor, for several calls clipped by one norm).  Returns the norm, or None."""
+    here or given as `grad_norm` (a one-element float32 tensor, for several calls clipped by one norm).  Returns the norm, or None.
+    Memory that is rewritten (parameters, moments, scales, steps) stands in one place of the lists only."""
     params, grads, exp_avgs, exp_avg_sqs, steps = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps)
     n, eight = len(params), scales is not None
     scales = list(scales) if eight else [None] * n
@@ -885,9 +886,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     if eight and not all(s.dtype is torch.float32 and s.is_contiguous() and s.shape == ((k + ADAMW_BLOCK - 1) // ADAMW_BLOCK, 2) for s, k in zip(scales, sizes)):
         raise _lib.IgcnError('scales must be contiguous float32 [ceil(numel / %d), 2]' % ADAMW_BLOCK)
     at = [[t.data_ptr() for t in ts] for ts in (params, exp_avgs, exp_avg_sqs, steps)]
-    written = [a for column in at for a in column if a]                                  # (an empty tensor has no address)
-    if len(set(written)) != len(written):
-        raise _lib.IgcnError('a tensor stands in the lists twice: every parameter, moment and step is rewritten by one place only')
     at[1:1] = [[g.data_ptr() for g in grads]]
     at[4:4] = [[s.data_ptr() for s in scales] if eight else [0] * n]
     rows = array.array('q', itertools.chain.from_iterable(zip(*at, sizes, [_DTYPE_CODES[p] | _DTYPE_CODES[g] << 32 for p, g in zip(pt, gt)])))
@@ -909,12 +907,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
         ws = torch.empty(L.igcn_adamw_workspace_bytes(table, n), dtype=torch.uint8, device=device)
         norm, max_norm, norm_out = norm_in, 0., None
         if max_grad_norm is not None:
-            max_norm = max_grad_norm
+            max_norm = float(max_grad_norm)
             if norm_in is None:
                 norm = torch.empty((), dtype=torch.float32, device=device)
                 norm_out = norm.data_ptr()
-        code = L.igcn_adamw_step(table, n, 8 if eight else 32, lr, _lib.ptr(lr_dev), betas[0], betas[1], eps, weight_decay, max_norm, _lib.ptr(norm_in),
-                                 norm_out, seed & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), _lib.current_stream())
+        code = L.igcn_adamw_step(table, n, 8 if eight else 32, float(lr), _lib.ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
+                                 float(weight_decay), max_norm, _lib.ptr(norm_in),
+                                 norm_out, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), _lib.current_stream())
         if code:
             _lib.check(code, 'igcn_adamw_step')
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
@@ -945,7 +944,7 @@ def _require_vector(t, name, n, like):
 def quantize_rows_i8(x):
     """(codes int8 [M, K], scale float32 [M]) of the rows of x (float32, bfloat16 or float16 [M, K], rows contiguous): scale =
     max|row| / 127, codes = row / scale to the nearest whole number, ties to even (igcn_quantize_rows_i8).  A row of zeros has scale 0;
-    one with a NaN or an infinity has scale NaN, so that what is computed from it shows it."""
+    one with a NaN or an infinity has scale NaN, so that what is computed from it shows it.  No gradient: rounding has none."""
     _require_rows(x, 'x', tuple(_DTYPE_CODES))
     m, k = x.shape
     with _on(x.device):
@@ -1000,7 +999,7 @@ def matmul_i8(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
 
 def linear_i8(x, b, b_scale, bias=None, dtype=None):
     """[M, N] of `dtype` (None: that of x): the rows of x made 8-bit, as quantize_rows_i8 makes them, and multiplied with those of b, as
-    matmul_i8 does (igcn_linear_i8: one call, a few short rows in one launch)."""
+    matmul_i8 does (igcn_linear_i8: one call, a few short rows in one launch).  For answering: no gradient."""
     _require_rows(x, 'x', tuple(_DTYPE_CODES))
     _require_rows(b, 'b', (torch.int8,))
     (m, k), n = x.shape, b.shape[0]

@@ -63,6 +63,9 @@ class AdamW(torch.optim.Optimizer):
             self.grad_norm = got
         return loss
 
+    def __getstate__(self):                # (copies and pickles keep what torch's form of it does not know)
+        return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm, 'seed': self.seed, 'grad_norm': self.grad_norm}
+
     def load_state_dict(self, state_dict):
         """As torch's, but the state keeps its own types (torch's casts every floating state to its parameter's).  Takes the state of
         torch.optim.AdamW too; a group's state_bits then follow from what the state holds."""

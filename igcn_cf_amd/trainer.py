@@ -213,7 +213,7 @@ class BasicTrainer:
         return (self._token(getattr(m, 'norm_adj', None)), self._token(getattr(m, 'feat_mat', None)), self._token(self.opt),
                 self.batch_size, getattr(m, 'dropout', None), bool(m.training), getattr(self, 'l2_reg', None),
                 getattr(self, 'aux_reg', None), tuple(float(g['lr']) for g in self.opt.param_groups)) + \
-            ((self.opt.max_grad_norm,) + tuple((*g['betas'], g['eps'], g['weight_decay']) for g in self.opt.param_groups)
+            ((self.opt.max_grad_norm, self.opt.seed) + tuple((*g['betas'], g['eps'], g['weight_decay']) for g in self.opt.param_groups)
              if isinstance(self.opt, AdamW) else ())
 
     def _graph_step(self, inputs, loss_fn, kind='nodes'):

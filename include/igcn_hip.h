@@ -33,6 +33,7 @@ extern "C" {
 #define IGCN_E_NO_DEVICE  -5   /* no HIP device is available               */
 #define IGCN_E_CAPTURE    -6   /* the stream is capturing and the call cannot be captured: igcn_csr_transpose (rocPRIM's sort),
                                   or a kernel that carries scratch (none does in the library as built; csrc/common.h) */
+#define IGCN_E_OVERLAP    -7   /* memory that the call rewrites is named twice */
 
 #define IGCN_MAX_ADDS      8   /* epilogue addends of igcn_spmm_csr_f32     */
 #define IGCN_SPMM_MASKED_ROWS_ZERO  1   /* flags of igcn_spmm_csr_f32: rows with row_mask[r] == 0 are set to zero (else left untouched) */
@@ -505,7 +506,8 @@ typedef struct igcn_adamw_tensor {
  * s_m = max|m| / 448, s_v = max v / 57344, rounded stochastically with 16 bits of a hash of (seed, tensor's place in the list, step,
  * element); v > 0 is never held as 0; a block below 2^-100 is held as zeros, one with a NaN or an infinity gets a NaN scale.
  * The averages themselves are formed unrounded before the parameter is updated.
- * workspace: igcn_adamw_workspace_bytes(...) bytes, 16-byte aligned; one call's own.  No two tensors of a call may overlap. */
+ * workspace: igcn_adamw_workspace_bytes(...) bytes, 16-byte aligned; one call's own.  Memory that the call rewrites stands in one
+ * place of the list only, gradients included (IGCN_E_OVERLAP); a tensor has at most (2^24 - 1) * 2048 elements. */
 int64_t igcn_adamw_workspace_bytes(const igcn_adamw_tensor *tensors_host, int64_t n_tensors);
 int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, int32_t moment_bits, double lr, const float *lr_dev,
                     double beta1, double beta2, double eps, double weight_decay, double max_norm, const float *norm_in, float *norm_out,

@@ -223,3 +223,58 @@ def test_captured_products_follow_new_inputs_and_streams_do_not_meet():
                 got.append([ops.linear_i8(x, b, sb) for _ in range(3)])
         torch.cuda.synchronize()
         assert all(torch.equal(y, want) for ys in got for y in ys)
+
+
+@pytest.mark.parametrize('m,n', [(5, 40), (20, 9), (150, 70)])
+def test_rows_megabytes_apart(m, n):
+    """Leading dimensions over 2^23: offsets within a tile would pass 31 bits."""
+    from igcn_cf_amd import ops
+    g, k, ld = _rng(m), 100, (1 << 23) + 48
+    a, b = _codes((m, k), g), _codes((n, k), g)
+    sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+    for far_a, far_b in ((True, False), (False, True), (True, True)):
+        def spread(t, far):
+            if not far:
+                return t
+            rows = torch.empty((t.shape[0] - 1) * ld + k, dtype=torch.int8, device=DEV).as_strided(t.shape, (ld, 1))
+            return rows.copy_(t)
+        y = check(spread(a, far_a), sa, spread(b, far_b), sb)
+        assert torch.equal(y, ops.matmul_i8(a, sa, b, sb))
+
+
+def test_more_rows_and_columns_than_a_launch_takes():
+    """2^22 rows and 2^23 columns are what one launch is given."""
+    from igcn_cf_amd import ops
+    g = _rng(5)
+    x = torch.randn((1 << 22) + 70, 3, device=DEV, generator=g).to(torch.bfloat16)
+    q, s = ops.quantize_rows_i8(x)
+    want_q, want_s = _quantized(x)
+    assert torch.equal(q, want_q) and torch.equal(s, want_s)
+    assert torch.equal(ops.dequantize_rows_i8(q, s), q.float() * s[:, None])
+    q, s = _codes((2, (1 << 23) + 11), g), torch.rand(2, device=DEV, generator=g)
+    assert torch.equal(ops.dequantize_rows_i8(q, s, dtype=torch.float16), (q.float() * s[:, None]).half())
+
+
+def test_refusals():
+    from igcn_cf_amd import ops
+    Error = ops._lib.IgcnError
+    x, q, s = torch.zeros(6, 32, device=DEV), torch.zeros(6, 32, dtype=torch.int8, device=DEV), torch.ones(6, device=DEV)
+    bad = [lambda: ops.quantize_rows_i8(x.double()), lambda: ops.quantize_rows_i8(x[0]), lambda: ops.quantize_rows_i8(x.t()), lambda: ops.quantize_rows_i8(x[:1].expand(6, 32)),
+           lambda: ops.quantize_rows_i8(x[None]), lambda: ops.quantize_rows_i8(x[:, ::2]), lambda: ops.quantize_rows_i8(x.to_sparse()), lambda: ops.quantize_rows_i8([1.]),
+           lambda: ops.dequantize_rows_i8(x, s), lambda: ops.dequantize_rows_i8(q, s[:5]), lambda: ops.dequantize_rows_i8(q, s.double()), lambda: ops.dequantize_rows_i8(q, s.cpu()),
+           lambda: ops.dequantize_rows_i8(q, s, dtype=torch.float64), lambda: ops.dequantize_rows_i8(q.view(torch.uint8), s)]
+    for name, call in (('a', ops.matmul_i8), ('x', ops.linear_i8)):
+        def product(a=None, sa=s, b=q, sb=s, call=call, own=q if name == 'a' else x, **kw):
+            a = own if a is None else a
+            return call(a, sa, b, sb, **kw) if call is ops.matmul_i8 else call(a, b, sb, **kw)
+        assert product().shape == (6, 6)
+        own = q if name == 'a' else x
+        bad += [lambda f=product: f(b=q[:, :31]), lambda f=product: f(sb=s[:5]), lambda f=product: f(sb=s[None]), lambda f=product: f(b=x), lambda f=product: f(b=q.t()),
+                lambda f=product: f(bias=s[:3]), lambda f=product: f(bias=s.half()), lambda f=product: f(bias=s.cpu()), lambda f=product: f(b=q.cpu()),
+                lambda f=product: f(dtype=torch.int32), lambda f=product, o=own: f(a=o[:, :, None]), lambda f=product, o=own: f(a=o.cpu()),
+                lambda f=product, o=own: f(a=o[:, ::2]), lambda f=product, o=own: f(a=o.double())]
+    bad += [lambda: ops.matmul_i8(q, s[:5], q, s), lambda: ops.matmul_i8(x, s, q, s), lambda: ops.linear_i8(q, q, s)]
+    for i, call in enumerate(bad):
+        with pytest.raises(Error):
+            call()
+            print('not refused:', i)

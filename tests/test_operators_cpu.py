@@ -128,3 +128,48 @@ def test_dense_orders_are_told_from_views_with_gaps():
     for t in (x[:, 1], x[..., :3], x[::2], torch.zeros(1).expand(5)):
         assert not ops._dense(t)
     assert ops._same_order(x.transpose(0, 1), torch.empty_like(x.transpose(0, 1))) and not ops._same_order(x.transpose(0, 2), torch.zeros(10, 8, 6))
+
+
+def test_the_c_step_refuses_shared_memory_and_tensors_too_long():
+    L = _lib.lib()
+
+    def step(*tables, bits=32):
+        t = array.array('q')
+        for x in tables:
+            t.extend(x)
+        return L.igcn_adamw_step(t.buffer_info()[0], len(tables), bits, 1e-3, None, 0.9, 0.999, 1e-8, 0.01, 0., None, None, 0, 0x100, None)
+    far = dict(param=0x11000, m=0x13000, v=0x14000, scales=0x15000, step=0x16000)
+    for kw in (dict(m=0x1000), dict(v=0x13fc), dict(param=0x3ffc), dict(step=0x1100), dict(step=0x4000), dict(grad=0x1200), dict(grad=0x3004)):
+        assert step(_table(**kw)) == -7, kw
+    assert step(_table(scales=0x3080), bits=8) == -7                                  # (the 256 codes of m end at 0x3100)
+    assert step(_table(), _table()) == -7 and step(_table(), _table(**{**far, 'step': 0x6000})) == -7
+    assert step(_table(), _table(**{**far, 'grad': 0x13000})) == -7 and step(_table(n=8192), _table(**far)) == -7
+    assert step(_table(), _table(**{**far, 'dtype': 1, 'm': 0x111fc})) == -7          # 256 bfloat16 values end at 0x11200
+    long = (2 ** 24 - 1) * 2048
+    assert step(_table(n=long + 1)) == -2 and L.igcn_error_string(-7)
+
+
+def test_the_c_linear_rejects_bad_arguments_before_any_launch():
+    L = _lib.lib()
+    P = 0x1000
+
+    def linear(x=P, x_dtype=0, ldx=4096, b=P, ldb=4096, sb=P, bias=None, m=4, n=8, k=4096, y=P, dtype=0, ldy=8, ws=P):
+        return L.igcn_linear_i8(x, x_dtype, ldx, b, ldb, sb, bias, m, n, k, y, dtype, ldy, ws, None)
+    assert linear(dtype=3) == -4 and linear(x_dtype=-1) == -4 and linear(ldx=4095) == -2 and linear(ldb=1) == -2 and linear(ldy=7) == -2 and linear(m=-1) == -2
+    assert linear(k=131072, ldx=1 << 18, ldb=1 << 18) == -4 and linear(m=1 << 31) == -2
+    for kw in (dict(x=None), dict(b=None), dict(sb=None), dict(y=None), dict(ws=None)):
+        assert linear(**kw) == -1, kw
+    assert linear(x=0x1002) == -3 and linear(y=0x1002) == -3 and linear(sb=0x1001) == -3 and linear(bias=0x1002) == -3 and linear(ws=0x1008) == -3
+    assert linear(m=0, x=None, ws=None) == 0 and linear(n=0, ldy=0, ws=None) == 0
+    size = L.igcn_linear_i8_workspace_bytes
+    assert size(-1, 4) == -1 and size(4, -1) == -1 and size(4, 131072) == -1 and size(1 << 31, 4) == -1
+    assert size(1, 64) == 0 and size(4, 4096) >= 4 * 4096 + 16 and size(3, 8001) >= 3 * 8001 + 12
+
+
+def test_a_copied_optimizer_keeps_its_settings():
+    import copy
+    import pickle
+    w = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([w], lr=0.1, state_bits=8, max_grad_norm=2., seed=5)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.max_grad_norm == 2. and other.seed == 5 and other.param_groups[0]['state_bits'] == 8 and other.grad_norm is None

@@ -450,3 +450,59 @@ def test_train_in_8_bits_clip_quantize_and_answer():
         slack = (half + 8 * 2.0 ** -24) * (want.abs() + bound) + 64 * 2.0 ** -24 * u.abs().sum(1, keepdim=True) * i.abs().amax(1)
         assert bool(((got.double() - want).abs() <= bound * (1 + 1e-5) + slack).all())
     assert torch.equal(model.predict_i8(users), model.predict_i8(users, items))
+
+
+def test_refusals_leave_everything_as_it_was():
+    from igcn_cf_amd import _lib, ops
+    def lists(eight=False, shape=(40, 8)):
+        ps = [torch.ones(shape, device=DEV), torch.ones(300, device=DEV)]
+        gs = [torch.ones_like(p) for p in ps]
+        if eight:
+            ms, vs = ([torch.zeros_like(p, dtype=torch.uint8).view(d) for p in ps] for d in ops.MOMENT_DTYPES)
+        else:
+            ms, vs = ([torch.zeros_like(p) for p in ps] for _ in range(2))
+        steps = [torch.zeros((), device=DEV) for _ in ps]
+        scales = [torch.zeros((p.numel() + 127) // 128, 2, device=DEV) for p in ps]
+        return dict(params=ps, grads=gs, exp_avgs=ms, exp_avg_sqs=vs, steps=steps, scales=scales if eight else None, lr=0.1)
+
+    def change(name, at, value):
+        def f(kw):
+            kw[name][at] = value(kw) if callable(value) else value
+        return f
+
+    def setting(**new):
+        return lambda kw: kw.update(new)
+    buffer = torch.ones(700, device=DEV)
+    both = [change('params', 1, lambda kw: kw['params'][0]), change('steps', 1, lambda kw: kw['steps'][0]), change('exp_avgs', 1, lambda kw: kw['exp_avgs'][0]),
+            change('exp_avgs', 1, lambda kw: kw['exp_avg_sqs'][1].view(kw['exp_avgs'][1].dtype)), change('grads', 1, lambda kw: kw['params'][1]),
+            lambda kw: kw.update(params=[buffer[:320].view(40, 8), buffer[319:619]]),
+            change('grads', 0, torch.ones(8, 40, device=DEV)), change('grads', 0, torch.ones(8, 40, device=DEV).t()), change('grads', 0, torch.ones(40, 8, device=DEV, dtype=torch.float16)),
+            change('grads', 0, torch.ones(40, 8)), change('grads', 0, torch.ones(40, 1, device=DEV).expand(40, 8)), change('grads', 0, None),
+            change('params', 0, torch.ones(40, 8, device=DEV, dtype=torch.float64)), change('params', 0, torch.ones(40, 16, device=DEV)[:, ::2]),
+            change('exp_avgs', 0, torch.zeros(320, device=DEV)), change('exp_avg_sqs', 1, torch.zeros(300, device=DEV, dtype=torch.bfloat16)),
+            change('steps', 0, torch.zeros(2, device=DEV)), change('steps', 0, torch.zeros((), device=DEV, dtype=torch.int64)), change('steps', 0, torch.zeros(())),
+            lambda kw: kw['steps'].pop(), setting(lr=-1.), setting(lr=torch.ones(2, device=DEV)), setting(lr=torch.ones(())), setting(lr=torch.ones((), device=DEV, dtype=torch.float64)),
+            setting(betas=(0.9, 1.)), setting(eps=-1.), setting(weight_decay=float('nan')), setting(max_grad_norm=-1.), setting(max_grad_norm=float('nan')),
+            setting(max_grad_norm=1., grad_norm=torch.ones(())), setting(max_grad_norm=1., grad_norm=2.)]
+    eight_only = [change('scales', 0, torch.zeros(2, 2, device=DEV)), change('scales', 1, torch.zeros(3, 2, device=DEV, dtype=torch.float64)), change('scales', 0, torch.zeros(2, 3, device=DEV).t()),
+                  lambda kw: kw['scales'].pop(), setting(scales=None), change('exp_avgs', 0, torch.zeros(40, 8, device=DEV)), change('scales', 1, lambda kw: kw['scales'][0])]
+    for eight in (False, True):
+        for i, spoil in enumerate(both + (eight_only if eight else [])):
+            kw = lists(eight)
+            spoil(kw)
+            with pytest.raises(_lib.IgcnError):
+                ops.adamw_step(**kw)
+                print('not refused:', eight, i)
+            for name, want in (('params', 1.), ('steps', 0.)):
+                for t in kw[name]:
+                    assert bool((t.double() == want).all()), (eight, i, name)
+        kw = lists(eight)
+        kw['lr'], kw['betas'] = np.float32(0.1), (np.float32(0.9), np.float64(0.999))                       # numbers of any make
+        ops.adamw_step(seed=np.int64(-3), max_grad_norm=np.float32(1.), **kw)
+        shared = lists(eight, shape=(300,))
+        shared['grads'][1] = shared['grads'][0]                                                            # gradients may be one
+        ops.adamw_step(**shared)
+        assert bool((shared['params'][0] < 1).all()) and torch.equal(shared['params'][0], shared['params'][1])
+    for gs in ([torch.ones(3)], [torch.ones(3, device=DEV).double()], [torch.ones(1, device=DEV).expand(3)], [None], [torch.ones(4, 4, device=DEV)[:, 1]]):
+        with pytest.raises(_lib.IgcnError):
+            ops.grad_norm(gs)
