@@ -32,13 +32,25 @@ __device__ __forceinline__ void store_out(const GemmArgs &G, int64_t r, int64_t 
     else static_cast<__half *>(G.y)[r * G.ldy + c] = from_float<__half>(v);
 }
 
-// 16 codes of a row from k on, zeros behind its end
-__device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int64_t k, int64_t n)
+// 16 codes without their first `by` (16 and more: zeros)
+__device__ __forceinline__ i32x4 behind(i32x4 v, int by)
 {
+    const uint64_t lo = (uint32_t)v[0] | (uint64_t)(uint32_t)v[1] << 32, hi = (uint32_t)v[2] | (uint64_t)(uint32_t)v[3] << 32;
+    const int bits = 8 * (by & 7);
+    const uint64_t a = by >= 16 ? 0 : by >= 8 ? hi : lo, b = by >= 8 ? 0 : hi, c = a >> bits | (b << 1) << (63 - bits), d = b >> bits;
+    return i32x4{(int)c, (int)(c >> 32), (int)d, (int)(d >> 32)};
+}
+__device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ p) { return *reinterpret_cast<const i32x4_any *>(p); }
+// 16 codes of a row of n from k on, zeros behind its end: the last 16 of the row hold what is there of them
+__device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int k, int n)
+{
+    if (n >= 16) {
+        const int at = min(k, n - 16);
+        return behind(load16(row + at), k - at);
+    }
     i32x4 v = {0, 0, 0, 0};
-    if (k + 16 <= n) return *reinterpret_cast<const i32x4_any *>(row + k);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 15; ++i)
         if (k + i < n) v[i >> 2] |= (int)(uint8_t)row[k + i] << (8 * (i & 3));
     return v;
 }
@@ -87,6 +99,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     constexpr int kWaves = WM * WN, RT = TM / WM / 32, CT = TN / WN / 32, NA = TM / 8 / kWaves, NB = TN / 8 / kWaves;
     constexpr int kStage = (TM + TN) * kDepth;
     static_assert(!BY_DEPTH || (RT == 1 && CT == 1 && kWaves == kDepth / 32), "a quarter of the depth for each of four waves");
+    constexpr int AHEAD = TM <= 64 ? 3 : TM <= 128 ? 2 : 1;      // stages on their way in registers, where they go that way
     constexpr int AR = BY_DEPTH ? WM : RT, AC = BY_DEPTH ? WN : CT;       // pieces whose sums a wave holds
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     unsigned char *const ring = smem + (TM + 2 * TN) * 4;       // the stages; behind them, the strips of the way out
@@ -109,37 +122,45 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
     for (int i = 0; i < NB; ++i) ob[i] = (unsigned)min(8 * (wave * NB + i) + (lane >> 3), last_b) * (unsigned)G.ldb + piece(wave * NB + i);
     const int64_t stages = (G.k + kDepth - 1) / kDepth;
-    i32x4 held[DIRECT ? 1 : NA + NB];
+    i32x4 held[DIRECT ? 1 : AHEAD][DIRECT ? 1 : NA + NB];
     const unsigned lds0 = (unsigned)(uintptr_t)(lds_void *)ring;
 
-    auto fetch = [&](int64_t s) {                                // stage s of both sides: on its way to LDS, or to registers
-        const int64_t k0 = s * kDepth;
+    const int k = (int)G.k;
+    auto fetch = [&](int64_t s, auto &h) {                       // stage s of both sides: on its way to LDS, or to registers
+        const int k0 = (int)s * kDepth;
         if constexpr (DIRECT) {
             const unsigned at = lds0 + (unsigned)(s % STAGES) * kStage + wave * NA * 1024, bt = at + TM * kDepth + wave * (NB - NA) * 1024;
-            if (k0 + kDepth <= G.k) {
+            if (k0 + kDepth <= k) {
 #pragma unroll
                 for (int i = 0; i < NA; ++i) to_lds(base_a + k0, oa[i], at + 1024 * i);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) to_lds(base_b + k0, ob[i], bt + 1024 * i);
             } else {                                             // (pieces are whole: the depth is a multiple of 16)
 #pragma unroll
-                for (int i = 0; i < NA; ++i) to_lds(k0 + piece(wave * NA + i) < G.k ? (const void *)(base_a + k0 + oa[i]) : (const void *)&g_zeros, at + 1024 * i);
+                for (int i = 0; i < NA; ++i) to_lds(k0 + piece(wave * NA + i) < k ? (const void *)(base_a + k0 + oa[i]) : (const void *)&g_zeros, at + 1024 * i);
 #pragma unroll
-                for (int i = 0; i < NB; ++i) to_lds(k0 + piece(wave * NB + i) < G.k ? (const void *)(base_b + k0 + ob[i]) : (const void *)&g_zeros, bt + 1024 * i);
+                for (int i = 0; i < NB; ++i) to_lds(k0 + piece(wave * NB + i) < k ? (const void *)(base_b + k0 + ob[i]) : (const void *)&g_zeros, bt + 1024 * i);
             }
-        } else {
+        } else {                                                 // (past the end: the row's last 16 codes, put in place by land())
 #pragma unroll
-            for (int i = 0; i < NA; ++i) held[i] = load16(base_a + oa[i] - piece(wave * NA + i), k0 + piece(wave * NA + i), G.k);
+            for (int i = 0; i < NA; ++i) h[i] = load16(base_a + (oa[i] - piece(wave * NA + i)) + min(k0 + piece(wave * NA + i), k - 16));
 #pragma unroll
-            for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + ob[i] - piece(wave * NB + i), k0 + piece(wave * NB + i), G.k);
+            for (int i = 0; i < NB; ++i) h[NA + i] = load16(base_b + (ob[i] - piece(wave * NB + i)) + min(k0 + piece(wave * NB + i), k - 16));
         }
     };
-    auto land = [&](int64_t s) {                                 // registers to LDS
+    auto land = [&](int64_t s, auto &h) {                        // registers to LDS
         i32x4 *at = reinterpret_cast<i32x4 *>(ring + (s % STAGES) * kStage);
+        const int k0 = (int)s * kDepth;
+        if (k0 + kDepth > k && k >= 16) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = held[i];
+            for (int i = 0; i < NA; ++i) h[i] = behind(h[i], max(k0 + piece(wave * NA + i) - (k - 16), 0));
 #pragma unroll
-        for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
+            for (int i = 0; i < NB; ++i) h[NA + i] = behind(h[NA + i], max(k0 + piece(wave * NB + i) - (k - 16), 0));
+        }
+#pragma unroll
+        for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = h[i];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = h[NA + i];
     };
 
     i32x16 acc[AR][AC] = {};
@@ -152,9 +173,21 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         fc[i] = G.bias && i <= last_b ? G.bias[n0 + i] : 0.f;
     }
     if constexpr (DIRECT) {
-        for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s);
-    } else if (stages) { fetch(0); land(0); }
-    for (int64_t s = 0; s < stages; ++s) {
+        for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s, held[0]);
+    } else if (k >= 16) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+            if (d < stages) fetch(d, held[d]);
+        land(0, held[0]);
+        if (AHEAD < stages) fetch(AHEAD, held[0]);
+    } else if (k > 0) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) held[0][i] = load16(base_a + (oa[i] - piece(wave * NA + i)), piece(wave * NA + i), k);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) held[0][NA + i] = load16(base_b + (ob[i] - piece(wave * NB + i)), piece(wave * NB + i), k);
+        land(0, held[0]);
+    }
+    auto stage = [&](int64_t s, auto &h) {
         if constexpr (DIRECT) {                                  // stage s is there: all but the STAGES - 2 behind it
             if (s + STAGES - 2 < stages) wait_for_lds<(STAGES - 2) * (NA + NB)>(); else wait_for_lds<0>();
         }
@@ -169,7 +202,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
             for (int c = 0; c < AC; ++c) bv[c] = *reinterpret_cast<const i32x4 *>(sb + c * 32 * kDepth + at);
         };
         read(BY_DEPTH ? wave : 0);                               // (before the next stage is sent for: its addresses take a while)
-        if (s + STAGES - 1 < stages) fetch(s + STAGES - 1);
+        if constexpr (DIRECT) if (s + STAGES - 1 < stages) fetch(s + STAGES - 1, h);
 #pragma unroll
         for (int j = 0; j < (BY_DEPTH ? 1 : kDepth / 32); ++j) {
             if (j) read(j);
@@ -178,7 +211,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
                 for (int c = 0; c < AC; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[c], av[r], acc[r][c], 0, 0, 0);
         }
-        if constexpr (!DIRECT) if (s + 1 < stages) land(s + 1);
+        if constexpr (!DIRECT) if (s + 1 < stages) {
+            land(s + 1, h);
+            if (s + 1 + AHEAD < stages) fetch(s + 1 + AHEAD, h);
+        }
+    };
+    if constexpr (DIRECT) for (int64_t s = 0; s < stages; ++s) stage(s, held[0]);
+    else for (int64_t s = 0; s < stages; s += AHEAD) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+            if (s + d < stages) stage(s + d, held[(d + 1) % AHEAD]);
     }
     __syncthreads();
     if constexpr (BY_DEPTH) {                                    // piece q of the tile goes to wave q: [piece][the three other waves][4 sums a lane and quarter]
@@ -268,7 +310,7 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
         size_t ring = (size_t)stages * (TM + TN) * kDepth;
         const size_t strips = WM * WN * 32 * (TN / WN * 4 + 16);
         if (ring < strips) ring = strips;
-        if (direct && BY_DEPTH && ring < kExchanged) ring = kExchanged;
+        if (BY_DEPTH && ring < kExchanged) ring = kExchanged;
         const size_t lds = (TM + 2 * TN) * 4 + ring;
         if (lds > 65536) {                                       // (once would do; it is a host call of well under a microsecond)
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -277,7 +319,7 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
         hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
         return launch_status();
     };
-    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true, BY_DEPTH>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false, false>, 2);
+    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true, BY_DEPTH>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false, BY_DEPTH>, 2);
 }
 
 // ---- up to 8 rows of a ----------------------------------------------------------------------------------------------------------------
@@ -325,14 +367,17 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int64_t r = (tile0 + t) * 16 + (lane & 15);
-            row[t] = G.b + (r < G.n ? r : G.n - 1) * G.ldb + 16 * quarter;
+            row[t] = G.b + (r < G.n ? r : G.n - 1) * G.ldb;
         }
     };
-    auto load = [&](int s) {                                     // steps s ... s + KEEP - 1, all of them whole
+    const int k = (int)G.k;
+    auto load = [&](int s, int to) {                             // steps s ... s + KEEP - 1; behind the wave's last one that one again,
+#pragma unroll                                                   // behind the row's end its last 16 codes
+        for (int u = 0; u < KEEP; ++u) {
+            const int at = min(min(s + u, to - 1) * kStep + 16 * quarter, k - 16);
 #pragma unroll
-        for (int u = 0; u < KEEP; ++u)
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) v[u][t] = *reinterpret_cast<const i32x4_any *>(row[t] + (int64_t)(s + u) * kStep);
+            for (int t = 0; t < TILES; ++t) v[u][t] = load16(row[t] + at);
+        }
     };
     auto range = [&](int p0, int &from, int &to) {               // this wave's steps of the panel from p0 on
         const int p1 = min(p0 + F.panel, steps);
@@ -345,7 +390,7 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     if (group0 * TILES < tiles) {                                // the first loads, before anything else
         range(0, from, to);
         rows_of(group0 * TILES);
-        if (from + KEEP <= min(to, whole)) { load(from); loaded = true; }
+        if (from < to && k >= 16) { load(from, to); loaded = true; }
     }
 
     if constexpr (kFloat) {                                      // (one panel: the whole depth)
@@ -383,7 +428,7 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
                 __syncthreads();
                 for (int i = threadIdx.x; i < (p1 - p0) * 4 * rows2; i += kBlock) {
                     const int r = i & (rows2 - 1), piece = i >> F.shift;
-                    xs[i] = r < m ? load16(G.a + r * G.lda, (int64_t)(p0 * 4 + piece) * 16, G.k) : i32x4{0, 0, 0, 0};
+                    xs[i] = r < m ? load16(G.a + r * G.lda, (p0 * 4 + piece) * 16, k) : i32x4{0, 0, 0, 0};
                 }
                 __syncthreads();
             }
@@ -392,26 +437,31 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t], xv, acc[t], 0, 0, 0);
             };
-            const int full = min(to, whole);
-            int s = from;
-            if (s + KEEP <= full && !loaded) load(s);
-            loaded = false;
-            while (s + KEEP <= full) {
-                i32x4 w[KEEP][TILES];
+            if (k >= 16) {
+                if (from < to && !loaded) load(from, to);
+                loaded = false;
+                for (int s = from; s < to; s += KEEP) {
+                    i32x4 w[KEEP][TILES];
 #pragma unroll
-                for (int u = 0; u < KEEP; ++u)
+                    for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-                    for (int t = 0; t < TILES; ++t) w[u][t] = v[u][t];
-                s += KEEP;
-                if (s + KEEP <= full) load(s);                   // the next ones while these are multiplied
+                        for (int t = 0; t < TILES; ++t) w[u][t] = v[u][t];
+                    if (s + KEEP < to) load(s + KEEP, to);       // the next ones while these are multiplied
 #pragma unroll
-                for (int u = 0; u < KEEP; ++u) multiply(w[u], s - KEEP + u);
-            }
-            for (; s < to; ++s) {
+                    for (int u = 0; u < KEEP; ++u)
+                        if (s + u < to) {
+                            if (s + u >= whole) {
+#pragma unroll
+                                for (int t = 0; t < TILES; ++t) w[u][t] = behind(w[u][t], max((s + u) * kStep + 16 * quarter - (k - 16), 0));
+                            }
+                            multiply(w[u], s + u);
+                        }
+                }
+            } else if (from < to) {
                 i32x4 w[TILES];
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) w[t] = load16(row[t] - 16 * quarter, (int64_t)s * kStep + 16 * quarter, G.k);
-                multiply(w, s);
+                for (int t = 0; t < TILES; ++t) w[t] = load16(row[t], 16 * quarter, k);
+                multiply(w, from);
             }
         }
         if constexpr (SHARE) {                                   // lane l holds rows of b 4 (l / 16) + i, row l % 16 of a
