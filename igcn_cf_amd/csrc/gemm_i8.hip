@@ -9,6 +9,7 @@
 namespace igcn {
 
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef int int_any __attribute__((aligned(1)));
 
 struct GemmArgs {
     const int8_t *a, *b;
@@ -327,9 +328,14 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
 // operand straight from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and the rows of a, the second
 // operand, from LDS, where a workgroup lays them out once in the order the lanes read them: [64 codes of depth][16 of them][row][16 bytes].
 // Rows of a are rounded up to a power of two there (lanes past it read another row's bytes; what they compute is not stored).
-// SHARE: with a long depth the four waves of a workgroup take a quarter of it each and add their sums up in LDS (whole numbers: in any
-// order), which fills the card four times as well where b has few rows; with a short one every wave has TILES of its own.  KEEP loads of
-// a wave are under way at a time, the first ones before the rows of a are laid out: their time hides behind the bytes of b.
+// SHARE: the four waves of a workgroup take a quarter of the depth each and add their sums up in LDS (whole numbers: in any order); else
+// every wave has TILES of its own.  The first fills the card where b has few rows and a wave's loads where they are long, the second
+// has fewer workgroups to start (8 rows, us: 562 x 64 3.6 and 6.1, 16384 x 512 5.8 and 10.2, 50000 x 256 12.4 and 9.1, 96421 x 64 10.0 and 7.4, 96421 x 512
+// 18.8 and 16.5, x 768 20.2 and 21.2, x 960 21.8 and 27.0).  KEEP loads of a wave are under way at a time, the first ones before the rows
+// of a are laid out: their time hides behind the bytes of b.
+// BYTES: rows of b at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it (1 row
+// against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first and the last row
+// of b, whose words may reach over its ends, are loaded as they are.  Codes of b behind the row's end meet zeros of a.
 // x in floating point (X is not int8_t): every workgroup makes it 8-bit on the way, with the quantiser's own steps — no launch, no
 // buffer; worth it while that is less work than a launch (against 16384 rows of b: 1 x 2048 10.9 us this way and 12.4 in two launches,
 // 1 x 4096 19.5 and 16.1; 4 x 512 against 96421 rows 16.7 and 19.4, 4 x 2048 against 16384 13.1 and 12.3).
@@ -346,7 +352,7 @@ struct FewArgs {
     int64_t jobs;                                                // of a workgroup at most: tile groups it walks
 };
 
-template <int TILES, int KEEP, bool SHARE, typename X>
+template <int TILES, int KEEP, bool SHARE, bool BYTES, typename X>
 __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -361,23 +367,32 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     const int64_t group0 = (int64_t)blockIdx.x * F.jobs * (SHARE ? 1 : 4) + (SHARE ? 0 : wave);
     constexpr bool kFloat = !std::is_same<X, int8_t>::value;
 
+    const int k = (int)G.k;
     const int8_t *row[TILES];
+    int off[TILES], last[TILES], more[TILES];                    // BYTES: of the row behind a multiple of 4; the last piece's place; to the fifth word
     i32x4 v[KEEP][TILES], acc[TILES];
+    int fifth[KEEP][TILES];
     auto rows_of = [&](int64_t tile0) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const int64_t r = (tile0 + t) * 16 + (lane & 15);
-            row[t] = G.b + (r < G.n ? r : G.n - 1) * G.ldb;
+            const int64_t r = min((tile0 + t) * 16 + (lane & 15), G.n - 1);
+            const bool inner = BYTES && r > 0 && r < G.n - 1;
+            row[t] = G.b + r * G.ldb;
+            off[t] = inner ? (int)(reinterpret_cast<uintptr_t>(row[t]) & 3) : 0;
+            last[t] = inner ? (k + 3) / 4 * 4 - 16 : k - 16;
+            more[t] = inner ? 16 : 0;
+            row[t] -= off[t];
         }
     };
-    const int k = (int)G.k;
     auto load = [&](int s, int to) {                             // steps s ... s + KEEP - 1; behind the wave's last one that one again,
 #pragma unroll                                                   // behind the row's end its last 16 codes
-        for (int u = 0; u < KEEP; ++u) {
-            const int at = min(min(s + u, to - 1) * kStep + 16 * quarter, k - 16);
+        for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) v[u][t] = load16(row[t] + at);
-        }
+            for (int t = 0; t < TILES; ++t) {
+                const int8_t *p = row[t] + min(min(s + u, to - 1) * kStep + 16 * quarter, last[t]);
+                v[u][t] = load16(p);
+                if constexpr (BYTES) fifth[u][t] = *reinterpret_cast<const int_any *>(p + more[t]);
+            }
     };
     auto range = [&](int p0, int &from, int &to) {               // this wave's steps of the panel from p0 on
         const int p1 = min(p0 + F.panel, steps);
@@ -445,14 +460,21 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
 #pragma unroll
                     for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-                        for (int t = 0; t < TILES; ++t) w[u][t] = v[u][t];
+                        for (int t = 0; t < TILES; ++t) {
+                            w[u][t] = v[u][t];
+                            if constexpr (BYTES) {
+                                const int five[5] = {v[u][t][0], v[u][t][1], v[u][t][2], v[u][t][3], fifth[u][t]};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) w[u][t][i] = (int)__builtin_amdgcn_alignbyte((uint32_t)five[i + 1], (uint32_t)five[i], (uint32_t)off[t]);
+                            }
+                        }
                     if (s + KEEP < to) load(s + KEEP, to);       // the next ones while these are multiplied
 #pragma unroll
                     for (int u = 0; u < KEEP; ++u)
                         if (s + u < to) {
                             if (s + u >= whole) {
 #pragma unroll
-                                for (int t = 0; t < TILES; ++t) w[u][t] = behind(w[u][t], max((s + u) * kStep + 16 * quarter - (k - 16), 0));
+                                for (int t = 0; t < TILES; ++t) w[u][t] = behind(w[u][t], max((s + u) * kStep + 16 * quarter - last[t], 0));
                             }
                             multiply(w[u], s + u);
                         }
@@ -460,7 +482,7 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
             } else if (from < to) {
                 i32x4 w[TILES];
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) w[t] = load16(row[t], 16 * quarter, k);
+                for (int t = 0; t < TILES; ++t) w[t] = load16(row[t] + off[t], 16 * quarter, k);
                 multiply(w, from);
             }
         }
@@ -502,7 +524,7 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     while ((1 << F.shift) < F.g.m) ++F.shift;
     const int64_t fits = kPanelBytes / (kStep << F.shift);
     F.panel = (int)(steps < fits ? (steps ? steps : 1) : fits);
-    const bool share = steps >= 16;                              // a quarter of the depth is a batch of loads at least
+    const bool share = steps >= 12 || tiles <= 2048;
     constexpr int kOwn = 4;
     const int64_t per = share ? 1 : 4 * kOwn, groups = (tiles + per - 1) / per;
     // a workgroup that lays the rows of a out once and walks several tiles with them: as many as keep 2 048 workgroups busy
@@ -510,8 +532,10 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     const int64_t blocks = (groups + F.jobs - 1) / F.jobs;
     if (blocks >= ((int64_t)1 << 32) / kBlock) return IGCN_E_SHAPE;              // (2^32 threads of a launch)
     const size_t lds = ((size_t)F.panel * kStep << F.shift) + (share ? 4 * 16 * 17 * 4 : 0);
-    if (share) hipLaunchKernelGGL((few_rows_i8_kernel<1, 4, true, X>), dim3((unsigned)blocks), dim3(kBlock), lds, st, F);
-    else hipLaunchKernelGGL((few_rows_i8_kernel<kOwn, 1, false, X>), dim3((unsigned)blocks), dim3(kBlock), lds, st, F);
+    const bool bytes = ((reinterpret_cast<uintptr_t>(F.g.b) | (uintptr_t)F.g.ldb) & 3) != 0;
+    auto launch = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), lds, st, F); };
+    if (share) bytes ? launch(few_rows_i8_kernel<1, 4, true, true, X>) : launch(few_rows_i8_kernel<1, 4, true, false, X>);
+    else bytes ? launch(few_rows_i8_kernel<kOwn, 1, false, true, X>) : launch(few_rows_i8_kernel<kOwn, 1, false, false, X>);
     return launch_status();
 }
 
