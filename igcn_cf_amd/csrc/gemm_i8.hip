@@ -328,21 +328,21 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
 // operand straight from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and the rows of a, the second
 // operand, from LDS, where a workgroup lays them out once in the order the lanes read them: [64 codes of depth][16 of them][row][16 bytes].
 // Rows of a are rounded up to a power of two there (lanes past it read another row's bytes; what they compute is not stored).
-// SHARE: the four waves of a workgroup take a quarter of the depth each and add their sums up in LDS (whole numbers: in any order); else
-// every wave has TILES of its own.  The first fills the card where b has few rows and a wave's loads where they are long, the second
-// has fewer workgroups to start (8 rows, us: 562 x 64 3.6 and 6.1, 16384 x 512 5.8 and 10.2, 50000 x 256 12.4 and 9.1, 96421 x 64 10.0 and 7.4, 96421 x 512
-// 18.8 and 16.5, x 768 20.2 and 21.2, x 960 21.8 and 27.0).  KEEP loads of a wave are under way at a time, the first ones before the rows
-// of a are laid out: their time hides behind the bytes of b.
+// SHARE: the four waves of a workgroup take a quarter of the depth each and add their sums up in LDS (whole numbers: in any order), which
+// fills the card where b has few rows and a wave's loads where they are long.  KEEP loads of a wave are under way at a time, the first
+// ones before the rows of a are laid out: their time hides behind the bytes of b.  Many short rows of b start too many workgroups this way
+// (shares_depth): 64 x 64 tiles take them (8 rows, us this way and in tiles: 562 x 64 3.5 and 3.7, 16384 x 500 5.2 and 5.0, 65536 x 64 7.6 and 5.0,
+// 65536 x 500 14.7 and 11.0, x 1024 16.9 and 16.3, 1 row 65536 x 2193 41 and 54), or, x in floating point, waves with TILES of their own.
 // BYTES: rows of b at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it (1 row
 // against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first and the last row
 // of b, whose words may reach over its ends, are loaded as they are.  Codes of b behind the row's end meet zeros of a.
 // x in floating point (X is not int8_t): every workgroup makes it 8-bit on the way, with the quantiser's own steps — no launch, no
-// buffer; worth it while that is less work than a launch (against 16384 rows of b: 1 x 2048 10.9 us this way and 12.4 in two launches,
-// 1 x 4096 19.5 and 16.1; 4 x 512 against 96421 rows 16.7 and 19.4, 4 x 2048 against 16384 13.1 and 12.3).
+// buffer; worth it while that is less work than a launch (us this way and in two launches: 1 x 1024 against 4000 rows 5.3 and 7.0, 4 x 1024 5.6 and
+// 8.0, 8 x 1024 8.3 and 8.6, against 16384 13.1 and 11.2; 1 x 2048 8.7 and 7.7, against 96421 47.0 and 42.0).
 constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
-constexpr int kFewRows = 8;                                      // (12 rows against 16384 x 8192: 40 us, 34 in tiles; 8 rows: 32 and 34)
+constexpr int kFewRows = 8;                                      // (9 rows against 562 x 1024: 4.9 us, 5.9 in tiles; against 16384 x 4096 22.7 and 14.1; 8 rows: 16 and 14)
 constexpr int kPanelBytes = 32768;                               // of LDS for the rows of a: four workgroups on a CU
-constexpr int64_t kFusedValues = 2048;
+constexpr int64_t kFusedValues = 4096, kFusedDepth = 1024;
 
 struct FewArgs {
     GemmArgs g;
@@ -517,6 +517,8 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     }
 }
 
+static bool shares_depth(const GemmArgs &G) { return G.k > 11 * kStep || G.n <= 32768; }
+
 template <typename X> static int few_rows(FewArgs F, hipStream_t st)
 {
     const int64_t steps = (F.g.k + kStep - 1) / kStep, tiles = (F.g.n + 15) / 16;
@@ -524,7 +526,7 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     while ((1 << F.shift) < F.g.m) ++F.shift;
     const int64_t fits = kPanelBytes / (kStep << F.shift);
     F.panel = (int)(steps < fits ? (steps ? steps : 1) : fits);
-    const bool share = steps >= 12 || tiles <= 2048;
+    const bool share = std::is_same<X, int8_t>::value || shares_depth(F.g);
     constexpr int kOwn = 4;
     const int64_t per = share ? 1 : 4 * kOwn, groups = (tiles + per - 1) / per;
     // a workgroup that lays the rows of a out once and walks several tiles with them: as many as keep 2 048 workgroups busy
@@ -535,13 +537,13 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     const bool bytes = ((reinterpret_cast<uintptr_t>(F.g.b) | (uintptr_t)F.g.ldb) & 3) != 0;
     auto launch = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), lds, st, F); };
     if (share) bytes ? launch(few_rows_i8_kernel<1, 4, true, true, X>) : launch(few_rows_i8_kernel<1, 4, true, false, X>);
-    else bytes ? launch(few_rows_i8_kernel<kOwn, 1, false, true, X>) : launch(few_rows_i8_kernel<kOwn, 1, false, false, X>);
+    else if constexpr (!std::is_same<X, int8_t>::value) bytes ? launch(few_rows_i8_kernel<kOwn, 1, false, true, X>) : launch(few_rows_i8_kernel<kOwn, 1, false, false, X>);
     return launch_status();
 }
 
 static int product(const GemmArgs &G, hipStream_t st)
 {
-    if (G.m <= kFewRows || G.lda > kMostApart || G.ldb > kMostApart) {
+    if ((G.m <= kFewRows && shares_depth(G)) || G.lda > kMostApart || G.ldb > kMostApart) {
         const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
         for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 8 at a time)
             FewArgs F = {};
@@ -580,7 +582,7 @@ static int check_product(const float *sa, const int8_t *b, int64_t ldb, const fl
     return IGCN_OK;
 }
 
-static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && m * k <= kFusedValues; }      // (as steps of up to 8 rows well under kPanelBytes)
+static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && k <= kFusedDepth && m * k <= kFusedValues; }      // (8 rows of such steps are well under kPanelBytes)
 static int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 
 }  // namespace igcn
