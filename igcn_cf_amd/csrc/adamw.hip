@@ -110,20 +110,54 @@ template <int THREADS = kBlock> __device__ __forceinline__ double block_sum(doub
     return s;
 }
 
-// partial[blockIdx.x] = squares of the chunks blockIdx.x, + gridDim.x, ...: sums in float64, in an order that depends on the sizes alone
-__global__ __launch_bounds__(kBlock) void grad_squares_kernel(const TensorTable T, double *__restrict__ partial)
+// squares of elements i, i + kChunk, ... below `end`: four loads under way before the first sum
+template <typename G> __device__ __forceinline__ double run_squares(const G *__restrict__ g, int64_t i, int64_t end)
+{
+    constexpr int kDeep = 4;
+    double s = 0.0;
+    for (; i + (kDeep - 1) * kChunk + kPer <= end; i += kDeep * kChunk) {
+        G x[kDeep][kPer];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) load_vector(x[d], g + i + d * kChunk);
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) { const double y = to_float(x[d][k]); s = fma(y, y, s); }
+    }
+    for (; i < end; i += kChunk) s += chunk_squares(g, i, end);
+    return s;
+}
+
+// partial[blockIdx.x] = squares of the chunks per blockIdx.x ... + per - 1: sums in float64, in an order that depends on the sizes alone
+__global__ __launch_bounds__(kBlock) void grad_squares_kernel(const TensorTable T, int per, double *__restrict__ partial)
 {
     __shared__ double lds[kBlock / kWave];
     double s = 0.0;
-    for (int chunk = blockIdx.x; chunk < T.first[T.n]; chunk += gridDim.x) s += grad_chunk(T, chunk, threadIdx.x);
+    const int to = min((int)(blockIdx.x + 1) * per, T.first[T.n]);
+    for (int chunk = blockIdx.x * per; chunk < to;) {            // from tensor to tensor
+        const int k = tensor_of_chunk(T, chunk), stop = min(to, T.first[k + 1]);
+        const igcn_adamw_tensor &t = T.t[k];
+        const int64_t i = (int64_t)(chunk - T.first[k]) * kChunk + threadIdx.x * kPer, end = min(t.n, (int64_t)(stop - T.first[k]) * kChunk);
+        if (t.grad_dtype == IGCN_DTYPE_F32) s += run_squares(static_cast<const float *>(t.grad), i, end);
+        else if (t.grad_dtype == IGCN_DTYPE_BF16) s += run_squares(static_cast<const __hip_bfloat16 *>(t.grad), i, end);
+        else s += run_squares(static_cast<const __half *>(t.grad), i, end);
+        chunk = stop;
+    }
     s = block_sum(s, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
 __device__ __forceinline__ double norm_of(const double *__restrict__ partial, int n, double *lds)
 {
+    constexpr int kEach = kNormBlocks / kBlock;                  // (all of one launch's at once)
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += kBlock) s += partial[i];
+    for (int i0 = threadIdx.x; i0 < n; i0 += kNormBlocks) {
+        double x[kEach];
+#pragma unroll
+        for (int d = 0; d < kEach; ++d) x[d] = i0 + d * kBlock < n ? partial[i0 + d * kBlock] : 0.0;
+#pragma unroll
+        for (int d = 0; d < kEach; ++d) s += x[d];
+    }
     return sqrt(block_sum(s, lds));
 }
 
@@ -362,8 +396,8 @@ static int grad_squares(const igcn_adamw_tensor *tensors, int64_t n, double *par
     return for_tables(tensors, n, [&](const TensorTable &T, int) {
         const int chunks = T.first[T.n];
         if (chunks == 0) return (int)IGCN_OK;
-        const int blocks = chunks < kNormBlocks ? chunks : kNormBlocks;
-        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, T, partial + *n_partial);
+        const int least = (chunks + kNormBlocks - 1) / kNormBlocks, per = least == 1 ? 1 : (least + 3) / 4 * 4, blocks = (chunks + per - 1) / per;
+        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, T, per, partial + *n_partial);
         *n_partial += blocks;
         return launch_status();
     });
