@@ -3,6 +3,9 @@
 //   y[m, n] = (sum_k a[m, k] b[n, k]) sa[m] sb[n] (+ bias[n])
 //
 // The sum is exact (int32: K <= 131 071); the scales are applied once, in float32, before the one rounding to the output's type.
+//
+// Measured: 8192 x 8192 x 4096 to bfloat16 264 us = 2.1 POP/s (a library's bare int8 product: 306 us), 512 x 96421 x 64 to float32 48-56 us = 4.2 TB/s
+// of y (the same stores alone 45), 4 x 16384 x 8192 31 us = 4.4 TB/s of b, 1 x 96421 x 64 from float32 7.5 us.
 #include "quant_i8.h"
 #include <type_traits>
 
@@ -61,14 +64,14 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int k, i
 // 32 x 32 pieces (v_mfma_i32_32x32x32_i8: lane l holds row l % 32, 16 bytes of depth at 16 (l / 32)).  128 codes of depth of either side
 // go to LDS per stage, two stages in turn: the next one is on its way from memory while this one is multiplied, one barrier a stage.
 // DIRECT (rows 16-byte aligned, depth a multiple of 16): memory to LDS without registers (global_load_lds, 1 KiB a wave and
-// instruction, lane after lane); else through registers.  A row's eight 16-byte pieces stand in LDS at piece ^ (row / 2 % 8): 16 lanes that read the
+// instruction, lane after lane); else through registers, AHEAD stages of them under way (13 x 5466 x 1917: 10.9 us; one: 18.1).  A row's eight 16-byte pieces stand in LDS at piece ^ (row / 2 % 8): 16 lanes that read the
 // same piece of 16 neighbouring rows hit 64 different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
 // Depth past the end reads a block of zeros, rows past the end the last row (not stored).
 // BY_DEPTH (a 64 x 64 tile of four waves): a wave takes a quarter of the stage's depth for the whole tile instead of all of it for its own piece,
 // and they exchange sums in the end: LDS is read half as often and no product waits for the one before it (64 x 1000 x 8192: 23.6 -> 18.1 us;
 // 64 x 96421 x 64: 8.2 -> 11.4, so only where the depth pays for the exchange).
 // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, 4 tiles of a deep at a time, so that the tiles under way there
-// share their rows in its L2.
+// share their rows in its L2 (512 x 96421 x 64, whose rows of y end inside a line, without: 47 -> 74 us).
 constexpr int kDepth = 128;
 __device__ const i32x4 g_zeros = {0, 0, 0, 0};
 
