@@ -780,19 +780,13 @@ ADAMW_BLOCK = 128                  # IGCN_ADAMW_BLOCK: consecutive elements that
 MOMENT_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)                        # of exp_avg and exp_avg_sq in 8 bits
 
 
-class _on:
-    """The device of a tensor as the current one, for a call's launches and workspaces (nothing to do where it is already)."""
+def _elsewhere(t):
+    """Whether the launches for t would go to another device than the current one."""
+    return t.get_device() != torch._C._cuda_getDevice()
 
-    def __init__(self, device):
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _stream_of(t):
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _dense(t):
@@ -813,16 +807,16 @@ def _same_order(a, b):
 
 def _check_grads(grads):
     """The one device the gradients are on."""
-    if not grads:
-        return None
-    if not all(isinstance(g, torch.Tensor) for g in grads) or not all(g.is_cuda for g in grads) or {g.layout for g in grads} != {torch.strided} \
-            or not {g.dtype for g in grads} <= _DTYPE_CODES.keys():
-        raise _lib.IgcnError('gradients must be dense float32, bfloat16 or float16 tensors on the GPU (no CPU path)')
-    if len({g.get_device() for g in grads}) != 1:
-        raise _lib.IgcnError('the tensors of a call must be on one device')
-    if not all(g.is_contiguous() or _dense(g) for g in grads):
-        raise _lib.IgcnError('gradients must fill a stretch of memory (a view with gaps or repeats does not)')
-    return grads[0].device
+    at = None
+    for g in grads:
+        if not isinstance(g, torch.Tensor) or not g.is_cuda or g.dtype not in _DTYPE_CODES or g.layout is not torch.strided:
+            raise _lib.IgcnError('gradients must be dense float32, bfloat16 or float16 tensors on the GPU (no CPU path)')
+        if not g.is_contiguous() and not _dense(g):
+            raise _lib.IgcnError('gradients must fill a stretch of memory (a view with gaps or repeats does not)')
+        if at is not None and g.get_device() != at:
+            raise _lib.IgcnError('the tensors of a call must be on one device')
+        at = g.get_device()
+    return grads[0].device if grads else None
 
 
 def grad_norm(grads):
@@ -833,14 +827,16 @@ def grad_norm(grads):
     device = _check_grads(grads)
     if not grads:
         return torch.zeros((), dtype=torch.float32, device='cuda')
+    if _elsewhere(grads[0]):
+        with torch.cuda.device(device):
+            return grad_norm(grads)
     rows = array.array('q')
     for g in grads:
         rows.extend((0, g.data_ptr(), 0, 0, 0, 0, g.numel(), _DTYPE_CODES[g.dtype] << 32))
-    with _on(device):
-        L, table = _lib.lib(), rows.buffer_info()[0]
-        ws = torch.empty(L.igcn_adamw_workspace_bytes(table, len(grads)), dtype=torch.uint8, device=device)
-        out = torch.empty((), dtype=torch.float32, device=device)
-        _lib.check(L.igcn_grad_norm(table, len(grads), out.data_ptr(), ws.data_ptr(), _lib.current_stream()), 'igcn_grad_norm')
+    L, table = _lib.lib(), rows.buffer_info()[0]
+    ws = torch.empty(L.igcn_adamw_workspace_bytes(table, len(grads)), dtype=torch.uint8, device=device)
+    out = torch.empty((), dtype=torch.float32, device=device)
+    _lib.check(L.igcn_grad_norm(table, len(grads), out.data_ptr(), ws.data_ptr(), _stream_of(out)), 'igcn_grad_norm')
     return out
 
 
@@ -867,6 +863,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and weight_decay >= 0.):
         raise _lib.IgcnError('betas must be in [0, 1), eps and weight_decay not negative')
     device = _check_grads(grads)
+    if n and _elsewhere(grads[0]):
+        with torch.cuda.device(device):
+            return adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay, max_grad_norm, scales if eight else None, seed, grad_norm)
     if n and {t.get_device() for ts in (params, exp_avgs, exp_avg_sqs, steps, scales if eight else ()) for t in ts} != {device.index}:
         raise _lib.IgcnError('the tensors of a call must be on one device, a GPU')
     pt, gt = [p.dtype for p in params], [g.dtype for g in grads]
@@ -902,38 +901,40 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
         norm_in = grad_norm
     if n == 0:
         return None if max_grad_norm is None else norm_in if norm_in is not None else torch.zeros((), dtype=torch.float32, device='cuda')
-    with _on(device):
-        L, table = _lib.lib(), rows.buffer_info()[0]
-        ws = torch.empty(L.igcn_adamw_workspace_bytes(table, n), dtype=torch.uint8, device=device)
-        norm, max_norm, norm_out = norm_in, 0., None
-        if max_grad_norm is not None:
-            max_norm = float(max_grad_norm)
-            if norm_in is None:
-                norm = torch.empty((), dtype=torch.float32, device=device)
-                norm_out = norm.data_ptr()
-        code = L.igcn_adamw_step(table, n, 8 if eight else 32, float(lr), _lib.ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
-                                 float(weight_decay), max_norm, _lib.ptr(norm_in),
-                                 norm_out, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), _lib.current_stream())
-        if code:
-            _lib.check(code, 'igcn_adamw_step')
+    L, table = _lib.lib(), rows.buffer_info()[0]
+    ws = torch.empty(L.igcn_adamw_workspace_bytes(table, n), dtype=torch.uint8, device=device)
+    norm, max_norm, norm_out = norm_in, 0., None
+    if max_grad_norm is not None:
+        max_norm = float(max_grad_norm)
+        if norm_in is None:
+            norm = torch.empty((), dtype=torch.float32, device=device)
+            norm_out = norm.data_ptr()
+    code = L.igcn_adamw_step(table, n, 8 if eight else 32, float(lr), _lib.ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
+                             float(weight_decay), max_norm, _lib.ptr(norm_in),
+                             norm_out, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index))
+    if code:
+        _lib.check(code, 'igcn_adamw_step')
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
     return norm
 
 
 # ---- rows in 8-bit integers and their product (csrc/gemm_i8.hip) ------------------------------------------------------------------
 MAX_I8_DEPTH = 131071              # IGCN_MAX_I8_DEPTH: the longest sum of 8-bit products that int32 holds
+_INT8 = (torch.int8,)
 
 
-def _require_rows(t, name, dtypes):
+def _rows_ld(t, name, dtypes):
+    """Leading dimension of 2-D rows on the GPU (a single row has whatever stride)."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
         raise _lib.IgcnError('%s must be a %s tensor on the GPU (no CPU path)' % (name, ' / '.join(str(d).replace('torch.', '') for d in dtypes)))
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise _lib.IgcnError('%s must be 2-D, its rows contiguous and apart' % name)
-
-
-def _ld(t):
-    """Leading dimension of 2-D rows (a single row has whatever stride)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    if t.dim() == 2 and t.layout is torch.strided:
+        m, k = t.shape
+        if t.is_contiguous():
+            return k
+        apart, one = t.stride()
+        if (k <= 1 or one == 1) and (m <= 1 or apart >= k):
+            return apart if m > 1 else k
+    raise _lib.IgcnError('%s must be 2-D, its rows contiguous and apart' % name)
 
 
 def _require_vector(t, name, n, like):
@@ -945,27 +946,30 @@ def quantize_rows_i8(x):
     """(codes int8 [M, K], scale float32 [M]) of the rows of x (float32, bfloat16 or float16 [M, K], rows contiguous): scale =
     max|row| / 127, codes = row / scale to the nearest whole number, ties to even (igcn_quantize_rows_i8).  A row of zeros has scale 0;
     one with a NaN or an infinity has scale NaN, so that what is computed from it shows it.  No gradient: rounding has none."""
-    _require_rows(x, 'x', tuple(_DTYPE_CODES))
+    ld = _rows_ld(x, 'x', _DTYPE_CODES)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return quantize_rows_i8(x)
     m, k = x.shape
-    with _on(x.device):
-        q = torch.empty((m, k), dtype=torch.int8, device=x.device)
-        scale = torch.empty(m, dtype=torch.float32, device=x.device)
-        _lib.check(_lib.lib().igcn_quantize_rows_i8(x.data_ptr(), _DTYPE_CODES[x.dtype], _ld(x), m, k, q.data_ptr(), k, scale.data_ptr(),
-                                                    _lib.current_stream()), 'igcn_quantize_rows_i8')
+    q, scale = x.new_empty((m, k), dtype=torch.int8), x.new_empty(m, dtype=torch.float32)
+    _lib.check(_lib.lib().igcn_quantize_rows_i8(x.data_ptr(), _DTYPE_CODES[x.dtype], ld, m, k, q.data_ptr(), k, scale.data_ptr(), _stream_of(x)),
+               'igcn_quantize_rows_i8')
     return q, scale
 
 
 def dequantize_rows_i8(codes, scale, dtype=torch.float32):
     """[M, K] of `dtype`: the values that rows of codes stand for, codes[m, k] * scale[m] (igcn_dequantize_rows_i8)."""
-    _require_rows(codes, 'codes', (torch.int8,))
+    ld = _rows_ld(codes, 'codes', _INT8)
     if dtype not in _DTYPE_CODES:
         raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
     m, k = codes.shape
     _require_vector(scale, 'scale', m, codes)
-    with _on(codes.device):
-        y = torch.empty((m, k), dtype=dtype, device=codes.device)
-        _lib.check(_lib.lib().igcn_dequantize_rows_i8(codes.data_ptr(), _ld(codes), scale.data_ptr(), m, k, y.data_ptr(), _DTYPE_CODES[dtype], k,
-                                                      _lib.current_stream()), 'igcn_dequantize_rows_i8')
+    if _elsewhere(codes):
+        with torch.cuda.device(codes.device):
+            return dequantize_rows_i8(codes, scale, dtype)
+    y = codes.new_empty((m, k), dtype=dtype)
+    _lib.check(_lib.lib().igcn_dequantize_rows_i8(codes.data_ptr(), ld, scale.data_ptr(), m, k, y.data_ptr(), _DTYPE_CODES[dtype], k, _stream_of(codes)),
+               'igcn_dequantize_rows_i8')
     return y
 
 
@@ -983,35 +987,37 @@ def _check_product(a, name, m, k, b, b_scale, bias):
 def matmul_i8(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
     """[M, N] of `dtype`: (a @ b.T) * a_scale[:, None] * b_scale (+ bias) for 8-bit integer rows a [M, K] and b [N, K] with a float32
     scale each (igcn_matmul_i8).  The sums are exact, K <= 131071."""
-    _require_rows(a, 'a', (torch.int8,))
-    _require_rows(b, 'b', (torch.int8,))
+    lda, ldb = _rows_ld(a, 'a', _INT8), _rows_ld(b, 'b', _INT8)
     (m, k), n = a.shape, b.shape[0]
     _check_product(a, 'a', m, k, b, b_scale, bias)
     if dtype not in _DTYPE_CODES:
         raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
     _require_vector(a_scale, 'a_scale', m, a)
-    with _on(a.device):
-        y = torch.empty((m, n), dtype=dtype, device=a.device)
-        _lib.check(_lib.lib().igcn_matmul_i8(a.data_ptr(), _ld(a), a_scale.data_ptr(), b.data_ptr(), _ld(b), b_scale.data_ptr(), _lib.ptr(bias),
-                                             m, n, k, y.data_ptr(), _DTYPE_CODES[dtype], n, _lib.current_stream()), 'igcn_matmul_i8')
+    if _elsewhere(a):
+        with torch.cuda.device(a.device):
+            return matmul_i8(a, a_scale, b, b_scale, bias, dtype)
+    y = a.new_empty((m, n), dtype=dtype)
+    _lib.check(_lib.lib().igcn_matmul_i8(a.data_ptr(), lda, a_scale.data_ptr(), b.data_ptr(), ldb, b_scale.data_ptr(), _lib.ptr(bias), m, n, k,
+                                         y.data_ptr(), _DTYPE_CODES[dtype], n, _stream_of(a)), 'igcn_matmul_i8')
     return y
 
 
 def linear_i8(x, b, b_scale, bias=None, dtype=None):
     """[M, N] of `dtype` (None: that of x): the rows of x made 8-bit, as quantize_rows_i8 makes them, and multiplied with those of b, as
     matmul_i8 does (igcn_linear_i8: one call, a few short rows in one launch).  For answering: no gradient."""
-    _require_rows(x, 'x', tuple(_DTYPE_CODES))
-    _require_rows(b, 'b', (torch.int8,))
+    ldx, ldb = _rows_ld(x, 'x', _DTYPE_CODES), _rows_ld(b, 'b', _INT8)
     (m, k), n = x.shape, b.shape[0]
     _check_product(x, 'x', m, k, b, b_scale, bias)
     out = _DTYPE_CODES.get(x.dtype if dtype is None else dtype)
     if out is None:
         raise _lib.IgcnError('dtype must be float32, bfloat16 or float16')
-    with _on(x.device):
-        L = _lib.lib()
-        y = torch.empty((m, n), dtype=dtype or x.dtype, device=x.device)
-        need = L.igcn_linear_i8_workspace_bytes(m, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        _lib.check(L.igcn_linear_i8(x.data_ptr(), _DTYPE_CODES[x.dtype], _ld(x), b.data_ptr(), _ld(b), b_scale.data_ptr(), _lib.ptr(bias), m, n, k,
-                                    y.data_ptr(), out, n, _lib.ptr(ws), _lib.current_stream()), 'igcn_linear_i8')
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return linear_i8(x, b, b_scale, bias, dtype)
+    L = _lib.lib()
+    y = x.new_empty((m, n), dtype=dtype or x.dtype)
+    need = L.igcn_linear_i8_workspace_bytes(m, k)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    _lib.check(L.igcn_linear_i8(x.data_ptr(), _DTYPE_CODES[x.dtype], ldx, b.data_ptr(), ldb, b_scale.data_ptr(), _lib.ptr(bias), m, n, k,
+                                y.data_ptr(), out, n, _lib.ptr(ws), _stream_of(x)), 'igcn_linear_i8')
     return y
