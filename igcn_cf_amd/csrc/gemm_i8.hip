@@ -326,32 +326,173 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
     return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true, BY_DEPTH>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false, BY_DEPTH>, 2);
 }
 
-// ---- up to 8 rows of a ----------------------------------------------------------------------------------------------------------------
-// Bound by the bytes of b, each used once: no tile of b is worth staging.  A wave takes 16 rows of b as the matrix instruction's first
-// operand straight from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and the rows of a, the second
-// operand, from LDS, where a workgroup lays them out once in the order the lanes read them: [64 codes of depth][16 of them][row][16 bytes].
-// Rows of a are rounded up to a power of two there (lanes past it read another row's bytes; what they compute is not stored).
-// SHARE: the four waves of a workgroup take a quarter of the depth each and add their sums up in LDS (whole numbers: in any order), which
-// fills the card where b has few rows and a wave's loads where they are long.  KEEP loads of a wave are under way at a time, the first
-// ones before the rows of a are laid out: their time hides behind the bytes of b.  Many short rows of b start too many workgroups this way
-// (shares_depth): 64 x 64 tiles take them (8 rows, us this way and in tiles: 562 x 64 3.5 and 3.7, 16384 x 500 5.2 and 5.0, 65536 x 64 7.6 and 5.0,
-// 65536 x 500 14.7 and 11.0, x 1024 16.9 and 16.3, 1 row 65536 x 2193 41 and 54), or, x in floating point, waves with TILES of their own.
-// BYTES: rows of b at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it (1 row
-// against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first and the last row
-// of b, whose words may reach over its ends, are loaded as they are.  Codes of b behind the row's end meet zeros of a.
-// x in floating point (X is not int8_t): every workgroup makes it 8-bit on the way, with the quantiser's own steps — no launch, no
-// buffer; worth it while that is less work than a launch (us this way and in two launches: 1 x 1024 against 4000 rows 5.3 and 7.0, 4 x 1024 5.6 and
-// 8.0, 8 x 1024 8.3 and 8.6, against 16384 13.1 and 11.2; 1 x 2048 8.7 and 7.7, against 96421 47.0 and 42.0).
+// ---- a few rows of a ------------------------------------------------------------------------------------------------------------------
+// Bound by the bytes of b, each used once: no tile is worth staging.  A wave takes 16 rows of b as the matrix instruction's first operand straight
+// from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and up to 16 rows of a, which stay in L2, as the
+// second.  KEEP steps' loads are under way while the ones before are multiplied.
 constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
-constexpr int kFewRows = 8;                                      // (9 rows against 562 x 1024: 4.9 us, 5.9 in tiles; against 16384 x 4096 22.7 and 14.1; 8 rows: 16 and 14)
-constexpr int kPanelBytes = 32768;                               // of LDS for the rows of a: four workgroups on a CU
+
+// A lane's row of b.  BYTES: rows at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it
+// (1 row against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first
+// and the last row of b, whose words may reach over its ends, are loaded as they are.  What is behind a row's end meets zeros of a.
+template <bool BYTES> struct RowOfB {
+    const int8_t *p;
+    int off, last, more;                                         // of the row behind a multiple of 4; the last piece's place; to the fifth word
+    struct Piece { i32x4 v; int fifth; };
+    __device__ __forceinline__ void at_row(const GemmArgs &G, int64_t r)
+    {
+        r = min(r, G.n - 1);
+        const int k = (int)G.k;
+        const bool inner = BYTES && r > 0 && r < G.n - 1;
+        p = G.b + r * G.ldb;
+        off = inner ? (int)(reinterpret_cast<uintptr_t>(p) & 3) : 0;
+        last = inner ? (k + 3) / 4 * 4 - 16 : k - 16;
+        more = inner ? 16 : 0;
+        p -= off;
+    }
+    __device__ __forceinline__ Piece load(int at) const          // depth `at` on; behind the row's end its last 16 codes (a row of 16 and more)
+    {
+        const int8_t *q = p + min(at, last);
+        Piece c;
+        c.v = load16(q);
+        if constexpr (BYTES) c.fifth = *reinterpret_cast<const int_any *>(q + more);
+        return c;
+    }
+    __device__ __forceinline__ i32x4 codes(const Piece &c) const
+    {
+        i32x4 w = c.v;
+        if constexpr (BYTES) {
+            const int five[5] = {c.v[0], c.v[1], c.v[2], c.v[3], c.fifth};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (int)__builtin_amdgcn_alignbyte((uint32_t)five[i + 1], (uint32_t)five[i], (uint32_t)off);
+        }
+        return w;
+    }
+    __device__ __forceinline__ i32x4 in_place(i32x4 w, int at) const { return behind(w, max(at - last, 0)); }      // of the last, broken step
+    __device__ __forceinline__ i32x4 short_row(int at, int k) const { return load16(p + off, at, k); }             // a row of fewer than 16
+};
+
+// 16 MG rows of a at most, TILES x 16 rows of b a workgroup.  Its four waves take a quarter of the depth each and add their sums up in LDS (whole
+// numbers: in any order), which fills the card where b has few rows and a wave's loads where they are long.  Rows of a come from L2 like
+// those of b from memory, no barrier until the end: laid out in LDS first, 8 rows against 4096 x 8192 took 17.4 us, this way 9.5.
+template <int MG, int TILES, bool BYTES>
+__global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
+{
+    constexpr int KEEP = 4;
+    __shared__ int sums[MG * TILES * 4 * 16 * 17];               // [group of a, tile, wave][row of a][17]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at_lane = 16 * (lane >> 4), m = (int)G.m, k = (int)G.k;
+    const int steps = (k + kStep - 1) / kStep, whole = k / kStep, from = steps * wave / 4, to = steps * (wave + 1) / 4;
+    const int64_t tile0 = (int64_t)blockIdx.x * TILES;
+    RowOfB<BYTES> row[TILES];
+    const int8_t *row_a[MG];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) row[t].at_row(G, (tile0 + t) * 16 + (lane & 15));
+#pragma unroll
+    for (int g = 0; g < MG; ++g) row_a[g] = G.a + min(16 * g + (lane & 15), m - 1) * G.lda;      // (rows past the end: not stored)
+    typename RowOfB<BYTES>::Piece v[KEEP][TILES];
+    i32x4 x[KEEP][MG], acc[MG][TILES];
+#pragma unroll
+    for (int g = 0; g < MG; ++g)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) acc[g][t] = i32x4{0, 0, 0, 0};
+    auto load = [&](int s) {                                     // steps s ... s + KEEP - 1; behind the wave's last one that one again
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) {
+            const int at = min(s + u, to - 1) * kStep + at_lane;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) v[u][t] = row[t].load(at);
+#pragma unroll
+            for (int g = 0; g < MG; ++g) x[u][g] = load16(row_a[g] + min(at, k - 16));
+        }
+    };
+    auto multiply = [&](const i32x4 (&w)[TILES], const i32x4 (&y)[MG]) {
+#pragma unroll
+        for (int g = 0; g < MG; ++g)
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) acc[g][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t], y[g], acc[g][t], 0, 0, 0);
+    };
+    if (k >= 16) {
+        if (from < to) load(from);
+        for (int s = from; s < to; s += KEEP) {
+            i32x4 w[KEEP][TILES], y[KEEP][MG];
+#pragma unroll
+            for (int u = 0; u < KEEP; ++u) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) w[u][t] = row[t].codes(v[u][t]);
+#pragma unroll
+                for (int g = 0; g < MG; ++g) y[u][g] = x[u][g];
+            }
+            if (s + KEEP < to) load(s + KEEP);                   // the next ones while these are multiplied
+#pragma unroll
+            for (int u = 0; u < KEEP; ++u)
+                if (s + u < to) {
+                    if (s + u >= whole) {
+                        const int at = (s + u) * kStep + at_lane;
+#pragma unroll
+                        for (int t = 0; t < TILES; ++t) w[u][t] = row[t].in_place(w[u][t], at);
+#pragma unroll
+                        for (int g = 0; g < MG; ++g) y[u][g] = behind(y[u][g], max(at - (k - 16), 0));
+                    }
+                    multiply(w[u], y[u]);
+                }
+        }
+    } else if (from < to) {
+        i32x4 w[TILES], y[MG];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) w[t] = row[t].short_row(at_lane, k);
+#pragma unroll
+        for (int g = 0; g < MG; ++g) y[g] = load16(row_a[g], at_lane, k);
+        multiply(w, y);
+    }
+    const int mine = lane & 15, quarter = lane >> 4;             // lane l holds rows of b 4 (l / 16) + i, row l % 16 of a
+#pragma unroll
+    for (int g = 0; g < MG; ++g)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[(((g * TILES + t) * 4 + wave) * 16 + mine) * 17 + 4 * quarter + i] = acc[g][t][i];
+    __syncthreads();
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+#pragma unroll
+    for (int g = 0; g < MG; ++g)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int64_t n = (tile0 + t) * 16 + c;
+            if (n < G.n && 16 * g + r < m) {
+                int sum = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) sum += sums[(((g * TILES + t) * 4 + w) * 16 + r) * 17 + c];
+                store_out(G, 16 * g + r, n, scaled(sum, G.sa[16 * g + r], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
+            }
+        }
+}
+
+static bool any_byte(const void *p, int64_t ld) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)ld) & 3) != 0; }
+static bool fits_launch(int64_t blocks) { return blocks < ((int64_t)1 << 32) / kBlock; }       // of kBlock threads: 2^32 in all
+
+template <int MG, int TILES> static int stream(const GemmArgs &G, hipStream_t st)
+{
+    const int64_t blocks = (G.n + 16 * TILES - 1) / (16 * TILES);
+    if (!fits_launch(blocks)) return IGCN_E_SHAPE;
+    auto launch = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, G); };
+    any_byte(G.b, G.ldb) ? launch(stream_i8_kernel<MG, TILES, true>) : launch(stream_i8_kernel<MG, TILES, false>);
+    return launch_status();
+}
+
+// The same for a few short rows in floating point: every workgroup makes them 8-bit on the way, with the quantiser's own steps, and lays them
+// out in LDS in the order the lanes read them: [16 codes of depth][row][16 bytes], rows rounded up to a power of two (lanes past them read
+// another row's bytes; what they compute is not stored).  No launch, no buffer; worth it while that is less work than a launch (us this way
+// and in two launches: 1 x 1024 against 4000 rows 5.3 and 7.0, 4 x 1024 5.6 and 8.0, 8 x 1024 8.3 and 8.6, against 16384 13.1 and 11.2; 1 x 2048 8.7 and
+// 7.7, against 96421 47.0 and 42.0).  SHARE: as above, else every wave has TILES of its own, which starts fewer workgroups where b has many
+// short rows (8 rows, us: 50000 x 256 12.4 and 9.1, 96421 x 64 10.0 and 7.4, x 768 20.2 and 21.2; 16384 x 512 5.8 and 10.2).
+constexpr int kFewRows = 8;
 constexpr int64_t kFusedValues = 4096, kFusedDepth = 1024;
 
 struct FewArgs {
     GemmArgs g;
-    const void *x;                                               // the rows of a in floating point (ldx apart), or NULL
+    const void *x;                                               // the rows of a in floating point, ldx apart
     int64_t ldx;
-    int shift, panel;                                            // 2^shift rows of a in LDS; steps of depth that fit there
+    int shift;                                                   // 2^shift rows of a in LDS
     int64_t jobs;                                                // of a workgroup at most: tile groups it walks
 };
 
@@ -361,151 +502,99 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float sx[kFewRows];
     const GemmArgs &G = F.g;
-    i32x4 *const xs = reinterpret_cast<i32x4 *>(smem);           // [step][quarter][row] x 16 bytes
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
-    const int rows2 = 1 << F.shift, m = (int)G.m;
-    int *const sums = reinterpret_cast<int *>(smem + (int64_t)F.panel * kStep * rows2);       // SHARE: [tile, wave][row of a][17]
-    const int steps = (int)((G.k + kStep - 1) / kStep), whole = (int)(G.k / kStep);
-    const int64_t tiles = (G.n + 15) / 16;
-    const int64_t group0 = (int64_t)blockIdx.x * F.jobs * (SHARE ? 1 : 4) + (SHARE ? 0 : wave);
-    constexpr bool kFloat = !std::is_same<X, int8_t>::value;
+    const i32x4 *const xs = reinterpret_cast<const i32x4 *>(smem);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4, rows2 = 1 << F.shift, m = (int)G.m, k = (int)G.k;
+    const int steps = (k + kStep - 1) / kStep, whole = k / kStep, from = SHARE ? steps * wave / 4 : 0, to = SHARE ? steps * (wave + 1) / 4 : steps;
+    int *const sums = reinterpret_cast<int *>(smem + (int64_t)steps * kStep * rows2);         // SHARE: [wave][row of a][17]
+    const int64_t tiles = (G.n + 15) / 16, group0 = (int64_t)blockIdx.x * F.jobs * (SHARE ? 1 : 4) + (SHARE ? 0 : wave);
+    static_assert(!SHARE || TILES == 1, "one tile's sums");
 
-    const int k = (int)G.k;
-    const int8_t *row[TILES];
-    int off[TILES], last[TILES], more[TILES];                    // BYTES: of the row behind a multiple of 4; the last piece's place; to the fifth word
-    i32x4 v[KEEP][TILES], acc[TILES];
-    int fifth[KEEP][TILES];
+    RowOfB<BYTES> row[TILES];
+    typename RowOfB<BYTES>::Piece v[KEEP][TILES];
+    i32x4 acc[TILES];
     auto rows_of = [&](int64_t tile0) {
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const int64_t r = min((tile0 + t) * 16 + (lane & 15), G.n - 1);
-            const bool inner = BYTES && r > 0 && r < G.n - 1;
-            row[t] = G.b + r * G.ldb;
-            off[t] = inner ? (int)(reinterpret_cast<uintptr_t>(row[t]) & 3) : 0;
-            last[t] = inner ? (k + 3) / 4 * 4 - 16 : k - 16;
-            more[t] = inner ? 16 : 0;
-            row[t] -= off[t];
-        }
+        for (int t = 0; t < TILES; ++t) row[t].at_row(G, (tile0 + t) * 16 + (lane & 15));
     };
-    auto load = [&](int s, int to) {                             // steps s ... s + KEEP - 1; behind the wave's last one that one again,
-#pragma unroll                                                   // behind the row's end its last 16 codes
+    auto load = [&](int s) {
+#pragma unroll
         for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                const int8_t *p = row[t] + min(min(s + u, to - 1) * kStep + 16 * quarter, last[t]);
-                v[u][t] = load16(p);
-                if constexpr (BYTES) fifth[u][t] = *reinterpret_cast<const int_any *>(p + more[t]);
-            }
+            for (int t = 0; t < TILES; ++t) v[u][t] = row[t].load(min(s + u, to - 1) * kStep + 16 * quarter);
     };
-    auto range = [&](int p0, int &from, int &to) {               // this wave's steps of the panel from p0 on
-        const int p1 = min(p0 + F.panel, steps);
-        from = SHARE ? p0 + (p1 - p0) * wave / 4 : p0;
-        to = SHARE ? p0 + (p1 - p0) * (wave + 1) / 4 : p1;
-        return p1;
-    };
-    int from, to;
-    bool loaded = false;
-    if (group0 * TILES < tiles) {                                // the first loads, before anything else
-        range(0, from, to);
-        rows_of(group0 * TILES);
-        if (from < to && k >= 16) { load(from, to); loaded = true; }
-    }
+    rows_of(group0 * TILES);
+    bool loaded = k >= 16 && from < to && group0 * TILES < tiles;
+    if (loaded) load(from);                                      // the first loads, before anything else
 
-    if constexpr (kFloat) {                                      // (one panel: the whole depth)
-        constexpr int E = Chunk<X>::kValues;
-        for (int r = wave; r < m; r += 4) {
-            const X *from_x = static_cast<const X *>(F.x) + r * F.ldx;
-            Largest<X> most;
-            for (int at = lane * E; at < G.k; at += 64 * E) { Chunk<X> c; c.load(from_x + at, G.k - at); most.of(c); }
-            uint32_t big = most.bits();
+    constexpr int E = Chunk<X>::kValues;
+    for (int r = wave; r < m; r += 4) {
+        const X *from_x = static_cast<const X *>(F.x) + r * F.ldx;
+        Largest<X> most;
+        for (int at = lane * E; at < k; at += 64 * E) { Chunk<X> c; c.load(from_x + at, k - at); most.of(c); }
+        uint32_t big = most.bits();
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off));
-            const RowScale s(big);
-            if (lane == 0) sx[r] = s.s;
-            for (int at = lane * E; at < steps * kStep; at += 64 * E) {
-                Chunk<X> c;
-                uint32_t w[E / 4];
-                c.load(from_x + at, G.k - at);
-                pack_codes<X>(w, c, s);
-                __builtin_memcpy(smem + ((at >> 4) * rows2 + r) * 16 + (at & 15), w, E);
-            }
+        for (int off = 32; off > 0; off >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off));
+        const RowScale s(big);
+        if (lane == 0) sx[r] = s.s;
+        for (int at = lane * E; at < steps * kStep; at += 64 * E) {
+            Chunk<X> c;
+            uint32_t w[E / 4];
+            c.load(from_x + at, k - at);
+            pack_codes<X>(w, c, s);
+            __builtin_memcpy(smem + ((at >> 4) * rows2 + r) * 16 + (at & 15), w, E);
         }
-    } else if (threadIdx.x < m) sx[threadIdx.x] = G.sa[threadIdx.x];
+    }
     __syncthreads();
 
     for (int64_t job = 0; job < F.jobs; ++job) {
         const int64_t tile0 = (group0 + job * (SHARE ? 1 : 4)) * TILES;
         if (SHARE ? tile0 >= tiles : tile0 - (int64_t)wave * TILES >= tiles) break;          // (the same for the whole workgroup)
-        if (job) { rows_of(tile0); loaded = false; }
-        else if (tile0 >= tiles) rows_of(tile0);
+        if (job) rows_of(tile0);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) acc[t] = i32x4{0, 0, 0, 0};
-        for (int p0 = 0; p0 < steps; p0 += F.panel) {
-            const int p1 = range(p0, from, to);
-            if constexpr (!kFloat) if (job == 0 || F.panel < steps) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < (p1 - p0) * 4 * rows2; i += kBlock) {
-                    const int r = i & (rows2 - 1), piece = i >> F.shift;
-                    xs[i] = r < m ? load16(G.a + r * G.lda, (p0 * 4 + piece) * 16, k) : i32x4{0, 0, 0, 0};
-                }
-                __syncthreads();
-            }
-            auto multiply = [&](const i32x4 (&w)[TILES], int s) {
-                const i32x4 xv = xs[((s - p0) * 4 + quarter) * rows2 + (lane & 15 & (rows2 - 1))];
+        auto multiply = [&](const i32x4 (&w)[TILES], int s) {
+            const i32x4 xv = xs[(s * 4 + quarter) * rows2 + (lane & 15 & (rows2 - 1))];
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t], xv, acc[t], 0, 0, 0);
-            };
-            if (k >= 16) {
-                if (from < to && !loaded) load(from, to);
-                loaded = false;
-                for (int s = from; s < to; s += KEEP) {
-                    i32x4 w[KEEP][TILES];
+            for (int t = 0; t < TILES; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t], xv, acc[t], 0, 0, 0);
+        };
+        if (k >= 16) {
+            if (from < to && !loaded) load(from);
+            loaded = false;
+            for (int s = from; s < to; s += KEEP) {
+                i32x4 w[KEEP][TILES];
 #pragma unroll
-                    for (int u = 0; u < KEEP; ++u)
+                for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-                        for (int t = 0; t < TILES; ++t) {
-                            w[u][t] = v[u][t];
-                            if constexpr (BYTES) {
-                                const int five[5] = {v[u][t][0], v[u][t][1], v[u][t][2], v[u][t][3], fifth[u][t]};
+                    for (int t = 0; t < TILES; ++t) w[u][t] = row[t].codes(v[u][t]);
+                if (s + KEEP < to) load(s + KEEP);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) w[u][t][i] = (int)__builtin_amdgcn_alignbyte((uint32_t)five[i + 1], (uint32_t)five[i], (uint32_t)off[t]);
-                            }
+                for (int u = 0; u < KEEP; ++u)
+                    if (s + u < to) {
+                        if (s + u >= whole) {
+#pragma unroll
+                            for (int t = 0; t < TILES; ++t) w[u][t] = row[t].in_place(w[u][t], (s + u) * kStep + 16 * quarter);
                         }
-                    if (s + KEEP < to) load(s + KEEP, to);       // the next ones while these are multiplied
-#pragma unroll
-                    for (int u = 0; u < KEEP; ++u)
-                        if (s + u < to) {
-                            if (s + u >= whole) {
-#pragma unroll
-                                for (int t = 0; t < TILES; ++t) w[u][t] = behind(w[u][t], max((s + u) * kStep + 16 * quarter - last[t], 0));
-                            }
-                            multiply(w[u], s + u);
-                        }
-                }
-            } else if (from < to) {
-                i32x4 w[TILES];
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) w[t] = load16(row[t] + off[t], 16 * quarter, k);
-                multiply(w, from);
+                        multiply(w[u], s + u);
+                    }
             }
+        } else if (from < to) {
+            i32x4 w[TILES];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) w[t] = row[t].short_row(16 * quarter, k);
+            multiply(w, from);
         }
-        if constexpr (SHARE) {                                   // lane l holds rows of b 4 (l / 16) + i, row l % 16 of a
-            __syncthreads();                                     // (everyone is through with the last job's sums)
+        if constexpr (SHARE) {
+            if (job) __syncthreads();                            // (everyone is through with the last job's sums)
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sums[((t * 4 + wave) * 16 + (lane & 15)) * 17 + 4 * quarter + i] = acc[t][i];
+            for (int i = 0; i < 4; ++i) sums[(wave * 16 + (lane & 15)) * 17 + 4 * quarter + i] = acc[0][i];
             __syncthreads();
             const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+            const int64_t n = tile0 * 16 + c;
+            if (n < G.n && r < m) {
+                int sum = 0;
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                const int64_t n = (tile0 + t) * 16 + c;
-                if (n < G.n && r < m) {
-                    int sum = 0;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) sum += sums[((t * 4 + w) * 16 + r) * 17 + c];
-                    store_out(G, r, n, scaled(sum, sx[r], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
-                }
+                for (int w = 0; w < 4; ++w) sum += sums[(w * 16 + r) * 17 + c];
+                store_out(G, r, n, scaled(sum, sx[r], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
             }
         } else {
 #pragma unroll
@@ -520,42 +609,57 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     }
 }
 
-static bool shares_depth(const GemmArgs &G) { return G.k > 11 * kStep || G.n <= 32768; }
+static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && k <= kFusedDepth && m * k <= kFusedValues; }
 
 template <typename X> static int few_rows(FewArgs F, hipStream_t st)
 {
     const int64_t steps = (F.g.k + kStep - 1) / kStep, tiles = (F.g.n + 15) / 16;
     F.shift = 0;
     while ((1 << F.shift) < F.g.m) ++F.shift;
-    const int64_t fits = kPanelBytes / (kStep << F.shift);
-    F.panel = (int)(steps < fits ? (steps ? steps : 1) : fits);
-    const bool share = std::is_same<X, int8_t>::value || shares_depth(F.g);
+    const bool share = steps >= 12 || tiles <= 2048;
     constexpr int kOwn = 4;
     const int64_t per = share ? 1 : 4 * kOwn, groups = (tiles + per - 1) / per;
     // a workgroup that lays the rows of a out once and walks several tiles with them: as many as keep 2 048 workgroups busy
-    F.jobs = F.panel >= steps ? (groups + 2047) / 2048 : 1;
+    F.jobs = (groups + 2047) / 2048;
     const int64_t blocks = (groups + F.jobs - 1) / F.jobs;
-    if (blocks >= ((int64_t)1 << 32) / kBlock) return IGCN_E_SHAPE;              // (2^32 threads of a launch)
-    const size_t lds = ((size_t)F.panel * kStep << F.shift) + (share ? 4 * 16 * 17 * 4 : 0);
-    const bool bytes = ((reinterpret_cast<uintptr_t>(F.g.b) | (uintptr_t)F.g.ldb) & 3) != 0;
+    const size_t lds = ((size_t)steps * kStep << F.shift) + (share ? 4 * 16 * 17 * 4 : 0);    // (kFusedValues, rounded up twice: well under 64 KiB)
+    const bool bytes = any_byte(F.g.b, F.g.ldb);
     auto launch = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), lds, st, F); };
     if (share) bytes ? launch(few_rows_i8_kernel<1, 4, true, true, X>) : launch(few_rows_i8_kernel<1, 4, true, false, X>);
-    else if constexpr (!std::is_same<X, int8_t>::value) bytes ? launch(few_rows_i8_kernel<kOwn, 1, false, true, X>) : launch(few_rows_i8_kernel<kOwn, 1, false, false, X>);
+    else bytes ? launch(few_rows_i8_kernel<kOwn, 1, false, true, X>) : launch(few_rows_i8_kernel<kOwn, 1, false, false, X>);
     return launch_status();
+}
+
+// Where rows stream and are not put together to tiles: 8 rows unless b has many short ones (8 rows, us, streamed and in tiles: 16384 x 512 5.3 and
+// 5.2, 28672 x 512 8.0 and 7.0, 65536 x 64 5.8 and 5.0, x 1024 14.7 and 16.3, 16384 x 8192 27 and 32), 16 and 32 where 64 x 64 tiles would not fill the card and
+// 256 workgroups here do (16 rows: 4096 x 4096 7.0 and 11.0, 8192 x 8192 15.0 and 18.1, 11008 x 8192 26.6 and 21.6; 32 rows: 4096 x 4096 9.1 and 11.2, 6144 x 4096
+// 14.2 and 11.3), 32 only with rows of a on words (1024 x 4095: 20.3 and 17.2).
+static bool streams(const GemmArgs &G)
+{
+    if (G.m <= 8) return G.k > 11 * kStep || G.n <= 24576;
+    if (G.m <= 16) return G.n <= 8192;
+    return G.m <= 32 && G.n <= 4096 && !any_byte(G.a, G.lda);
+}
+static int stream_few(const GemmArgs &G, hipStream_t st)
+{
+    if (G.m > 16) return stream<2, 1>(G, st);
+    // two tiles a workgroup halve the reads of a where there is a workgroup for every CU all the same (16 rows against 8192 x 8192: 15.0 us, one tile 17.2;
+    // 4096 x 8192 14.1 and 10.7; 1 row against 28672 x 8192 46 and 41)
+    return G.m > 4 && G.n > 4096 && G.k >= 2048 ? stream<1, 2>(G, st) : stream<1, 1>(G, st);
 }
 
 static int product(const GemmArgs &G, hipStream_t st)
 {
-    if ((G.m <= kFewRows && shares_depth(G)) || G.lda > kMostApart || G.ldb > kMostApart) {
+    if (streams(G)) return stream_few(G, st);
+    if (G.lda > kMostApart || G.ldb > kMostApart) {              // rows megabytes apart, in whatever number: 16 at a time
         const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
-        for (int64_t at = 0; at < G.m; at += kFewRows) {         // (rows megabytes apart, in whatever number: 8 at a time)
-            FewArgs F = {};
-            F.g = G;
-            F.g.a += at * G.lda;
-            F.g.sa += at;
-            F.g.y = static_cast<char *>(G.y) + at * G.ldy * size;
-            F.g.m = G.m - at < kFewRows ? G.m - at : kFewRows;
-            const int rc = few_rows<int8_t>(F, st);
+        for (int64_t at = 0; at < G.m; at += 16) {
+            GemmArgs Q = G;
+            Q.a += at * G.lda;
+            Q.sa += at;
+            Q.y = static_cast<char *>(G.y) + at * G.ldy * size;
+            Q.m = G.m - at < 16 ? G.m - at : 16;
+            const int rc = stream<1, 1>(Q, st);
             if (rc != IGCN_OK) return rc;
         }
         return IGCN_OK;
@@ -568,7 +672,10 @@ static int product(const GemmArgs &G, hipStream_t st)
     if (G.m > 64) {
         if (G.k <= kDepth && G.out == IGCN_DTYPE_F32) return tiles_launch<64, 128, 2, 4, 2>(G, st);
         if (G.k > kDepth && tiles(256, 256) >= 200) return tiles_launch<256, 256, 2, 4, 2>(G, st);
-        if (tiles(128, 128) >= 200) return tiles_launch<128, 128, 2, 2, 2>(G, st);
+        // eight waves, two to a SIMD, one reading LDS while the other multiplies (512 x 8192 x 512 6.9 us, four waves 8.1; x 4096 27 and 28); a third stage
+        // where a CU has one workgroup anyway and the depth pays for it (256 x 16384 x 8192 56 and 68, x 1024 10.4 and 10.3; 3000 x 3000 x 4096 69 and 58)
+        const int64_t middle = tiles(128, 128);
+        if (middle >= 200) return middle <= 256 && G.k >= 2048 ? tiles_launch<128, 128, 2, 4, 3>(G, st) : tiles_launch<128, 128, 2, 4, 2>(G, st);
     }
     return G.k >= 512 ? tiles_launch<64, 64, 2, 2, 4, true>(G, st) : tiles_launch<64, 64, 2, 2, 4>(G, st);
 }
@@ -585,7 +692,6 @@ static int check_product(const float *sa, const int8_t *b, int64_t ldb, const fl
     return IGCN_OK;
 }
 
-static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && k <= kFusedDepth && m * k <= kFusedValues; }      // (8 rows of such steps are well under kPanelBytes)
 static int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 
 }  // namespace igcn
