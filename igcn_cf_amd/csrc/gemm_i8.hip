@@ -482,18 +482,18 @@ template <int MG, int TILES> static int stream(const GemmArgs &G, hipStream_t st
 // The same for a few short rows in floating point: every workgroup makes them 8-bit on the way, with the quantiser's own steps, and lays them
 // out in LDS in the order the lanes read them: [16 codes of depth][row][16 bytes], rows rounded up to a power of two (lanes past them read
 // another row's bytes; what they compute is not stored).  No launch, no buffer; worth it while that is less work than a launch (us this way
-// and in two launches: 1 x 1024 against 4000 rows 5.3 and 7.0, 4 x 1024 5.6 and 8.0, 8 x 1024 8.3 and 8.6, against 16384 13.1 and 11.2; 1 x 2048 8.7 and
-// 7.7, against 96421 47.0 and 42.0).  SHARE: as above, else every wave has TILES of its own, which starts fewer workgroups where b has many
-// short rows (8 rows, us: 50000 x 256 12.4 and 9.1, 96421 x 64 10.0 and 7.4, x 768 20.2 and 21.2; 16384 x 512 5.8 and 10.2).
+// and in two launches: 1 x 64 against 96421 rows 6.7 and 8.8, 1 x 512 16.8 and 20.2, 1 x 1024 against 16384 8.8 and 8.0, 4000 5.1 and 7.1, 96421 26.8 and 21.4; 8 x 512
+// against 4000 6.5 and 7.5, 8 x 1024 8.7 and 7.4; and from the host a launch less).  SHARE: as above, else every wave has TILES of its own, which
+// starts fewer workgroups where b has many short rows (8 rows, us: 50000 x 256 12.4 and 9.1, 96421 x 64 10.0 and 7.4, x 768 20.2 and 21.2; 16384 x 512 5.8 and 10.2).
 constexpr int kFewRows = 8;
-constexpr int64_t kFusedValues = 4096, kFusedDepth = 1024;
+constexpr int64_t kFusedValues = 4096, kFusedDepth = 512, kFusedShort = 16384;
 
 struct FewArgs {
     GemmArgs g;
     const void *x;                                               // the rows of a in floating point, ldx apart
     int64_t ldx;
     int shift;                                                   // 2^shift rows of a in LDS
-    int64_t jobs;                                                // of a workgroup at most: tile groups it walks
+    int64_t jobs;                                                // of a workgroup at most: tile groups it walks (SHARE: one)
 };
 
 template <int TILES, int KEEP, bool SHARE, bool BYTES, typename X>
@@ -584,7 +584,6 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
             multiply(w, from);
         }
         if constexpr (SHARE) {
-            if (job) __syncthreads();                            // (everyone is through with the last job's sums)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sums[(wave * 16 + (lane & 15)) * 17 + 4 * quarter + i] = acc[0][i];
             __syncthreads();
@@ -609,17 +608,20 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     }
 }
 
-static bool quantises_on_the_way(int64_t m, int64_t k) { return m <= kFewRows && k <= kFusedDepth && m * k <= kFusedValues; }
+static bool quantises_on_the_way(int64_t m, int64_t n, int64_t k)
+{
+    return m <= kFewRows && m * k <= kFusedValues && k <= (n <= kFusedShort ? 2 * kFusedDepth : kFusedDepth);
+}
 
 template <typename X> static int few_rows(FewArgs F, hipStream_t st)
 {
     const int64_t steps = (F.g.k + kStep - 1) / kStep, tiles = (F.g.n + 15) / 16;
     F.shift = 0;
     while ((1 << F.shift) < F.g.m) ++F.shift;
-    const bool share = steps >= 12 || tiles <= 2048;
+    const bool share = tiles <= 2048;                            // (more have at most 8 steps: quantises_on_the_way)
     constexpr int kOwn = 4;
     const int64_t per = share ? 1 : 4 * kOwn, groups = (tiles + per - 1) / per;
-    // a workgroup that lays the rows of a out once and walks several tiles with them: as many as keep 2 048 workgroups busy
+    // a workgroup that lays the rows of a out once and walks several groups with them: as many as keep 2 048 workgroups busy
     F.jobs = (groups + 2047) / 2048;
     const int64_t blocks = (groups + F.jobs - 1) / F.jobs;
     const size_t lds = ((size_t)steps * kStep << F.shift) + (share ? 4 * 16 * 17 * 4 : 0);    // (kFusedValues, rounded up twice: well under 64 KiB)
@@ -713,7 +715,7 @@ extern "C" int igcn_matmul_i8(const int8_t *a, int64_t lda, const float *sa, con
 extern "C" int64_t igcn_linear_i8_workspace_bytes(int64_t m, int64_t k)
 {
     if (m < 0 || k < 0 || k > IGCN_MAX_I8_DEPTH || m > 0x7fffffff) return -1;
-    return quantises_on_the_way(m, k) ? 0 : up16(m * up16(k)) + 4 * m;
+    return quantises_on_the_way(m, INT64_MAX, k) ? 0 : up16(m * up16(k)) + 4 * m;
 }
 
 extern "C" int igcn_linear_i8(const void *x, int32_t x_dtype, int64_t ldx, const int8_t *b, int64_t ldb, const float *sb, const float *bias,
@@ -728,7 +730,7 @@ extern "C" int igcn_linear_i8(const void *x, int32_t x_dtype, int64_t ldx, const
     if (misaligned(x, x_dtype)) return IGCN_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
     GemmArgs G = {nullptr, b, nullptr, sb, bias, y, 0, ldb, ldy, m, n, k, dtype};
-    if (quantises_on_the_way(m, k)) {
+    if (quantises_on_the_way(m, n, k)) {
         FewArgs F = {};
         F.g = G;
         F.x = x;

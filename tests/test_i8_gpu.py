@@ -114,7 +114,8 @@ def check(a, sa, b, sb, bias=None, dtype=torch.float32):
 SIZES = [(1, 1, 1), (1, 17, 64), (2, 33, 16), (3, 5, 48), (4, 100, 8), (5, 1000, 64), (8, 64, 1024), (13, 77, 129), (16, 129, 100), (17, 300, 64), (31, 31, 31),
          (32, 200, 4096), (33, 65, 63), (48, 96, 256), (63, 1025, 64), (64, 64, 64), (65, 129, 100), (100, 4097, 128), (127, 127, 255), (128, 256, 512), (129, 257, 65),
          (255, 255, 1000), (256, 512, 192), (257, 300, 515), (300, 700, 2048), (512, 512, 4096), (513, 1029, 333), (1, 5000, 8191), (7, 3001, 5000), (1000, 1, 777),
-         (0, 5, 3), (5, 0, 3), (6, 7, 0)]
+         (7, 5001, 2100), (16, 8000, 2049), (12, 4100, 4096), (3, 30000, 333), (2, 25000, 64), (30, 4096, 2000), (22, 1000, 130), (1800, 2050, 2064), (1800, 2050, 2051),
+         (2100, 2100, 160), (2100, 2100, 71), (0, 5, 3), (5, 0, 3), (6, 7, 0)]
 
 
 @pytest.mark.parametrize('m,n,k', SIZES)
@@ -169,7 +170,8 @@ def test_offsets_past_32_bits(m):
 
 
 @pytest.mark.parametrize('m,n,k,dtype', [(1, 1000, 64, torch.float32), (1, 700, 4096, torch.bfloat16), (4, 333, 8192, torch.float16), (16, 500, 100, torch.float32),
-                                         (20, 500, 1000, torch.bfloat16), (300, 400, 64, torch.float32), (2, 99, 131071, torch.float32), (3, 50, 7, torch.bfloat16)])
+                                         (20, 500, 1000, torch.bfloat16), (300, 400, 64, torch.float32), (2, 99, 131071, torch.float32), (3, 50, 7, torch.bfloat16), (2, 600001, 40, torch.float32),
+                                         (8, 40000, 500, torch.bfloat16), (4, 16384, 1000, torch.float16), (4, 16385, 1000, torch.float16), (1, 33000, 15, torch.float32)])
 def test_a_linear_is_its_two_parts_and_takes_the_inputs_type(m, n, k, dtype):
     from igcn_cf_amd import ops
     g = _rng(k)
