@@ -44,6 +44,16 @@ __device__ __forceinline__ i32x4 behind(i32x4 v, int by)
     const uint64_t a = by >= 16 ? 0 : by >= 8 ? hi : lo, b = by >= 8 ? 0 : hi, c = a >> bits | (b << 1) << (63 - bits), d = b >> bits;
     return i32x4{(int)c, (int)(c >> 32), (int)d, (int)(d >> 32)};
 }
+// 16 codes of which the first `keep` stay (0 and less: none)
+__device__ __forceinline__ i32x4 first(i32x4 v, int keep)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = min(max(keep - 4 * i, 0), 4);
+        v[i] &= (int)(((uint64_t)1 << 8 * n) - 1);
+    }
+    return v;
+}
 __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ p) { return *reinterpret_cast<const i32x4_any *>(p); }
 // 16 codes of a row of n from k on, zeros behind its end: the last 16 of the row hold what is there of them
 __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int k, int n)
@@ -327,24 +337,23 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
 }
 
 // ---- a few rows of a ------------------------------------------------------------------------------------------------------------------
-// Bound by the bytes of b, each used once: no tile is worth staging.  A wave takes 16 rows of b as the matrix instruction's first operand straight
+// Bound by the bytes of b, each used once, or by the way through the depth where neither side has many: no tile is worth staging.  A wave takes 16 rows of b as the matrix instruction's first operand straight
 // from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and up to 16 rows of a, which stay in L2, as the
 // second.  KEEP steps' loads are under way while the ones before are multiplied.
 constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
 
-// A lane's row of b.  BYTES: rows at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it
+// A lane's row of either side.  BYTES: rows at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it
 // (1 row against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first
 // and the last row of b, whose words may reach over its ends, are loaded as they are.  What is behind a row's end meets zeros of a.
-template <bool BYTES> struct RowOfB {
+template <bool BYTES> struct Row {
     const int8_t *p;
     int off, last, more;                                         // of the row behind a multiple of 4; the last piece's place; to the fifth word
     struct Piece { i32x4 v; int fifth; };
-    __device__ __forceinline__ void at_row(const GemmArgs &G, int64_t r)
+    __device__ __forceinline__ void at_row(const int8_t *side, int64_t ld, int64_t r, int64_t rows, int k)      // (rows past the end: the last one)
     {
-        r = min(r, G.n - 1);
-        const int k = (int)G.k;
-        const bool inner = BYTES && r > 0 && r < G.n - 1;
-        p = G.b + r * G.ldb;
+        r = min(r, rows - 1);
+        const bool inner = BYTES && r > 0 && r < rows - 1;
+        p = side + r * ld;
         off = inner ? (int)(reinterpret_cast<uintptr_t>(p) & 3) : 0;
         last = inner ? (k + 3) / 4 * 4 - 16 : k - 16;
         more = inner ? 16 : 0;
@@ -372,7 +381,7 @@ template <bool BYTES> struct RowOfB {
     __device__ __forceinline__ i32x4 short_row(int at, int k) const { return load16(p + off, at, k); }             // a row of fewer than 16
 };
 
-// 16 MG rows of a at most, TILES x 16 rows of b a workgroup.  Its four waves take a quarter of the depth each and add their sums up in LDS (whole
+// 16 MG rows of a, TILES x 16 rows of b a workgroup.  Its four waves take a quarter of the depth each and add their sums up in LDS (whole
 // numbers: in any order), which fills the card where b has few rows and a wave's loads where they are long.  Rows of a come from L2 like
 // those of b from memory, no barrier until the end: laid out in LDS first, 8 rows against 4096 x 8192 took 17.4 us, this way 9.5.
 template <int MG, int TILES, bool BYTES>
@@ -380,17 +389,17 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
 {
     constexpr int KEEP = 4;
     __shared__ int sums[MG * TILES * 4 * 16 * 17];               // [group of a, tile, wave][row of a][17]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at_lane = 16 * (lane >> 4), m = (int)G.m, k = (int)G.k;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at_lane = 16 * (lane >> 4), k = (int)G.k;
     const int steps = (k + kStep - 1) / kStep, whole = k / kStep, from = steps * wave / 4, to = steps * (wave + 1) / 4;
-    const int64_t tile0 = (int64_t)blockIdx.x * TILES;
-    RowOfB<BYTES> row[TILES];
-    const int8_t *row_a[MG];
+    const int64_t tile0 = (int64_t)blockIdx.x * TILES, row0 = (int64_t)blockIdx.y * 16 * MG;
+    Row<BYTES> row[TILES];
+    Row<BYTES> row_a[MG];
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) row[t].at_row(G, (tile0 + t) * 16 + (lane & 15));
+    for (int t = 0; t < TILES; ++t) row[t].at_row(G.b, G.ldb, (tile0 + t) * 16 + (lane & 15), G.n, k);
 #pragma unroll
-    for (int g = 0; g < MG; ++g) row_a[g] = G.a + min(16 * g + (lane & 15), m - 1) * G.lda;      // (rows past the end: not stored)
-    typename RowOfB<BYTES>::Piece v[KEEP][TILES];
-    i32x4 x[KEEP][MG], acc[MG][TILES];
+    for (int g = 0; g < MG; ++g) row_a[g].at_row(G.a, G.lda, row0 + 16 * g + (lane & 15), G.m, k);
+    typename Row<BYTES>::Piece v[KEEP][TILES], x[KEEP][MG];
+    i32x4 acc[MG][TILES];
 #pragma unroll
     for (int g = 0; g < MG; ++g)
 #pragma unroll
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
 #pragma unroll
             for (int t = 0; t < TILES; ++t) v[u][t] = row[t].load(at);
 #pragma unroll
-            for (int g = 0; g < MG; ++g) x[u][g] = load16(row_a[g] + min(at, k - 16));
+            for (int g = 0; g < MG; ++g) x[u][g] = row_a[g].load(at);
         }
     };
     auto multiply = [&](const i32x4 (&w)[TILES], const i32x4 (&y)[MG]) {
@@ -420,7 +429,7 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) w[u][t] = row[t].codes(v[u][t]);
 #pragma unroll
-                for (int g = 0; g < MG; ++g) y[u][g] = x[u][g];
+                for (int g = 0; g < MG; ++g) y[u][g] = row_a[g].codes(x[u][g]);
             }
             if (s + KEEP < to) load(s + KEEP);                   // the next ones while these are multiplied
 #pragma unroll
@@ -431,7 +440,7 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
 #pragma unroll
                         for (int t = 0; t < TILES; ++t) w[u][t] = row[t].in_place(w[u][t], at);
 #pragma unroll
-                        for (int g = 0; g < MG; ++g) y[u][g] = behind(y[u][g], max(at - (k - 16), 0));
+                        for (int g = 0; g < MG; ++g) y[u][g] = first(row_a[g].in_place(y[u][g], at), k - at);
                     }
                     multiply(w[u], y[u]);
                 }
@@ -441,7 +450,7 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
 #pragma unroll
         for (int t = 0; t < TILES; ++t) w[t] = row[t].short_row(at_lane, k);
 #pragma unroll
-        for (int g = 0; g < MG; ++g) y[g] = load16(row_a[g], at_lane, k);
+        for (int g = 0; g < MG; ++g) y[g] = row_a[g].short_row(at_lane, k);
         multiply(w, y);
     }
     const int mine = lane & 15, quarter = lane >> 4;             // lane l holds rows of b 4 (l / 16) + i, row l % 16 of a
@@ -458,11 +467,12 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int64_t n = (tile0 + t) * 16 + c;
-            if (n < G.n && 16 * g + r < m) {
+            const int64_t at = row0 + 16 * g + r;
+            if (n < G.n && at < G.m) {
                 int sum = 0;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) sum += sums[(((g * TILES + t) * 4 + w) * 16 + r) * 17 + c];
-                store_out(G, 16 * g + r, n, scaled(sum, G.sa[16 * g + r], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
+                store_out(G, at, n, scaled(sum, G.sa[at], G.sb[n], G.bias != nullptr, G.bias ? G.bias[n] : 0.f));
             }
         }
 }
@@ -472,10 +482,10 @@ static bool fits_launch(int64_t blocks) { return blocks < ((int64_t)1 << 32) / k
 
 template <int MG, int TILES> static int stream(const GemmArgs &G, hipStream_t st)
 {
-    const int64_t blocks = (G.n + 16 * TILES - 1) / (16 * TILES);
-    if (!fits_launch(blocks)) return IGCN_E_SHAPE;
-    auto launch = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, G); };
-    any_byte(G.b, G.ldb) ? launch(stream_i8_kernel<MG, TILES, true>) : launch(stream_i8_kernel<MG, TILES, false>);
+    const int64_t blocks = (G.n + 16 * TILES - 1) / (16 * TILES), groups = (G.m + 16 * MG - 1) / (16 * MG);
+    if (!fits_launch(blocks) || groups > 65535) return IGCN_E_SHAPE;
+    auto launch = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)groups), dim3(kBlock), 0, st, G); };
+    any_byte(G.a, G.lda) || any_byte(G.b, G.ldb) ? launch(stream_i8_kernel<MG, TILES, true>) : launch(stream_i8_kernel<MG, TILES, false>);
     return launch_status();
 }
 
@@ -509,12 +519,12 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     const int64_t tiles = (G.n + 15) / 16, group0 = (int64_t)blockIdx.x * F.jobs * (SHARE ? 1 : 4) + (SHARE ? 0 : wave);
     static_assert(!SHARE || TILES == 1, "one tile's sums");
 
-    RowOfB<BYTES> row[TILES];
-    typename RowOfB<BYTES>::Piece v[KEEP][TILES];
+    Row<BYTES> row[TILES];
+    typename Row<BYTES>::Piece v[KEEP][TILES];
     i32x4 acc[TILES];
     auto rows_of = [&](int64_t tile0) {
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) row[t].at_row(G, (tile0 + t) * 16 + (lane & 15));
+        for (int t = 0; t < TILES; ++t) row[t].at_row(G.b, G.ldb, (tile0 + t) * 16 + (lane & 15), G.n, k);
     };
     auto load = [&](int s) {
 #pragma unroll
@@ -632,19 +642,21 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     return launch_status();
 }
 
-// Where rows stream and are not put together to tiles: 8 rows unless b has many short ones (8 rows, us, streamed and in tiles: 16384 x 512 5.3 and
-// 5.2, 28672 x 512 8.0 and 7.0, 65536 x 64 5.8 and 5.0, x 1024 14.7 and 16.3, 16384 x 8192 27 and 32), 16 and 32 where 64 x 64 tiles would not fill the card and
-// 256 workgroups here do (16 rows: 4096 x 4096 7.0 and 11.0, 8192 x 8192 15.0 and 18.1, 11008 x 8192 26.6 and 21.6; 32 rows: 4096 x 4096 9.1 and 11.2, 6144 x 4096
-// 14.2 and 11.3), 32 only with rows of a on words (1024 x 4095: 20.3 and 17.2).
+// Where rows stream and are not put together to tiles (us, streamed and in tiles): 8 rows unless b has many short ones (16384 x 512 5.3 and 5.2,
+// 28672 x 512 8.0 and 7.0, 65536 x 64 5.8 and 5.0, x 1024 14.7 and 16.3, 16384 x 8192 27 and 32); more where 256 workgroups do, one for each CU, which 64 x 64 tiles
+// would not fill (16 rows: 4096 x 4096 7.0 and 11.0, 8192 x 8192 15.0 and 18.1, 11008 x 8192 26.6 and 21.6; 32: 4096 x 4096 9.1 and 11.2, 8192 x 4096 14.2 and 11.5; 256 x
+// 512 x 8192 13.5 and 18.3, 512 x 512 x 8192 24.3 and 17.7, 189 x 48 x 5391 9.1 and 20.9).
+static int64_t up(int64_t n, int64_t by) { return (n + by - 1) / by; }
 static bool streams(const GemmArgs &G)
 {
     if (G.m <= 8) return G.k > 11 * kStep || G.n <= 24576;
     if (G.m <= 16) return G.n <= 8192;
-    return G.m <= 32 && G.n <= 4096 && !any_byte(G.a, G.lda);
+    return up(G.m, 32) * up(G.n, 16) <= 256;
 }
 static int stream_few(const GemmArgs &G, hipStream_t st)
 {
-    if (G.m > 16) return stream<2, 1>(G, st);
+    // 32 rows of a a workgroup where 16 would need more than one a CU (64 x 2048 x 4096 8.3 us, 16 rows 10.0; 33 x 1000 x 8192 13.7 and 10.4)
+    if (G.m > 16) return up(G.m, 16) * up(G.n, 16) <= 256 ? stream<1, 1>(G, st) : stream<2, 1>(G, st);
     // two tiles a workgroup halve the reads of a where there is a workgroup for every CU all the same (16 rows against 8192 x 8192: 15.0 us, one tile 17.2;
     // 4096 x 8192 14.1 and 10.7; 1 row against 28672 x 8192 46 and 41)
     return G.m > 4 && G.n > 4096 && G.k >= 2048 ? stream<1, 2>(G, st) : stream<1, 1>(G, st);
@@ -653,15 +665,16 @@ static int stream_few(const GemmArgs &G, hipStream_t st)
 static int product(const GemmArgs &G, hipStream_t st)
 {
     if (streams(G)) return stream_few(G, st);
-    if (G.lda > kMostApart || G.ldb > kMostApart) {              // rows megabytes apart, in whatever number: 16 at a time
+    if (G.lda > kMostApart || G.ldb > kMostApart) {              // rows megabytes apart, in whatever number
+        constexpr int64_t kMost = 65535 * 32;                    // of a in a launch
         const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
-        for (int64_t at = 0; at < G.m; at += 16) {
+        for (int64_t at = 0; at < G.m; at += kMost) {
             GemmArgs Q = G;
             Q.a += at * G.lda;
             Q.sa += at;
             Q.y = static_cast<char *>(G.y) + at * G.ldy * size;
-            Q.m = G.m - at < 16 ? G.m - at : 16;
-            const int rc = stream<1, 1>(Q, st);
+            Q.m = G.m - at < kMost ? G.m - at : kMost;
+            const int rc = stream<2, 1>(Q, st);
             if (rc != IGCN_OK) return rc;
         }
         return IGCN_OK;

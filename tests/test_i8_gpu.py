@@ -115,7 +115,7 @@ SIZES = [(1, 1, 1), (1, 17, 64), (2, 33, 16), (3, 5, 48), (4, 100, 8), (5, 1000,
          (32, 200, 4096), (33, 65, 63), (48, 96, 256), (63, 1025, 64), (64, 64, 64), (65, 129, 100), (100, 4097, 128), (127, 127, 255), (128, 256, 512), (129, 257, 65),
          (255, 255, 1000), (256, 512, 192), (257, 300, 515), (300, 700, 2048), (512, 512, 4096), (513, 1029, 333), (1, 5000, 8191), (7, 3001, 5000), (1000, 1, 777),
          (7, 5001, 2100), (16, 8000, 2049), (12, 4100, 4096), (3, 30000, 333), (2, 25000, 64), (30, 4096, 2000), (22, 1000, 130), (1800, 2050, 2064), (1800, 2050, 2051),
-         (2100, 2100, 160), (2100, 2100, 71), (0, 5, 3), (5, 0, 3), (6, 7, 0)]
+         (189, 48, 5391), (97, 66, 4678), (250, 500, 1999), (64, 2048, 77), (5000, 17, 40), (2100, 2100, 160), (2100, 2100, 71), (0, 5, 3), (5, 0, 3), (6, 7, 0)]
 
 
 @pytest.mark.parametrize('m,n,k', SIZES)
