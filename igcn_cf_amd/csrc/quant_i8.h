@@ -84,7 +84,8 @@ struct RowScale {
 
 // The codes of a piece, packed.  x inv + 1.5 2^23 in one operation leaves the nearest whole number in the low bits; off by at most
 // 127 2^-23 before that rounding, it is the right one unless what was cut off is within 2^-15 of a half: a wave that meets such a
-// value (one in 16 000) takes the exact way for the piece.  5 instructions a value instead of 16: at 16 they took as long as the bytes.
+// value takes the exact way for its place in the piece (one value in 16 000; in bfloat16, where half of the largest is a likely value, most
+// pieces: 50000 x 64 7.5 us when the whole piece went that way, 6.7 so).  5 instructions a value instead of 16: at 16 they took as long as the bytes.
 template <typename T> __device__ __forceinline__ void pack_codes(uint32_t (&w)[Chunk<T>::kValues / 4], const Chunk<T> &c, const RowScale &s)
 {
     constexpr int E = Chunk<T>::kValues;
@@ -104,9 +105,13 @@ template <typename T> __device__ __forceinline__ void pack_codes(uint32_t (&w)[C
     }
     if (__any((near >= kNear || s.s < 0x1p-120f) && s.inv > 0.f)) {
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) w[i] = 0u;
-#pragma unroll
-        for (int i = 0; i < E; ++i) w[i >> 2] |= (uint32_t)(s.code(c.value(i)) & 0xff) << (8 * (i & 3));
+        for (int i = 0; i < E; ++i) {
+            const float x = c.value(i), m = fmaf(x, s.inv, kMagic);
+            if (__any((fabsf(fmaf(x, s.inv, kMagic - m)) >= kNear || s.s < 0x1p-120f) && s.inv > 0.f)) {
+                const int shift = 8 * (i & 3);
+                w[i >> 2] = (w[i >> 2] & ~(0xffu << shift)) | (uint32_t)(s.code(x) & 0xff) << shift;
+            }
+        }
     }
 }
 
