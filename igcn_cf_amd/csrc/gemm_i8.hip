@@ -4,8 +4,8 @@
 //
 // The sum is exact (int32: K <= 131 071); the scales are applied once, in float32, before the one rounding to the output's type.
 //
-// Measured: 8192 x 8192 x 4096 to bfloat16 264 us = 2.1 POP/s (a library's bare int8 product: 306 us), 512 x 96421 x 64 to float32 48-56 us = 4.2 TB/s
-// of y (the same stores alone 45), 4 x 16384 x 8192 31 us = 4.4 TB/s of b, 1 x 96421 x 64 from float32 7.5 us.
+// Measured: 8192 x 8192 x 4096 to bfloat16 264 us = 2.1 POP/s (a library's bare int8 product: 306 us), 512 x 96421 x 64 to float32 45-54 us = 3.7-4.4
+// TB/s of y (the same stores alone 45), 4 x 16384 x 8192 28 us = 4.8 TB/s of b, 16 x 4096 x 4096 7 us, 1 x 96421 x 64 from float32 7.1 us.
 #include "quant_i8.h"
 #include <type_traits>
 
