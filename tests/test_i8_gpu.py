@@ -280,3 +280,15 @@ def test_refusals():
         with pytest.raises(Error):
             call()
             print('not refused:', i)
+
+
+def test_quantised_values_past_32_bits():
+    from igcn_cf_amd import ops
+    rows, k = 40000, 60000                                                               # 2.4e9 values, 4.8 GB
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEV)
+    x[-40:] = torch.randn(40, k, device=DEV, generator=_rng(8)).to(torch.bfloat16)
+    q, s = ops.quantize_rows_i8(x)
+    want_q, want_s = _quantized(x[-40:])
+    assert torch.equal(q[-40:], want_q) and torch.equal(s[-40:], want_s) and not bool(s[:-40].any()) and not bool(q[-80:-40].any())
+    y = ops.dequantize_rows_i8(q, s, dtype=torch.float16)
+    assert torch.equal(y[-40:], (want_q.float() * want_s[:, None]).half()) and not bool(y[-80:-40].any())

@@ -506,3 +506,31 @@ def test_refusals_leave_everything_as_it_was():
     for gs in ([torch.ones(3)], [torch.ones(3, device=DEV).double()], [torch.ones(1, device=DEV).expand(3)], [None], [torch.ones(4, 4, device=DEV)[:, 1]]):
         with pytest.raises(_lib.IgcnError):
             ops.grad_norm(gs)
+
+
+@pytest.mark.parametrize('eight', [False, True])
+def test_elements_past_32_bits(eight):
+    """More than 2^31 elements (2^32 with 8-bit moments): the last ones are stepped like a tensor of their own, the ones before are not touched twice."""
+    from igcn_cf_amd import ops
+    n, tail = (2 ** 32 if eight else 2 ** 31) + 1000, 1000
+    p, g = torch.ones(n, dtype=torch.bfloat16, device=DEV), torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    g[-tail:] = torch.randn(tail, device=DEV, generator=torch.Generator(DEV).manual_seed(3)).to(torch.bfloat16)
+    g[:tail] = g[-tail:]
+    if eight:
+        m, v, scales = _zeros8(p)
+    else:
+        m, v, scales = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), None
+    step = torch.zeros((), device=DEV)
+    norm = ops.adamw_step([p], [g], [m], [v], [step], lr=0.25, weight_decay=0., eps=0.5, max_grad_norm=1e6, scales=[scales] if eight else None)
+    assert abs(float(norm) - float(g[-tail:].double().norm()) * 2 ** 0.5) <= 1e-6 * float(norm)
+    x = g[-tail:].double()
+    want = 1 - 0.25 * x / (x.abs() + 0.5)                                            # the first step: m / c1 = g, v / c2 = g^2 (its float32 roundings: well under 1e-5)
+    for part in (slice(0, tail), slice(n - tail, n)):
+        assert bool(((p[part].double() - want).abs() <= HALF_STEP[torch.bfloat16] * want.abs() + 1e-5).all())
+    assert bool((p[tail:2 * tail] == 1).all()) and bool((p[-2 * tail:-tail] == 1).all())
+    if eight:
+        block = torch.arange(n - tail, n, device=DEV) // 128                         # code steps: an eighth of the value, 2^-9 of the scale at least
+        s = scales[block, 0].double()
+        assert bool(((m[-tail:].float().double() * s - 0.1 * x).abs() <= 0.13 * (0.1 * x).abs() + s * 2.0 ** -9 * 1.01).all())
+    else:
+        assert bool(((m[-tail:].double() - 0.1 * x).abs() <= 1e-6 * x.abs()).all())
