@@ -221,12 +221,15 @@ __device__ __forceinline__ void step32(const igcn_adamw_tensor &t, int64_t i, co
     load8(static_cast<const float *>(t.exp_avg), i, t.n, ok, m);
     load8(static_cast<const float *>(t.exp_avg_sq), i, t.n, ok, v);
     load8(static_cast<const P *>(t.param), i, t.n, ok, p);
-    const float factor = q.factor, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2);
+    // m + a (x - m) has no error from beta's own rounding, which a long average with beta near 1 would add up; but what it cuts off is a
+    // part of the old average's size, so a short one (beta under a half), which keeps little of that, is formed term by term.
+    const float factor = q.factor, b1 = (float)H.beta1, b2 = (float)H.beta2, a1 = (float)(1.0 - H.beta1), a2 = (float)(1.0 - H.beta2);
+    const bool long_m = H.beta1 >= 0.5, long_v = H.beta2 >= 0.5;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const float x = to_float(g[k]) * factor;
-        m[k] = fmaf(a1, x - m[k], m[k]);
-        v[k] = fmaf(a2, fmaf(x, x, -v[k]), v[k]);
+        m[k] = long_m ? fmaf(a1, x - m[k], m[k]) : fmaf(b1, m[k], a1 * x);
+        v[k] = long_v ? fmaf(a2, fmaf(x, x, -v[k]), v[k]) : fmaf(b2, v[k], a2 * x * x);
         p[k] = from_float<P>(stepped(to_float(p[k]), m[k], v[k], q, H.eps));
     }
     store8(static_cast<float *>(t.exp_avg), i, t.n, ok, m);

@@ -534,3 +534,41 @@ def test_elements_past_32_bits(eight):
         assert bool(((m[-tail:].float().double() * s - 0.1 * x).abs() <= 0.13 * (0.1 * x).abs() + s * 2.0 ** -9 * 1.01).all())
     else:
         assert bool(((m[-tail:].double() - 0.1 * x).abs() <= 1e-6 * x.abs()).all())
+
+
+@pytest.mark.parametrize('eight', [False, True])
+@pytest.mark.parametrize('betas', [(0., 0.999), (0.9, 0.), (0., 0.), (0.1, 0.2), (0.49, 0.51), (0.5, 0.5), (0.51, 0.49), (0.999, 0.3), (1e-6, 1e-6)])
+def test_every_beta_leaves_what_its_moment_keeps(betas, eight):
+    """Old averages far above or far below the new gradient, for betas over the whole range: an average keeps beta of itself and takes
+    1 - beta of the new value, each to a few roundings of its own size.  u = 2^-24 a rounding: beta, 1 - beta, two products and the sum round,
+    so m is within 4 u (b |m| + a |x|) and v within 5 u (b v + a x^2); the update adds sqrt, reciprocal (1 ulp = 2 u each), its
+    factors and products: 16 u of its size in all.  8-bit codes hold a moment to an eighth / a quarter, or a step of their block."""
+    from igcn_cf_amd import ops
+    u, n = 2.0 ** -24, 700
+    hyper = dict(HYPER, betas=betas)
+    for old_m, old_v, size in ((0., 1., 1e-4), (1., 1., 1e-4), (1., 1e-8, 1e3), (1e-3, 1e-12, 1e-3), (0., 0., 1.)):
+        rng = np.random.default_rng(3)
+        g = torch.from_numpy((size * rng.standard_normal(n)).astype(np.float32)).to(DEV)
+        p, t = _params((n,), rng), torch.full((), 4., device=DEV)
+        m, v = torch.full((n,), old_m, device=DEV), torch.full((n,), old_v, device=DEV)
+        if eight:
+            s = torch.tensor([[old_m / 448 or 1., old_v / 57344 or 1.]], device=DEV).repeat(-(-n // 128), 1)
+            m8 = torch.full((n,), 126 if old_m else 0, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+            v8 = torch.full((n,), 123 if old_v else 0, dtype=torch.uint8, device=DEV).view(torch.float8_e5m2)
+            m, v = m8.float() * s[:, 0].repeat_interleave(128)[:n], v8.float() * s[:, 1].repeat_interleave(128)[:n]
+        p0, m0, v0, x = _flat(p), _flat(m), _flat(v), _flat(g)
+        ops.adamw_step([p], [g], [m8 if eight else m], [v8 if eight else v], [t], scales=[s] if eight else None, **hyper)
+        (b1, b2), c1, c2 = betas, 1 - betas[0] ** 5, 1 - betas[1] ** 5
+        size_m, size_v = b1 * np.abs(m0) + (1 - b1) * np.abs(x), b2 * v0 + (1 - b2) * x * x
+        m1, v1 = b1 * m0 + (1 - b1) * x, size_v
+        if eight:
+            sm, sv = (s[:, j].double().repeat_interleave(128)[:n].cpu().numpy() for j in (0, 1))
+            assert (np.abs(_flat(m8.float()) * sm - m1) <= np.abs(m1) / 8 + sm * 2.0 ** -9 + 8 * u * size_m).all(), (old_m, size)
+            assert (np.abs(_flat(v8.float()) * sv - v1) <= v1 / 4 + sv * 2.0 ** -16 + 8 * u * size_v).all(), (old_v, size)
+        else:
+            assert (np.abs(_flat(m) - m1) <= 4 * u * size_m).all(), (old_m, size)
+            assert (np.abs(_flat(v) - v1) <= 5 * u * size_v).all(), (old_v, size)
+        denom = np.sqrt(v1 / c2) + hyper['eps']
+        step = hyper['lr'] / c1
+        want = p0 * (1 - hyper['lr'] * hyper['weight_decay']) - step * m1 / denom
+        assert (np.abs(_flat(p) - want) <= 4 * u * np.abs(p0) + 16 * u * step * size_m / denom).all(), (old_m, old_v, size)
