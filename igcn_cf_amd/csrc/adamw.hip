@@ -229,7 +229,8 @@ __device__ __forceinline__ void step32(const igcn_adamw_tensor &t, int64_t i, co
     for (int k = 0; k < kPer; ++k) {
         const float x = to_float(g[k]) * factor;
         m[k] = long_m ? fmaf(a1, x - m[k], m[k]) : fmaf(b1, m[k], a1 * x);
-        v[k] = long_v ? fmaf(a2, fmaf(x, x, -v[k]), v[k]) : fmaf(b2, v[k], a2 * x * x);
+        // (a x first: x^2 passes float32 where a x^2 does not; and an infinite v stays one)
+        v[k] = fmaf(a2 * x, x, long_v && v[k] < INFINITY ? fmaf(-a2, v[k], v[k]) : b2 * v[k]);
         p[k] = from_float<P>(stepped(to_float(p[k]), m[k], v[k], q, H.eps));
     }
     store8(static_cast<float *>(t.exp_avg), i, t.n, ok, m);

@@ -572,3 +572,28 @@ def test_every_beta_leaves_what_its_moment_keeps(betas, eight):
         step = hyper['lr'] / c1
         want = p0 * (1 - hyper['lr'] * hyper['weight_decay']) - step * m1 / denom
         assert (np.abs(_flat(p) - want) <= 4 * u * np.abs(p0) + 16 * u * step * size_m / denom).all(), (old_m, old_v, size)
+
+
+@pytest.mark.parametrize('eight', [False, True])
+def test_gradients_whose_squares_alone_pass_float32(eight):
+    """(1 - beta2) x^2 is a float32 number up to |x| = 5.8e20 at beta2 = 0.999, x^2 up to 1.8e19 only: what is held is the formula's."""
+    from igcn_cf_amd import ops
+    g = torch.tensor([1e19, -3e19, 1e20, -5e20], device=DEV)
+    for old in (0., 1e30):
+        p, t = torch.zeros(4, device=DEV), torch.zeros((), device=DEV)
+        m, v, s = torch.zeros(4, device=DEV), torch.full((4,), old, device=DEV), None
+        if eight:
+            m, v, s = _zeros8(p)
+        ops.adamw_step([p], [g], [m], [v], [t], scales=[s] if eight else None, **HYPER)
+        x = _flat(g)
+        v1 = 0.999 * (0. if eight else old) + 0.001 * x * x
+        if eight:
+            assert (np.abs(_flat(v.float()) * float(s[0, 1]) - v1) <= v1 / 4 + float(s[0, 1]) * 2.0 ** -16).all()
+        else:
+            assert (np.abs(_flat(v) - v1) <= 5 * 2.0 ** -24 * v1).all()
+        want = -HYPER['lr'] * x / np.sqrt(v1 / 0.001)
+        assert (np.abs(_flat(p) - want) <= 24 * 2.0 ** -24 * np.abs(want)).all()
+    if not eight:                                                                    # an infinite average stays one and moves nothing
+        p, m, v = torch.ones(4, device=DEV), torch.ones(4, device=DEV), torch.full((4,), float('inf'), device=DEV)
+        ops.adamw_step([p], [torch.ones(4, device=DEV)], [m], [v], [torch.zeros((), device=DEV)], lr=1e-3, weight_decay=0.)
+        assert bool(torch.isinf(v).all()) and bool((p == 1).all())
