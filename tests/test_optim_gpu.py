@@ -597,3 +597,49 @@ def test_gradients_whose_squares_alone_pass_float32(eight):
         p, m, v = torch.ones(4, device=DEV), torch.ones(4, device=DEV), torch.full((4,), float('inf'), device=DEV)
         ops.adamw_step([p], [torch.ones(4, device=DEV)], [m], [v], [torch.zeros((), device=DEV)], lr=1e-3, weight_decay=0.)
         assert bool(torch.isinf(v).all()) and bool((p == 1).all())
+
+
+def test_a_small_eps_and_second_moments_below_float32s_normal_numbers():
+    """eps is any number from 0 on, and v may be as small as float32 has them (2^-149): the update is step m / (sqrt(v / c2) + eps) of the
+    moments the step left, its roundings as ever (sqrt and reciprocal 1 ulp = 2 u each, four products, a constant each: 12 u), where neither
+    is lost below 2^-126 (4.6e-10 is where the kernels change over).  p starts at zero and nothing decays: what is there is the update."""
+    from igcn_cf_amd import ops
+    u = 2.0 ** -24
+    old = torch.tensor([2.0 ** e for e in (-149, -148, -145, -140, -133, -127, -126, -125, -110, -101, -100, -99, -90, -40, 0)] + [0.], device=DEV)
+    for eps in (0., 2.0 ** -149, 1e-42, 1e-40, 2.0 ** -127, 1.2e-38, 1e-35, 1e-30, 1e-20, 4.5e-10, 4.7e-10, 1e-8):
+        for near in (1., 2.0 ** -20):
+            p, g, t = torch.zeros(16, device=DEV), torch.zeros(16, device=DEV), torch.full((), 9., device=DEV)
+            m = (old.double().sqrt().clamp(min=max(float(np.float32(eps)), 2.0 ** -120)) * near).float()       # updates of ordinary size
+            v = old.clone()
+            ops.adamw_step([p], [g], [m], [v], [t], lr=1e-3, betas=(0.9, 0.999), eps=eps, weight_decay=0.)
+            m1, v1, eps32 = _flat(m), _flat(v), float(np.float32(eps))
+            with np.errstate(divide='ignore', invalid='ignore'):
+                want = -1e-3 / (1 - 0.9 ** 10) * m1 / (np.sqrt(v1 / (1 - 0.999 ** 10)) + eps32)
+            got = _flat(p)
+            wide = np.abs(want) > np.finfo(np.float32).max
+            assert (np.isinf(got) == (wide | np.isinf(want))).all(), (eps, near, got)
+            fine = np.isfinite(want) & ~wide
+            assert (np.abs(got[fine] - want[fine]) <= 12 * u * np.abs(want[fine]) + 2.0 ** -149).all(), (eps, near, got, want)
+    p, z = torch.zeros(3, device=DEV), [torch.zeros(3, device=DEV) for _ in range(3)]
+    ops.adamw_step([p], [z[0]], [z[1]], [z[2]], [torch.zeros((), device=DEV)], lr=1e-3, eps=1e-40)
+    assert not p.any()                                                              # 0 / eps
+
+
+@pytest.mark.parametrize('eight', [False, True])
+@pytest.mark.parametrize('n', [64, 20003])
+@pytest.mark.parametrize('eps', [0., 1e-42, 1e-30, 1e-8])
+def test_first_steps_from_gradients_whose_squares_are_hardly_there(n, eight, eps):
+    """A first step moves a parameter by lr g / (|g| + eps), whatever the size of g, in one launch and in two.  v = 0.001 g^2 may lie below 2^-126,
+    where float32 has steps of 2^-149: two such roundings of v, halved by the root, beside 16 u of the update (u = 2^-24)."""
+    from igcn_cf_amd import ops
+    u = 2.0 ** -24
+    g = torch.pow(2.0, -40 - 24 * torch.rand(n, device=DEV, generator=torch.Generator(DEV).manual_seed(n)))
+    g[::3] *= -1
+    for dtype in (torch.float32, torch.bfloat16):
+        p, gd, t = torch.zeros(n, device=DEV, dtype=dtype), g.to(dtype), torch.zeros((), device=DEV)
+        m, v, s = _zeros8(p) if eight else (torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), None)
+        ops.adamw_step([p], [gd], [m], [v], [t], scales=[s] if eight else None, lr=1e-3, betas=(0.9, 0.999), eps=eps)
+        x = _flat(gd)
+        want = -1e-3 * x / (np.abs(x) + float(np.float32(eps)))
+        off = (16 * u + 2.0 ** -149 / (0.001 * x * x)) * np.abs(want)
+        assert (np.abs(_flat(p) - want) <= off + HALF_STEP[dtype] * (np.abs(want) + off)).all(), (dtype, n, eps)
