@@ -441,6 +441,12 @@ def _compact_bpr_terms(rows_rep, rows_emb, batch):
     return ops.bpr_loss_terms(rr, rr, re, re, None, idx, idx, idx + batch, batch, batch)
 
 
+def _mark_shares(model, world):
+    """Parameters that are one rank's part of a larger one say so: a norm over this rank's alone is not the model's (optim.AdamW)."""
+    for p in model.parameters():
+        p.is_share = world > 1
+
+
 class ShardedLightGCN(torch.nn.Module):
     """LightGCN (model.py:75-123) with the embedding table, its gradient and the
     optimizer state row-sharded over the ranks.  One step:
@@ -472,6 +478,7 @@ class ShardedLightGCN(torch.nn.Module):
         self.emb_users = torch.nn.Parameter(eu.to(device))
         self.emb_items = torch.nn.Parameter(ei.to(device))
         self.loss_fn = loss_fn if loss_fn is not None else _compact_bpr_terms
+        _mark_shares(self, world)
 
     def get_rep_local(self):
         return _ShardedPropagateFn.apply(self.emb_users, self.emb_items, self.prop)
@@ -481,6 +488,12 @@ class ShardedLightGCN(torch.nn.Module):
         ids = torch.cat([users, self.n_users + pos_items, self.n_users + neg_items])
         rows_rep, rows_emb = _BatchRowsFn.apply(self.prop, ids, ru, ri, self.emb_users, self.emb_items)
         return self.loss_fn(rows_rep, rows_emb, users.numel())
+
+    def all_reduce(self, t):
+        """Sums t over the ranks, in place (what optim.AdamW's norm_reduce_fn has to do for the owned rows)."""
+        if self.prop.collectives.active():
+            self.prop.collectives.all_reduce(t)
+        return t
 
     def full_embedding(self):
         with torch.no_grad():
@@ -557,8 +570,10 @@ class ColumnShardedLightGCN(torch.nn.Module):
             from . import ops
             loss_fn = lambda rep, emb, u, p, i, nu, red: ops.bpr_loss_terms(rep, rep, emb, emb, None, u, p, i, nu, nu, red)
         self.propagate_fn, self.loss_fn = propagate_fn, loss_fn
+        _mark_shares(self, world)
 
-    def _allreduce(self, t):
+    def all_reduce(self, t):
+        """Sums t over the ranks, in place: the partial dots of a loss, and what optim.AdamW's norm_reduce_fn has to do."""
         if dist.is_available() and dist.is_initialized():
             dist.all_reduce(t, group=self.group)
         return t
@@ -567,7 +582,7 @@ class ColumnShardedLightGCN(torch.nn.Module):
         return self.propagate_fn(self.emb)
 
     def bpr_loss_terms(self, users, pos_items, neg_items):
-        return self.loss_fn(self.get_rep_local(), self.emb, users, pos_items, neg_items, self.n_users, self._allreduce)
+        return self.loss_fn(self.get_rep_local(), self.emb, users, pos_items, neg_items, self.n_users, self.all_reduce)
 
     def gather_columns(self, local):
         """[N, d/P] slices -> replicated [N, d] (once per evaluation)."""
@@ -613,4 +628,5 @@ def column_shard_model(model_config, dataset, rank, world, group=None, full_stat
                 dist.all_reduce(t, group=group)
             return t
     model.slice_reduce_fn = reduce_fn
+    _mark_shares(model, world)
     return model

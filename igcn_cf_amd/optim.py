@@ -11,10 +11,15 @@ class AdamW(torch.optim.Optimizer):
     state_dict it takes).  state_bits 8: exp_avg as float8_e4m3fn and exp_avg_sq as float8_e5m2 codes with two float32 scales a block
     of 128 elements ('scales') — 2.06 bytes a parameter instead of 8; a moment is codes.float() * its block's scale.
     max_grad_norm: clip by the norm over the gradients of ALL groups; the last step's norm is `grad_norm` (a tensor on the GPU).
+    norm_reduce_fn: for parameters that are a rank's share of a model (dist.ShardedLightGCN, ColumnShardedLightGCN: their all_reduce;
+    dist.column_shard_model: slice_reduce_fn, which the trainers pass): sums a tensor over the ranks, in place, so that every rank clips by
+    the norm over all shares (parameters that dist marks as shares are refused without).  Called once a step on one float64 number, also
+    where this rank has no gradient.
     seed: of the 8-bit moments' stochastic rounding.  The step count lives on the device and lr may be a one-element float32 tensor
     there: the step can sit in a HIP graph."""
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, seed=0):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, seed=0,
+                 norm_reduce_fn=None):
         if not isinstance(lr, torch.Tensor) and not lr >= 0.:
             raise ValueError('lr must not be negative')
         if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1.) or not eps >= 0. or not weight_decay >= 0.:
@@ -23,8 +28,15 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError('state_bits must be 8 or 32')
         if max_grad_norm is not None and not max_grad_norm > 0.:
             raise ValueError('max_grad_norm must be positive')
-        self.max_grad_norm, self.seed, self.grad_norm = max_grad_norm, int(seed), None
+        self.max_grad_norm, self.seed, self.grad_norm, self.norm_reduce_fn = max_grad_norm, int(seed), None, norm_reduce_fn
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        if self.max_grad_norm is not None and self.norm_reduce_fn is None and \
+                any(getattr(p, 'is_share', False) for p in self.param_groups[-1]['params']):
+            self.param_groups.pop()
+            raise ValueError('parameters that are a rank\'s share of a model are clipped by the norm over all ranks: norm_reduce_fn is missing')
 
     def _state_of(self, p, bits):
         state = self.state[p]
@@ -35,6 +47,15 @@ class AdamW(torch.optim.Optimizer):
             if bits == 8:
                 state['scales'] = torch.zeros(((p.numel() + ops.ADAMW_BLOCK - 1) // ops.ADAMW_BLOCK, 2), dtype=torch.float32, device=p.device)
         return state
+
+    def _common_norm(self, grads):
+        """The norm over the gradients of all groups, and of all ranks where they hold shares."""
+        norm = ops.grad_norm(grads) if grads else torch.zeros((), device=self.param_groups[0]['params'][0].device)
+        if self.norm_reduce_fn is not None:
+            square = norm.double().square()
+            self.norm_reduce_fn(square)
+            norm = square.sqrt().float()
+        return norm
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -52,8 +73,8 @@ class AdamW(torch.optim.Optimizer):
             if ps:
                 calls.append((gi, group, ps, gs))
         norm = None
-        if self.max_grad_norm is not None and len(calls) > 1:              # one norm over all groups
-            norm = ops.grad_norm([g for call in calls for g in call[3]])
+        if self.max_grad_norm is not None and (len(calls) > 1 or self.norm_reduce_fn is not None):
+            norm = self.grad_norm = self._common_norm([g for call in calls for g in call[3]])
         for gi, group, ps, gs in calls:
             states = [self._state_of(p, group['state_bits']) for p in ps]
             got = ops.adamw_step(ps, gs, [s['exp_avg'] for s in states], [s['exp_avg_sq'] for s in states], [s['step'] for s in states],
@@ -64,7 +85,8 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def __getstate__(self):                # (copies and pickles keep what torch's form of it does not know)
-        return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm, 'seed': self.seed, 'grad_norm': self.grad_norm}
+        return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm, 'seed': self.seed, 'grad_norm': self.grad_norm,
+                'norm_reduce_fn': self.norm_reduce_fn}
 
     def load_state_dict(self, state_dict):
         """As torch's, but the state keeps its own types (torch's casts every floating state to its parameter's).  Takes the state of

@@ -180,7 +180,17 @@ class BasicTrainer:
                 kw['capturable'] = True    # the step count lives on the device, so the step can sit in a HIP graph
         elif opt is AdamW:                 # the HIP step: its own settings under its own names
             kw = {k: self.config[k] for k in ('betas', 'eps', 'weight_decay', 'state_bits', 'max_grad_norm', 'seed') if k in self.config}
+            kw['norm_reduce_fn'] = self._norm_reduce_fn()
         self.opt = opt(self.model.parameters(), lr=self.config['lr'], **kw)
+
+    def _norm_reduce_fn(self):
+        """Where the parameters are a rank's share of a model: what sums over its ranks; else None."""
+        return getattr(self.model, 'slice_reduce_fn', None) or getattr(self.model, 'all_reduce', None)
+
+    def _optimizer_step(self):
+        if isinstance(self.opt, AdamW):
+            self.opt.norm_reduce_fn = self._norm_reduce_fn() or self.opt.norm_reduce_fn      # (the model's may have been replaced)
+        self.opt.step()
 
     # ---- one optimisation step as ONE captured HIP graph (config key 'hip_graph', default True) -----------------
     def _graph_wanted(self):
@@ -289,7 +299,7 @@ class BasicTrainer:
                     loss = loss_fn(*self._static_inputs)
                     self.opt.zero_grad()
                     loss.backward()
-                    self.opt.step()
+                    self._optimizer_step()
                     del loss                  # no autograd graph of the warm-up (its AccumulateGrad nodes) outlives it
         finally:
             torch.cuda.current_stream().wait_stream(side)
@@ -300,7 +310,7 @@ class BasicTrainer:
             with torch.cuda.graph(graph):
                 loss = loss_fn(*self._static_inputs)
                 loss.backward(one)
-                self.opt.step()
+                self._optimizer_step()
                 self._static_loss = loss.detach()
         except BaseException:
             torch.cuda.synchronize()
@@ -584,7 +594,7 @@ class BPRTrainer(BasicTrainer):
     def _optimise_loss(self, loss):
         self.opt.zero_grad()
         loss.backward()
-        self.opt.step()
+        self._optimizer_step()
         return loss.detach()
 
     def node_step(self, nodes):
@@ -672,7 +682,7 @@ class IGCNTrainer(BasicTrainer):
         loss = self._igcn_loss(nodes, aux_inputs)
         self.opt.zero_grad()
         loss.backward()
-        self.opt.step()
+        self._optimizer_step()
         return loss.detach()
 
     def _igcn_loss(self, nodes, aux_inputs):
@@ -689,7 +699,7 @@ class IGCNTrainer(BasicTrainer):
         loss = main_loss + self.aux_reg * aux_loss
         self.opt.zero_grad()
         loss.backward()
-        self.opt.step()
+        self._optimizer_step()
         return loss.detach()
 
     def train_one_epoch(self):

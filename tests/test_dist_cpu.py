@@ -523,3 +523,44 @@ def test_eight_ranks_some_owning_nothing_under_late_collectives(exchange, n_laye
         np.testing.assert_allclose(full, ref, rtol=1e-5, atol=1e-7)
     assert empties > 0
     assert sum(r[3] for r in res) == 2 * len(ta)
+
+
+# ---- clipping by the norm over all ranks ---------------------------------------------------------------------------
+def _norm_worker(rank, world, port, path, ret):
+    os.environ.update(MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port))
+    dist.init_process_group('gloo', rank=rank, world_size=world)
+    try:
+        from igcn_cf_amd import optim
+        from igcn_cf_amd.dataset import ProcessedDataset
+        from igcn_cf_amd.dist import ColumnShardedLightGCN, ShardedLightGCN
+        optim.ops.grad_norm = lambda gs: torch.sqrt(sum(g.double().square().sum() for g in gs)).float()      # the kernel runs on GPUs only
+        ds = ProcessedDataset({'name': 'ProcessedDataset', 'path': path, 'device': 'cpu'})
+        norms = []
+        for model in (ColumnShardedLightGCN(ds, 8, 2, rank, world, 'cpu', propagate_fn=lambda e: e, loss_fn=lambda *a: None),
+                      ShardedLightGCN(ds, 8, 2, rank, world, 'cpu', spmm_fn=lambda *a, **k: None, csr_factory=TorchCsrStub)):
+            try:
+                optim.AdamW(model.parameters(), max_grad_norm=1.)                    # a rank's own norm is not the model's
+                norms.append((0., 0.))
+            except ValueError:
+                pass
+            optim.AdamW(model.parameters())
+            opt = optim.AdamW(model.parameters(), max_grad_norm=1., norm_reduce_fn=model.all_reduce)
+            grads = [torch.full_like(p, 10. ** rank) for p in model.parameters()]
+            norms.append((float(opt._common_norm(grads)), float(sum(g.double().square().sum() for g in grads))))
+            norms.append((float(opt._common_norm(grads if rank else [])), float(sum(g.double().square().sum() for g in grads)) if rank else 0.))
+        ret[rank] = norms
+    finally:
+        dist.destroy_process_group()
+
+
+def TorchCsrStub(rowptr, col, val, shape, blocks=None):
+    return None
+
+
+def test_sharded_parameters_are_clipped_by_the_norm_over_all_ranks(golden):
+    """Every rank gets the one norm over all shares — row- and column-sharded, and where a rank has no gradient (it still joins the sum)."""
+    world = 2
+    ret = mp.Manager().dict()
+    mp.spawn(_norm_worker, args=(world, _free_port(), golden['path'], ret), nprocs=world, join=True)
+    for a, b in zip(ret[0], ret[1]):
+        assert a[0] == b[0] and abs(a[0] / np.sqrt(a[1] + b[1]) - 1) < 1e-6 and a[0] > 0

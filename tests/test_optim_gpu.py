@@ -643,3 +643,70 @@ def test_first_steps_from_gradients_whose_squares_are_hardly_there(n, eight, eps
         want = -1e-3 * x / (np.abs(x) + float(np.float32(eps)))
         off = (16 * u + 2.0 ** -149 / (0.001 * x * x)) * np.abs(want)
         assert (np.abs(_flat(p) - want) <= off + HALF_STEP[dtype] * (np.abs(want) + off)).all(), (dtype, n, eps)
+
+
+@pytest.mark.parametrize('name', ['MF', 'LightGCN', 'IGCN'])
+def test_a_model_cut_by_columns_is_clipped_by_the_norm_of_all_its_columns(name):
+    """Two column slices trained side by side (a thread each, the all-reduce a sum over both) hold the moments of the unsharded trainer:
+    clipping scales every column by the one factor.  The slices' own norms are far apart, so a factor of a slice's own would be off by
+    1.2 and more in one of them; gradients agree to the order of their float32 sums (1e-4 of the largest is far above it)."""
+    import threading
+    from igcn_cf_amd.dataset import SyntheticDataset
+    from igcn_cf_amd.dist import column_shard_model
+    from igcn_cf_amd.model import get_model
+    from igcn_cf_amd.trainer import get_trainer
+    ds = SyntheticDataset({'name': 'SyntheticDataset', 'n_users': 300, 'n_items': 200, 'n_inter': 5000, 'device': DEV, 'seed': 3})
+    mcfg = {'name': name, 'embedding_size': 32, 'n_layers': 2, 'dropout': 0., 'feature_ratio': 1., 'device': DEV}
+    tcfg = {'name': 'IGCNTrainer' if name == 'IGCN' else 'BPRTrainer', 'optimizer': 'AdamW', 'lr': 1e-3, 'l2_reg': 1e-2, 'aux_reg': 0.1, 'device': DEV,
+            'n_epochs': 1, 'batch_size': 256, 'topks': [20], 'weight_decay': 0., 'max_grad_norm': 1e-3, 'hip_graph': False}
+    torch.manual_seed(4)
+    whole = get_model(mcfg, ds)
+    with torch.no_grad():
+        for k, p in whole.state_dict().items():
+            if p.dim() == 2:
+                p[:, :16] *= 5.
+    state = {k: v.detach().clone() for k, v in whole.state_dict().items()}
+    batches = [torch.stack([torch.randint(0, hi, (256,), generator=torch.Generator().manual_seed(i)) for hi in (300, 200, 200)], 1).to(DEV) for i in range(3)]
+
+    def go(trainer):
+        trainer.model.train()
+        for b in batches:
+            if name == 'IGCN':
+                trainer.igcn_step(b, b)
+            else:
+                trainer.bpr_step(b)
+        torch.cuda.synchronize()
+    plain = get_trainer(tcfg, ds, whole)
+    go(plain)
+    assert float(plain.opt.grad_norm) > 3e-3                                         # (clipping does something)
+    barrier, slots, errors = threading.Barrier(2, timeout=60), [None, None], []
+
+    def reduce_of(rank):
+        def reduce(t):
+            slots[rank] = t.clone()
+            barrier.wait()
+            total = slots[0] + slots[1]
+            barrier.wait()
+            return t.copy_(total)
+        return reduce
+    trainers = [get_trainer(tcfg, ds, column_shard_model(mcfg, ds, r, 2, full_state=state, reduce_fn=reduce_of(r))) for r in range(2)]
+
+    def rank(r):
+        try:
+            go(trainers[r])
+        except Exception as e:                                                       # noqa: BLE001 (shown below)
+            errors.append(e)
+            barrier.abort()
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for k, p in dict(whole.named_parameters()).items():
+        for what in ('exp_avg', 'exp_avg_sq'):
+            want = plain.opt.state[p][what]
+            got = torch.cat([tr.opt.state[dict(tr.model.named_parameters())[k]][what] for tr in trainers], -1)
+            assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max()), (k, what)
+    for tr in trainers:
+        assert abs(float(tr.opt.grad_norm) / float(plain.opt.grad_norm) - 1) < 1e-4
