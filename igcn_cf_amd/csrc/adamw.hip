@@ -419,11 +419,11 @@ static int grad_squares(const igcn_adamw_tensor *tensors, int64_t n, double *par
     });
 }
 
-// Whether memory that the step writes is shared between two of its tensors, or with a gradient (gradients may share theirs).
-static int check_overlap(const igcn_adamw_tensor *tensors, int64_t n, bool eight)
+// Whether memory that the step writes is shared between two of its tensors, or with a gradient or a number that it reads (those may share theirs).
+static int check_overlap(const igcn_adamw_tensor *tensors, int64_t n, bool eight, const float *lr_dev, const float *norm_in, const float *norm_out)
 {
     struct Stretch { uintptr_t begin, end; bool written; };
-    const std::unique_ptr<Stretch[]> all(new (std::nothrow) Stretch[6 * n]);
+    const std::unique_ptr<Stretch[]> all(new (std::nothrow) Stretch[6 * n + 2]);
     if (!all) return (int)hipErrorOutOfMemory;
     int64_t count = 0;
     auto add = [&](const void *p, int64_t bytes, bool written) {
@@ -438,6 +438,8 @@ static int check_overlap(const igcn_adamw_tensor *tensors, int64_t n, bool eight
         add(t.step, 4, true);
         add(t.grad, t.n * (t.grad_dtype == IGCN_DTYPE_F32 ? 4 : 2), false);
     }
+    add(lr_dev, lr_dev ? 4 : 0, false);
+    add(norm_in ? norm_in : norm_out, norm_in || norm_out ? 4 : 0, !norm_in);
     std::sort(all.get(), all.get() + count, [](const Stretch &a, const Stretch &b) { return a.begin < b.begin; });
     uintptr_t any = 0, written = 0;                              // the furthest end so far
     for (int64_t i = 0; i < count; ++i) {
@@ -449,7 +451,8 @@ static int check_overlap(const igcn_adamw_tensor *tensors, int64_t n, bool eight
 }
 
 // moment_bits 0: only the gradients are looked at
-static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment_bits)
+static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment_bits, const float *lr_dev = nullptr, const float *norm_in = nullptr,
+                         const float *norm_out = nullptr)
 {
     if (n < 0 || n > 0x7fffffff) return IGCN_E_SHAPE;
     if (n > 0 && !tensors) return IGCN_E_NULL;
@@ -468,7 +471,7 @@ static int check_tensors(const igcn_adamw_tensor *tensors, int64_t n, int moment
         if (!eight && ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & 3)) return IGCN_E_ALIGN;
         if ((reinterpret_cast<uintptr_t>(t.scales) | reinterpret_cast<uintptr_t>(t.step)) & 3) return IGCN_E_ALIGN;
     }
-    return moment_bits ? check_overlap(tensors, n, eight) : (int)IGCN_OK;
+    return moment_bits ? check_overlap(tensors, n, eight, lr_dev, norm_in, norm_out) : (int)IGCN_OK;
 }
 
 }  // namespace igcn
@@ -504,7 +507,8 @@ extern "C" int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_
                                void *workspace, void *stream)
 {
     if (moment_bits != 8 && moment_bits != 32) return IGCN_E_RANGE;
-    const int rc = check_tensors(tensors_host, n_tensors, moment_bits);
+    const bool clipped = max_norm > 0.0;
+    const int rc = check_tensors(tensors_host, n_tensors, moment_bits, lr_dev, clipped ? norm_in : nullptr, clipped ? norm_out : nullptr);
     if (rc != IGCN_OK) return rc;
     if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(max_norm >= 0.0))
         return IGCN_E_RANGE;

@@ -819,29 +819,36 @@ def _check_grads(grads):
     return grads[0].device if grads else None
 
 
-def grad_norm(grads):
+def _check_one_number(t, name, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or not t.is_cuda or (device is not None and t.device != device):
+        raise _lib.IgcnError('%s must be a one-element float32 tensor on the GPU' % name)
+
+
+def grad_norm(grads, out=None):
     """float32 scalar on the GPU: the L2 norm over all elements of all tensors of the list (igcn_grad_norm), added up in float64 in
     an order that depends on the sizes alone.  What torch.nn.utils.clip_grad_norm_ returns, without touching the gradients:
-    adamw_step(..., max_grad_norm=..., grad_norm=...) clips by it on the way."""
+    adamw_step(..., max_grad_norm=..., grad_norm=...) clips by it on the way.  out: a one-element float32 tensor to hold it."""
     grads = list(grads)
     device = _check_grads(grads)
+    if out is not None:
+        _check_one_number(out, 'out', device)
     if not grads:
-        return torch.zeros((), dtype=torch.float32, device='cuda')
+        return torch.zeros((), dtype=torch.float32, device='cuda') if out is None else out.zero_()
     if _elsewhere(grads[0]):
         with torch.cuda.device(device):
-            return grad_norm(grads)
+            return grad_norm(grads, out)
     rows = array.array('q')
     for g in grads:
         rows.extend((0, g.data_ptr(), 0, 0, 0, 0, g.numel(), _DTYPE_CODES[g.dtype] << 32))
     L, table = _lib.lib(), rows.buffer_info()[0]
     ws = torch.empty(L.igcn_adamw_workspace_bytes(table, len(grads)), dtype=torch.uint8, device=device)
-    out = torch.empty((), dtype=torch.float32, device=device)
+    out = torch.empty((), dtype=torch.float32, device=device) if out is None else out
     _lib.check(L.igcn_grad_norm(table, len(grads), out.data_ptr(), ws.data_ptr(), _stream_of(out)), 'igcn_grad_norm')
     return out
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None,
-               scales=None, seed=0, grad_norm=None):
+               scales=None, seed=0, grad_norm=None, norm_out=None):
     """One AdamW step over all tensors of the lists, in place (igcn_adamw_step; optim.AdamW is the optimizer around it).
 
     params: float32, bfloat16 or float16, any shapes, dense in memory; grads: the same shape and order in memory, dtype of the
@@ -851,7 +858,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     its code times its block's scale), rounded stochastically from (seed, place in the list, step, element); zeros to start with.
     lr: a number, or a one-element float32 tensor on the GPU (read by the kernel: HIP-graph replays see its current value).
     max_grad_norm: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) on the way; norm = L2 norm over all of them, computed
-    here or given as `grad_norm` (a one-element float32 tensor, for several calls clipped by one norm).  Returns the norm, or None.
+    here (into `norm_out`, a one-element float32 tensor, where that is given) or given as `grad_norm` (one as well, for several calls
+    clipped by one norm).  Returns the norm, or None.
     Memory that is rewritten (parameters, moments, scales, steps) stands in one place of the lists only."""
     params, grads, exp_avgs, exp_avg_sqs, steps = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps)
     n, eight = len(params), scales is not None
@@ -865,7 +873,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
     device = _check_grads(grads)
     if n and _elsewhere(grads[0]):
         with torch.cuda.device(device):
-            return adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay, max_grad_norm, scales if eight else None, seed, grad_norm)
+            return adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay, max_grad_norm, scales if eight else None, seed, grad_norm,
+                              norm_out)
     if n and {t.get_device() for ts in (params, exp_avgs, exp_avg_sqs, steps, scales if eight else ()) for t in ts} != {device.index}:
         raise _lib.IgcnError('the tensors of a call must be on one device, a GPU')
     pt, gt = [p.dtype for p in params], [g.dtype for g in grads]
@@ -895,23 +904,25 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.99
         lr_dev, lr = lr, 0.
     elif not lr >= 0.:
         raise _lib.IgcnError('lr must not be negative')
+    if norm_out is not None:
+        _check_one_number(norm_out, 'norm_out', device)
     if max_grad_norm is not None and grad_norm is not None:
-        if not isinstance(grad_norm, torch.Tensor) or grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or (n and grad_norm.device != device):
-            raise _lib.IgcnError('grad_norm must be a one-element float32 tensor on the GPU')
+        _check_one_number(grad_norm, 'grad_norm', device)
         norm_in = grad_norm
     if n == 0:
-        return None if max_grad_norm is None else norm_in if norm_in is not None else torch.zeros((), dtype=torch.float32, device='cuda')
+        return None if max_grad_norm is None else norm_in if norm_in is not None else \
+            torch.zeros((), dtype=torch.float32, device='cuda') if norm_out is None else norm_out.zero_()
     L, table = _lib.lib(), rows.buffer_info()[0]
     ws = torch.empty(L.igcn_adamw_workspace_bytes(table, n), dtype=torch.uint8, device=device)
-    norm, max_norm, norm_out = norm_in, 0., None
+    norm, max_norm, norm_at = norm_in, 0., None
     if max_grad_norm is not None:
         max_norm = float(max_grad_norm)
         if norm_in is None:
-            norm = torch.empty((), dtype=torch.float32, device=device)
-            norm_out = norm.data_ptr()
+            norm = torch.empty((), dtype=torch.float32, device=device) if norm_out is None else norm_out
+            norm_at = norm.data_ptr()
     code = L.igcn_adamw_step(table, n, 8 if eight else 32, float(lr), _lib.ptr(lr_dev), float(betas[0]), float(betas[1]), float(eps),
                              float(weight_decay), max_norm, _lib.ptr(norm_in),
-                             norm_out, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index))
+                             norm_at, int(seed) & 0xFFFFFFFFFFFFFFFF, ws.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index))
     if code:
         _lib.check(code, 'igcn_adamw_step')
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])

@@ -10,7 +10,8 @@ class AdamW(torch.optim.Optimizer):
     """Adam with decoupled weight decay.  state_bits 32: moments in float32 (state names and meaning of torch.optim.AdamW, whose
     state_dict it takes).  state_bits 8: exp_avg as float8_e4m3fn and exp_avg_sq as float8_e5m2 codes with two float32 scales a block
     of 128 elements ('scales') — 2.06 bytes a parameter instead of 8; a moment is codes.float() * its block's scale.
-    max_grad_norm: clip by the norm over the gradients of ALL groups; the last step's norm is `grad_norm` (a tensor on the GPU).
+    max_grad_norm: clip by the norm over the gradients of ALL groups; the last step's norm is `grad_norm` (a tensor on the GPU, the same
+    one at every step, captured or not: copy it to keep it).
     norm_reduce_fn: for parameters that are a rank's share of a model (dist.ShardedLightGCN, ColumnShardedLightGCN: their all_reduce;
     dist.column_shard_model: slice_reduce_fn, which the trainers pass): sums a tensor over the ranks, in place, so that every rank clips by
     the norm over all shares (parameters that dist marks as shares are refused without).  Called once a step on one float64 number, also
@@ -49,12 +50,12 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def _common_norm(self, grads):
-        """The norm over the gradients of all groups, and of all ranks where they hold shares."""
-        norm = ops.grad_norm(grads) if grads else torch.zeros((), device=self.param_groups[0]['params'][0].device)
+        """self.grad_norm = the norm over the gradients of all groups, and of all ranks where they hold shares."""
+        norm = ops.grad_norm(grads, out=self.grad_norm) if grads else self.grad_norm.zero_()
         if self.norm_reduce_fn is not None:
             square = norm.double().square()
             self.norm_reduce_fn(square)
-            norm = square.sqrt().float()
+            norm.copy_(square.sqrt())
         return norm
 
     @torch.no_grad()
@@ -72,16 +73,20 @@ class AdamW(torch.optim.Optimizer):
             gs = [p.grad if ops._same_order(p, p.grad) else torch.empty_like(p, dtype=p.grad.dtype).copy_(p.grad) for p in ps]
             if ps:
                 calls.append((gi, group, ps, gs))
-        norm = None
-        if self.max_grad_norm is not None and (len(calls) > 1 or self.norm_reduce_fn is not None):
-            norm = self.grad_norm = self._common_norm([g for call in calls for g in call[3]])
+        norm = norm_out = None
+        if self.max_grad_norm is not None:
+            device = (calls[0][2] if calls else self.param_groups[0]['params'])[0].device
+            if self.grad_norm is None or self.grad_norm.device != device:
+                self.grad_norm = torch.zeros((), dtype=torch.float32, device=device)
+            norm_out = self.grad_norm
+            if len(calls) != 1 or self.norm_reduce_fn is not None:
+                norm = self._common_norm([g for call in calls for g in call[3]])
         for gi, group, ps, gs in calls:
             states = [self._state_of(p, group['state_bits']) for p in ps]
-            got = ops.adamw_step(ps, gs, [s['exp_avg'] for s in states], [s['exp_avg_sq'] for s in states], [s['step'] for s in states],
-                                 lr=group['lr'], betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'],
-                                 max_grad_norm=self.max_grad_norm, scales=[s['scales'] for s in states] if group['state_bits'] == 8 else None,
-                                 seed=self.seed + (gi << 32), grad_norm=norm)
-            self.grad_norm = got
+            ops.adamw_step(ps, gs, [s['exp_avg'] for s in states], [s['exp_avg_sq'] for s in states], [s['step'] for s in states],
+                           lr=group['lr'], betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'],
+                           max_grad_norm=self.max_grad_norm, scales=[s['scales'] for s in states] if group['state_bits'] == 8 else None,
+                           seed=self.seed + (gi << 32), grad_norm=norm, norm_out=norm_out)
         return loss
 
     def __getstate__(self):                # (copies and pickles keep what torch's form of it does not know)

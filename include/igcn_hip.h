@@ -507,7 +507,7 @@ typedef struct igcn_adamw_tensor {
  * element); v > 0 is never held as 0; a block below 2^-100 is held as zeros, one with a NaN or an infinity gets a NaN scale.
  * The averages themselves are formed unrounded before the parameter is updated.
  * workspace: igcn_adamw_workspace_bytes(...) bytes, 16-byte aligned; one call's own.  Memory that the call rewrites stands in one
- * place of the list only, gradients included (IGCN_E_OVERLAP); a tensor has at most (2^24 - 1) * 2048 elements. */
+ * place of the list only, gradients, lr_dev and the norm included (IGCN_E_OVERLAP); a tensor has at most (2^24 - 1) * 2048 elements. */
 int64_t igcn_adamw_workspace_bytes(const igcn_adamw_tensor *tensors_host, int64_t n_tensors);
 int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, int32_t moment_bits, double lr, const float *lr_dev,
                     double beta1, double beta2, double eps, double weight_decay, double max_norm, const float *norm_in, float *norm_out,

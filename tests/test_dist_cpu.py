@@ -533,7 +533,7 @@ def _norm_worker(rank, world, port, path, ret):
         from igcn_cf_amd import optim
         from igcn_cf_amd.dataset import ProcessedDataset
         from igcn_cf_amd.dist import ColumnShardedLightGCN, ShardedLightGCN
-        optim.ops.grad_norm = lambda gs: torch.sqrt(sum(g.double().square().sum() for g in gs)).float()      # the kernel runs on GPUs only
+        optim.ops.grad_norm = lambda gs, out: out.copy_(torch.sqrt(sum(g.double().square().sum() for g in gs)))      # the kernel runs on GPUs only
         ds = ProcessedDataset({'name': 'ProcessedDataset', 'path': path, 'device': 'cpu'})
         norms = []
         for model in (ColumnShardedLightGCN(ds, 8, 2, rank, world, 'cpu', propagate_fn=lambda e: e, loss_fn=lambda *a: None),
@@ -545,6 +545,7 @@ def _norm_worker(rank, world, port, path, ret):
                 pass
             optim.AdamW(model.parameters())
             opt = optim.AdamW(model.parameters(), max_grad_norm=1., norm_reduce_fn=model.all_reduce)
+            opt.grad_norm = torch.zeros(())
             grads = [torch.full_like(p, 10. ** rank) for p in model.parameters()]
             norms.append((float(opt._common_norm(grads)), float(sum(g.double().square().sum() for g in grads))))
             norms.append((float(opt._common_norm(grads if rank else [])), float(sum(g.double().square().sum() for g in grads)) if rank else 0.))

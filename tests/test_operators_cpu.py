@@ -173,3 +173,14 @@ def test_a_copied_optimizer_keeps_its_settings():
     opt = AdamW([w], lr=0.1, state_bits=8, max_grad_norm=2., seed=5)
     for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
         assert other.max_grad_norm == 2. and other.seed == 5 and other.param_groups[0]['state_bits'] == 8 and other.grad_norm is None
+
+
+def test_the_c_step_refuses_a_norm_or_a_rate_in_memory_that_it_rewrites():
+    L = _lib.lib()
+
+    def step(mx=1., lr_dev=None, ni=None, no=0x9000):
+        t = _table()
+        return L.igcn_adamw_step(t.buffer_info()[0], 1, 32, 1e-3, lr_dev, 0.9, 0.999, 1e-8, 0.01, mx, ni, no, 0, 0x100, None)
+    for at in (0x1000, 0x13fc, 0x3000, 0x4100, 0x6000):                               # parameter, moments, step
+        assert step(no=at) == -7 and step(ni=at) == -7 and step(lr_dev=at) == -7 and step(mx=0., lr_dev=at) == -7, hex(at)
+    assert step(no=0x2000) == -7                                                      # (a gradient: read by the step, so not to be written)

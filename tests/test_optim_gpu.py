@@ -710,3 +710,67 @@ def test_a_model_cut_by_columns_is_clipped_by_the_norm_of_all_its_columns(name):
             assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max()), (k, what)
     for tr in trainers:
         assert abs(float(tr.opt.grad_norm) / float(plain.opt.grad_norm) - 1) < 1e-4
+
+
+@pytest.mark.parametrize('name', ['MF', 'LightGCN'])
+def test_the_norm_is_the_last_steps_replayed_or_eager(name):
+    """Full batches replay a captured step, a shorter one runs eagerly: grad_norm is that of whichever ran last, in one tensor throughout.
+    Nothing moves (lr 0), so a batch's norm is the same whenever it runs, to the order of its float32 sums."""
+    ds, model, trainer = _trainer(name, True, 32)
+    for group in trainer.opt.param_groups:
+        group['lr'] = 0.
+    model.train()
+    if name == 'MF':
+        step, batches = trainer.flat_step, lambda n: next(iter(trainer.sampler.epoch_node_batches(n, 0)))
+    else:
+        step, batches = trainer.node_step, lambda n: next(iter(trainer.sampler.epoch_node_batches(n, ds.n_users)))
+    full, short = batches(1024).clone(), batches(40).clone()
+    step(full)
+    held, at_full = trainer.opt.grad_norm, float(trainer.opt.grad_norm)
+    step(short)
+    at_short = float(trainer.opt.grad_norm)
+    assert abs(at_short / at_full - 1) > 0.01
+    for _ in range(2):
+        step(full)
+        assert abs(float(trainer.opt.grad_norm) / at_full - 1) < 1e-4
+        step(short)
+        assert abs(float(trainer.opt.grad_norm) / at_short - 1) < 1e-4
+    assert trainer._graph is not None and trainer.opt.grad_norm is held
+
+
+def test_a_norm_goes_where_it_is_asked_to():
+    from igcn_cf_amd import _lib, ops
+    rng = np.random.default_rng(12)
+    gs = [_grads(s, rng) for s in ((3, 50), (70001,))]
+    want, out = ops.grad_norm(gs), torch.zeros(1, device=DEV)
+    assert ops.grad_norm(gs, out=out) is out and out[0] == want
+    assert ops.grad_norm([], out=out) is out and float(out) == 0.
+    for n in (1, 2):                                                                 # one launch, and more
+        for given in (None, torch.full((), 7., device=DEV)):
+            p = [torch.ones_like(g) for g in gs[:n]]
+            m, v, t = [torch.zeros_like(g) for g in p], [torch.zeros_like(g) for g in p], [torch.zeros((), device=DEV) for _ in p]
+            out.fill_(-1.)
+            got = ops.adamw_step(p, gs[:n], m, v, t, lr=0.1, max_grad_norm=1., grad_norm=given, norm_out=out)
+            assert (got is out and out[0] == ops.grad_norm(gs[:n])) if given is None else (got is given and float(out) == -1.)
+    for bad in (torch.zeros(()), torch.zeros(2, device=DEV), torch.zeros((), dtype=torch.float64, device=DEV), 1., t[0]):
+        with pytest.raises(_lib.IgcnError):
+            ops.adamw_step(p, gs, m, v, t, lr=0.1, max_grad_norm=1., norm_out=bad)
+        if bad is not t[0]:
+            with pytest.raises(_lib.IgcnError):
+                ops.grad_norm(gs, out=bad)
+    with pytest.raises(_lib.IgcnError):
+        ops.adamw_step(p, gs, m, v, t, lr=p[0][0, :1], max_grad_norm=1.)
+    with pytest.raises(_lib.IgcnError):
+        ops.adamw_step(p, gs, m, v, t, lr=0.1, max_grad_norm=1., grad_norm=t[1])
+
+
+def test_a_step_without_gradients_has_norm_zero():
+    from igcn_cf_amd.optim import AdamW
+    w = torch.nn.Parameter(torch.ones(3, device=DEV))
+    opt = AdamW([w], max_grad_norm=1.)
+    w.grad = torch.full((3,), 2., device=DEV)
+    opt.step()
+    assert abs(float(opt.grad_norm) - 12 ** 0.5) < 1e-6
+    w.grad = None
+    opt.step()
+    assert float(opt.grad_norm) == 0.
