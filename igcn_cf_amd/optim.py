@@ -93,24 +93,47 @@ class AdamW(torch.optim.Optimizer):
         return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm, 'seed': self.seed, 'grad_norm': self.grad_norm,
                 'norm_reduce_fn': self.norm_reduce_fn}
 
+    @staticmethod
+    def _loaded(p, saved):
+        """The state of p that a saved one stands for: float32 moments laid out like p, or codes and scales as they are."""
+        if set(saved) & {'step', 'exp_avg', 'exp_avg_sq'} != {'step', 'exp_avg', 'exp_avg_sq'}:
+            raise ValueError('a saved state holds step, exp_avg and exp_avg_sq')
+        step = torch.as_tensor(saved['step'], dtype=torch.float32)
+        moments = {name: saved[name] for name in ('exp_avg', 'exp_avg_sq')}
+        if step.numel() != 1 or any(value.shape != p.shape for value in moments.values()):
+            raise ValueError('a saved state has one step and moments of the parameter\'s shape (got %s and %s for %s)'
+                             % (tuple(step.shape), [tuple(m.shape) for m in moments.values()], tuple(p.shape)))
+        state = {'step': step.reshape(()).to(device=p.device, copy=True)}
+        if 'scales' not in saved:
+            if any(m.dtype not in (torch.float64, *ops._DTYPE_CODES) for m in moments.values()):
+                raise ValueError('8-bit moments come with their scales')
+            return {**state, **{name: torch.empty_like(p, dtype=torch.float32).copy_(m) for name, m in moments.items()}}
+        if tuple(m.dtype for m in moments.values()) != ops.MOMENT_DTYPES or \
+                saved['scales'].dtype != torch.float32 or saved['scales'].shape != ((p.numel() + ops.ADAMW_BLOCK - 1) // ops.ADAMW_BLOCK, 2):
+            raise ValueError('8-bit moments are float8_e4m3fn and float8_e5m2 with float32 scales [ceil(numel / %d), 2]' % ops.ADAMW_BLOCK)
+        if not all(ops._same_order(p, m) for m in moments.values()):
+            raise ValueError('8-bit moments share scales in memory order: they must lie in memory as their parameter does')
+        return {**state, **{name: m.to(device=p.device, copy=True) for name, m in moments.items()},
+                'scales': saved['scales'].to(device=p.device, copy=True, memory_format=torch.contiguous_format)}
+
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
-        """As torch's, but the state keeps its own types (torch's casts every floating state to its parameter's).  Takes the state of
-        torch.optim.AdamW too; a group's state_bits then follow from what the state holds."""
+        """As torch's, but the moments keep the form they are saved in, 8-bit or not (torch's casts every floating state to its
+        parameter's type), and what does not fit is refused before anything changes.  Takes the state of torch.optim.AdamW too, whose
+        moments may be in the parameter's type; a group's state_bits then follow from what the state holds."""
         if any(g.get('amsgrad') or g.get('maximize') for g in state_dict['param_groups']):
             raise ValueError('a state with amsgrad or maximize is another optimizer\'s')
-        super().load_state_dict(state_dict)
-        for saved, group in zip(state_dict['param_groups'], self.param_groups):
-            for name, value in self.defaults.items():
-                group.setdefault(name, value)
-            held = {8 if 'scales' in state_dict['state'][i] else 32 for i in saved['params'] if i in state_dict['state']}
-            if len(held) > 1:
-                raise ValueError('a group holds its moments in one form')
-            group['state_bits'] = held.pop() if held else group['state_bits']
         saved = [i for g in state_dict['param_groups'] for i in g['params']]
         mine = [p for g in self.param_groups for p in g['params']]
+        states = {i: self._loaded(p, state_dict['state'][i]) for i, p in zip(saved, mine) if state_dict['state'].get(i)}
+        held = [{8 if 'scales' in states[i] else 32 for i in g['params'] if i in states} for g in state_dict['param_groups']]
+        if any(len(bits) > 1 for bits in held):
+            raise ValueError('a group holds its moments in one form')
+        super().load_state_dict(state_dict)
+        for bits, group in zip(held, self.param_groups):
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+            group['state_bits'] = bits.pop() if bits else group['state_bits']
         for i, p in zip(saved, mine):
-            for name, value in state_dict['state'].get(i, {}).items():
-                if name == 'step':
-                    value = torch.as_tensor(value, dtype=torch.float32).reshape(())
-                if torch.is_tensor(value):
-                    self.state[p][name] = value.to(device=p.device, copy=True)
+            if i in states:
+                self.state[p].update(states[i])

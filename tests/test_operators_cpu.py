@@ -184,3 +184,69 @@ def test_the_c_step_refuses_a_norm_or_a_rate_in_memory_that_it_rewrites():
     for at in (0x1000, 0x13fc, 0x3000, 0x4100, 0x6000):                               # parameter, moments, step
         assert step(no=at) == -7 and step(ni=at) == -7 and step(lr_dev=at) == -7 and step(mx=0., lr_dev=at) == -7, hex(at)
     assert step(no=0x2000) == -7                                                      # (a gradient: read by the step, so not to be written)
+
+
+def _torch_state(w, steps=3):
+    """A torch.optim.AdamW state of w after some steps, and the optimizer's groups."""
+    opt = torch.optim.AdamW([w], lr=1e-2)
+    for k in range(steps):
+        w.grad = torch.randn(w.shape, generator=torch.Generator().manual_seed(k)).to(w.dtype)
+        opt.step()
+    return opt.state_dict()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('transposed,saved_transposed', [(False, False), (True, True), (True, False), (False, True)])
+def test_a_loaded_state_has_the_steps_types_and_its_parameters_order(dtype, transposed, saved_transposed):
+    """torch.optim.AdamW holds moments in the parameter's type, and a saved tensor may lie in memory in another order: what is loaded are float32
+    moments, laid out like the parameter, of the same values."""
+    def param(tr):
+        data = torch.randn(6, 10, generator=torch.Generator().manual_seed(9)).to(dtype)
+        return torch.nn.Parameter(data.t().contiguous().t() if tr else data)
+    saved = _torch_state(param(saved_transposed))
+    w = param(transposed)
+    opt = AdamW([w], lr=1e-2)
+    opt.load_state_dict(saved)
+    for name in ('exp_avg', 'exp_avg_sq'):
+        got, want = opt.state[w][name], saved['state'][0][name]
+        assert want.dtype == dtype and got.dtype == torch.float32 and torch.equal(got, want.float()), name
+        assert ops._same_order(w, got) and got.data_ptr() != want.data_ptr(), name
+    assert opt.state[w]['step'].dtype == torch.float32 and float(opt.state[w]['step']) == 3. and opt.param_groups[0]['state_bits'] == 32
+
+
+def test_a_state_that_does_not_fit_is_refused_and_changes_nothing():
+    """8-bit codes share scales in memory order, so they do not go to a parameter of another order; nor does a moment of another shape, nor half a
+    form.  The optimizer stays as it was."""
+    w = torch.nn.Parameter(torch.zeros(16, 24))
+    tr = torch.nn.Parameter(torch.zeros(24, 16).t())
+
+    def state(p, **new):
+        codes = [torch.full_like(p, 5, dtype=torch.uint8).view(d) for d in ops.MOMENT_DTYPES]
+        s = {'step': torch.tensor(4.), 'exp_avg': codes[0].detach(), 'exp_avg_sq': codes[1].detach(), 'scales': torch.rand(3, 2)}
+        s.update(new)
+        opt = AdamW([p], lr=0.5, state_bits=8)
+        return {'state': {0: {k: v for k, v in s.items() if v is not None}}, 'param_groups': opt.state_dict()['param_groups']}
+    fine = AdamW([w], lr=1e-2)
+    fine.load_state_dict(state(w))
+    assert fine.state[w]['exp_avg'].dtype == torch.float8_e4m3fn and fine.param_groups[0]['state_bits'] == 8 and fine.param_groups[0]['lr'] == 0.5
+    assert torch.equal(fine.state[w]['exp_avg'].view(torch.uint8), torch.full((16, 24), 5, dtype=torch.uint8))
+    f32 = torch.zeros(16, 24)
+    bad = [(w, state(tr)), (tr, state(w)), (w, state(w, scales=torch.rand(4, 2))), (w, state(w, exp_avg=f32)), (w, state(w, exp_avg_sq=None)),
+           (w, state(w, scales=None)), (w, state(w, exp_avg=f32, exp_avg_sq=torch.zeros(24, 16), scales=None)), (w, state(w, step=None)),
+           (w, state(w, step=torch.zeros(2))), (w, state(w, exp_avg=f32[:8], exp_avg_sq=f32[:8], scales=None))]
+    for i, (p, saved) in enumerate(bad):
+        opt = AdamW([p], lr=1e-2, state_bits=32)
+        opt.state[p].update(step=torch.tensor(1.), exp_avg=torch.zeros_like(p).detach(), exp_avg_sq=torch.zeros_like(p).detach())
+        held = dict(opt.state[p])
+        with pytest.raises(ValueError):
+            opt.load_state_dict(saved)
+            print('not refused:', i)
+        assert opt.param_groups[0]['lr'] == 1e-2 and opt.param_groups[0]['state_bits'] == 32 and all(opt.state[p][k] is v for k, v in held.items()), i
+    a, b = torch.nn.Parameter(torch.zeros(16, 24)), torch.nn.Parameter(torch.zeros(16, 24))
+    mixed = state(w)
+    mixed['param_groups'][0]['params'] = [0, 1]
+    mixed['state'][1] = {'step': torch.tensor(4.), 'exp_avg': f32, 'exp_avg_sq': f32}
+    opt = AdamW([a, b], lr=1e-2)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(mixed)
+    assert opt.param_groups[0]['lr'] == 1e-2 and not opt.state

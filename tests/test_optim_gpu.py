@@ -774,3 +774,32 @@ def test_a_step_without_gradients_has_norm_zero():
     w.grad = None
     opt.step()
     assert float(opt.grad_norm) == 0.
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_a_run_of_torchs_adamw_in_16_bits_goes_on(dtype):
+    """Its moments are in the parameter's type, one parameter is transposed in memory and one saved moment is not: the next step is the
+    formula's from the saved values (where torch's own steps left the parameter finite: 1e-8 is 0 in float16, and some of its second moments are)."""
+    from igcn_cf_amd.optim import AdamW
+    rng = np.random.default_rng(14)
+    ps = [torch.nn.Parameter(_params((33, 20), rng, dtype)), torch.nn.Parameter(_params((20, 33), rng, dtype).t())]
+    theirs = torch.optim.AdamW(ps, **HYPER)
+    for _ in range(3):
+        for p in ps:
+            p.grad = _grads((33, 20), rng, dtype)
+        theirs.step()
+    saved = theirs.state_dict()
+    saved['state'][1]['exp_avg'] = saved['state'][1]['exp_avg'].contiguous()
+    ours = AdamW(ps, **HYPER)
+    ours.load_state_dict(saved)
+    before = [(p.detach().clone(), ours.state[p]['exp_avg'].clone(), ours.state[p]['exp_avg_sq'].clone()) for p in ps]
+    for (p0, m0, v0), i in zip(before, range(2)):
+        assert m0.dtype == torch.float32 and torch.equal(m0, saved['state'][i]['exp_avg'].float()) and torch.equal(v0, saved['state'][i]['exp_avg_sq'].float())
+    gs = [torch.empty_like(p).copy_(_grads((33, 20), rng, dtype)) for p in ps]
+    for p, g in zip(ps, gs):
+        p.grad = g
+    ours.step()
+    for p, g, (p0, m0, v0) in zip(ps, gs, before):
+        fine = torch.isfinite(p0)
+        assert bool(torch.isclose(p[~fine], p0[~fine], equal_nan=True).all()) and bool(fine.any())
+        _check32(p0[fine], g[fine], m0[fine], v0[fine], 4, p[fine], ours.state[p]['exp_avg'][fine], ours.state[p]['exp_avg_sq'][fine])
