@@ -217,14 +217,23 @@ class BasicTrainer:
         return tok
 
     def _graph_key(self):
-        """Everything a captured step bakes in as pointers or launch constants: a swapped graph / feature matrix /
-        optimizer, or a changed dropout rate, regulariser weight or learning rate, captures again."""
-        m = self.model
-        return (self._token(getattr(m, 'norm_adj', None)), self._token(getattr(m, 'feat_mat', None)), self._token(self.opt),
-                self.batch_size, getattr(m, 'dropout', None), bool(m.training), getattr(self, 'l2_reg', None),
-                getattr(self, 'aux_reg', None), tuple(float(g['lr']) for g in self.opt.param_groups)) + \
-            ((self.opt.max_grad_norm, self.opt.seed) + tuple((*g['betas'], g['eps'], g['weight_decay']) for g in self.opt.param_groups)
-             if isinstance(self.opt, AdamW) else ())
+        """Everything a captured step bakes in as pointers or launch constants: a swapped graph / feature matrix / optimizer, a
+        replaced parameter or optimizer state (load_state_dict makes new tensors; each counts in its own place, so that an address that
+        comes back in another one is another key), or a changed dropout rate, regulariser weight or learning rate, captures again."""
+        m, opt = self.model, self.opt
+        key = [self._token(getattr(m, 'norm_adj', None)), self._token(getattr(m, 'feat_mat', None)), self._token(opt),
+               self.batch_size, getattr(m, 'dropout', None), bool(m.training), getattr(self, 'l2_reg', None),
+               getattr(self, 'aux_reg', None)]
+        for g in opt.param_groups:
+            key.append(float(g['lr']))
+            if isinstance(opt, AdamW):
+                key += [*g['betas'], g['eps'], g['weight_decay']]
+            for p in g['params']:
+                key.append(p.data_ptr())
+                key += [(name, t.data_ptr()) for name, t in opt.state.get(p, {}).items() if torch.is_tensor(t)]
+        if isinstance(opt, AdamW):
+            key += [opt.max_grad_norm, opt.seed]
+        return tuple(key)
 
     def _graph_step(self, inputs, loss_fn, kind='nodes'):
         """Replays the captured step on `inputs` (tensors copied into the static buffers the graph reads); captures
@@ -234,7 +243,7 @@ class BasicTrainer:
         if getattr(self, '_graph', None) is None or self._graph_for != key:
             self._graph = None
             self._capture_step(inputs, loss_fn)
-            self._graph_for = key
+            self._graph_for = self._graph_key() + (kind,)     # (the first steps made the optimizer's state)
         for st, t in zip(self._static_inputs, inputs):
             if st.data_ptr() != t.data_ptr():                # (a sampler that drew straight into the buffer: nothing to copy)
                 st.copy_(t)

@@ -250,3 +250,34 @@ def test_a_state_that_does_not_fit_is_refused_and_changes_nothing():
     with pytest.raises(ValueError):
         opt.load_state_dict(mixed)
     assert opt.param_groups[0]['lr'] == 1e-2 and not opt.state
+
+
+@pytest.mark.parametrize('make', [lambda ps: AdamW(ps, lr=0.1), lambda ps: AdamW(ps, lr=0.1, state_bits=8), lambda ps: torch.optim.Adam(ps, lr=0.1),
+                                  lambda ps: torch.optim.SGD(ps, lr=0.1, momentum=0.9)])
+def test_a_captured_steps_key_names_the_memory_the_optimizer_writes(make):
+    """A captured step holds the addresses of the parameters and of the optimizer's state: whatever replaces one of them — load_state_dict, a new
+    .data — makes another key; a step, which rewrites them in place, does not."""
+    import copy
+    from igcn_cf_amd.trainer import BPRTrainer
+    ps = [torch.nn.Parameter(torch.zeros(300, 4)), torch.nn.Parameter(torch.zeros(7))]
+    trainer = BPRTrainer.__new__(BPRTrainer)
+    trainer.model, trainer.opt, trainer.batch_size = torch.nn.Module(), make(ps), 4
+    for p in ps:
+        p.grad = torch.ones_like(p)
+        if isinstance(trainer.opt, AdamW):
+            trainer.opt._state_of(p, trainer.opt.param_groups[0]['state_bits'])
+    if not isinstance(trainer.opt, AdamW):
+        trainer.opt.step()
+    key = trainer._graph_key()
+    held = [dict(trainer.opt.state[p]) for p in ps]                                   # (so that no address comes back)
+    if not isinstance(trainer.opt, AdamW):
+        trainer.opt.step()
+    assert trainer._graph_key() == key
+    trainer.opt.load_state_dict(copy.deepcopy(trainer.opt.state_dict()))
+    after = trainer._graph_key()
+    assert after != key and trainer._graph_key() == after
+    old, ps[1].data = ps[1].data, torch.zeros(7)
+    assert trainer._graph_key() != after and held and old is not None
+    if isinstance(trainer.opt, AdamW):
+        trainer.opt.state.clear()
+        assert trainer._graph_key() != after

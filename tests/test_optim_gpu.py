@@ -803,3 +803,45 @@ def test_a_run_of_torchs_adamw_in_16_bits_goes_on(dtype):
         fine = torch.isfinite(p0)
         assert bool(torch.isclose(p[~fine], p0[~fine], equal_nan=True).all()) and bool(fine.any())
         _check32(p0[fine], g[fine], m0[fine], v0[fine], 4, p[fine], ours.state[p]['exp_avg'][fine], ours.state[p]['exp_avg_sq'][fine])
+
+
+@pytest.mark.parametrize('name,bits', [('MF', 32), ('LightGCN', 8), ('LightGCN', 32)])
+def test_captured_steps_follow_a_state_that_is_loaded_between_them(name, bits):
+    """Back to a checkpoint in mid-run: steps, a save, more steps, model and optimizer loaded, more steps — captured like eager.  Moments are what the
+    restored ones lead to (their steps go on from the checkpoint's); gradients come from float atomics, so they agree to their sums' order."""
+    import copy
+    ends = []
+    for hip_graph in (True, False):
+        ds, model, trainer = _trainer(name, hip_graph, bits)
+        if name == 'MF':
+            step, draw = trainer.flat_step, lambda n: trainer.sampler.epoch_node_batches(n, 0)
+        else:
+            step, draw = trainer.node_step, lambda n: trainer.sampler.epoch_node_batches(n, ds.n_users)
+        batches, short = [b.clone() for _, b in zip(range(6), draw(1024))], next(draw(40)).clone()
+        for b in batches + [short]:
+            users, items = b.view(3, -1)[0], b.view(3, -1)[1:] - (0 if name == 'MF' else ds.n_users)
+            assert 0 <= int(users.min()) and int(users.max()) < ds.n_users and 0 <= int(items.min()) and int(items.max()) < ds.n_items
+        model.train()
+        for b in batches[:3]:
+            step(b)
+        saved = copy.deepcopy((model.state_dict(), trainer.opt.state_dict()))
+        first = trainer._graph
+        for b in batches[3:]:
+            step(b)
+        assert trainer._graph is first and (first is not None) == hip_graph
+        held = [dict(s) for s in trainer.opt.state.values()]                          # (the old memory stays: nothing may still go there)
+        before = [{k: v.clone() for k, v in s.items()} for s in held]
+        model.load_state_dict(saved[0])
+        trainer.opt.load_state_dict(saved[1])
+        for b in batches[3:] * 2:
+            step(b)
+            step(short)                                                              # eager
+        torch.cuda.synchronize()
+        for h, b in zip(held, before):
+            assert all(torch.equal(h[k].view(torch.uint8) if h[k].dim() else h[k], b[k].view(torch.uint8) if b[k].dim() else b[k]) for k in h)
+        assert {float(s['step']) for s in trainer.opt.state.values()} == {15.}
+        ends.append([trainer.opt.state[p]['exp_avg'].float() if bits == 32 else
+                     trainer.opt.state[p]['exp_avg'].float().reshape(-1) * trainer.opt.state[p]['scales'][:, 0].repeat_interleave(128)[:p.numel()]
+                     for p in model.parameters()])
+    for a, b in zip(*ends):
+        assert float((a - b).abs().mean()) <= 1e-2 * float(b.abs().max())
