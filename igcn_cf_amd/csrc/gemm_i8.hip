@@ -6,6 +6,7 @@
 //
 // Measured: 8192 x 8192 x 4096 to bfloat16 264 us = 2.1 POP/s (a library's bare int8 product: 306 us), 512 x 96421 x 64 to float32 45-54 us = 3.7-4.4
 // TB/s of y (the same stores alone 45), 4 x 16384 x 8192 28 us = 4.8 TB/s of b, 16 x 4096 x 4096 7 us, 1 x 96421 x 64 from float32 7.1 us.
+#include "gemm_i8_rule.h"
 #include "quant_i8.h"
 #include <type_traits>
 
@@ -82,7 +83,6 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int k, i
 // 64 x 96421 x 64: 8.2 -> 11.4, so only where the depth pays for the exchange).
 // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, 4 tiles of a deep at a time, so that the tiles under way there
 // share their rows in its L2 (512 x 96421 x 64, whose rows of y end inside a line, without: 47 -> 74 us).
-constexpr int kDepth = 128;
 __device__ const i32x4 g_zeros = {0, 0, 0, 0};
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -102,7 +102,6 @@ __device__ __forceinline__ void to_lds(const void *p, unsigned lds)
 #pragma clang diagnostic pop
 template <int LEFT> __device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory"); }      // all but the last LEFT are there
 
-constexpr int64_t kMostApart = 1 << 23;                          // bytes between rows: 256 of them fit 31 bits
 struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; };
 
 constexpr size_t kExchanged = 3 * 4 * 4096;                      // of LDS: three waves' sums of four pieces
@@ -327,7 +326,7 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
     constexpr int64_t kMostTiles = ((int64_t)1 << 32) / (64 * WM * WN) - 8;      // a launch has fewer than 2^32 threads
     if (T.tiles_m > kMostTiles / T.tiles_n) return IGCN_E_SHAPE;
     T.per_xcd = (T.tiles_m * T.tiles_n + 7) / 8;
-    const bool direct = ((reinterpret_cast<uintptr_t>(G.a) | reinterpret_cast<uintptr_t>(G.b) | (uintptr_t)G.lda | (uintptr_t)G.ldb | (uintptr_t)G.k) & 15) == 0;
+    const bool direct = i8_direct(reinterpret_cast<uintptr_t>(G.a), reinterpret_cast<uintptr_t>(G.b), G.lda, G.ldb, G.k);
     auto launch = [&](auto *kernel, int most) {
         int64_t stages = (G.k + kDepth - 1) / kDepth;
         stages = stages < most ? stages : most;
@@ -350,8 +349,6 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
 // Bound by the bytes of b, each used once, or by the way through the depth where neither side has many: no tile is worth staging.  A wave takes 16 rows of b as the matrix instruction's first operand straight
 // from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and up to 16 rows of a, which stay in L2, as the
 // second.  KEEP steps' loads are under way while the ones before are multiplied.
-constexpr int kStep = 64;                                        // codes of depth a matrix instruction takes
-
 // A lane's row of either side.  BYTES: rows at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it
 // (1 row against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first
 // and the last row of b, whose words may reach over its ends, are loaded as they are.  What is behind a row's end meets zeros of a.
@@ -487,7 +484,7 @@ __global__ __launch_bounds__(kBlock) void stream_i8_kernel(const GemmArgs G)
         }
 }
 
-static bool any_byte(const void *p, int64_t ld) { return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)ld) & 3) != 0; }
+static bool any_byte(const void *p, int64_t ld) { return i8_any_byte(reinterpret_cast<uintptr_t>(p), ld); }
 static bool fits_launch(int64_t blocks) { return blocks < ((int64_t)1 << 32) / kBlock; }       // of kBlock threads: 2^32 in all
 
 template <int MG, int TILES> static int stream(const GemmArgs &G, hipStream_t st)
@@ -499,15 +496,9 @@ template <int MG, int TILES> static int stream(const GemmArgs &G, hipStream_t st
     return launch_status();
 }
 
-// The same for a few short rows in floating point: every workgroup makes them 8-bit on the way, with the quantiser's own steps, and lays them
-// out in LDS in the order the lanes read them: [16 codes of depth][row][16 bytes], rows rounded up to a power of two (lanes past them read
-// another row's bytes; what they compute is not stored).  No launch, no buffer; worth it while that is less work than a launch (us this way
-// and in two launches: 1 x 64 against 96421 rows 6.7 and 8.8, 1 x 512 16.8 and 20.2, 1 x 1024 against 16384 8.8 and 8.0, 4000 5.1 and 7.1, 96421 26.8 and 21.4; 8 x 512
-// against 4000 6.5 and 7.5, 8 x 1024 8.7 and 7.4; and from the host a launch less).  SHARE: as above, else every wave has TILES of its own, which
-// starts fewer workgroups where b has many short rows (8 rows, us: 50000 x 256 12.4 and 9.1, 96421 x 64 10.0 and 7.4, x 768 20.2 and 21.2; 16384 x 512 5.8 and 10.2).
-constexpr int kFewRows = 8;
-constexpr int64_t kFusedValues = 4096, kFusedDepth = 512, kFusedShort = 16384;
-
+// The same for a few short rows in floating point (i8_quantises_on_the_way): every workgroup makes them 8-bit on the way, with the quantiser's own
+// steps, and lays them out in LDS in the order the lanes read them: [16 codes of depth][row][16 bytes], rows rounded up to a power of two (lanes past
+// them read another row's bytes; what they compute is not stored).  No launch, no buffer.  SHARE: as above, else every wave has TILES of its own.
 struct FewArgs {
     GemmArgs g;
     const void *x;                                               // the rows of a in floating point, ldx apart
@@ -628,17 +619,12 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
     }
 }
 
-static bool quantises_on_the_way(int64_t m, int64_t n, int64_t k)
-{
-    return m <= kFewRows && m * k <= kFusedValues && k <= (n <= kFusedShort ? 2 * kFusedDepth : kFusedDepth);
-}
-
 template <typename X> static int few_rows(FewArgs F, hipStream_t st)
 {
     const int64_t steps = (F.g.k + kStep - 1) / kStep, tiles = (F.g.n + 15) / 16;
     F.shift = 0;
     while ((1 << F.shift) < F.g.m) ++F.shift;
-    const bool share = tiles <= 2048;                            // (more have at most 8 steps: quantises_on_the_way)
+    const bool share = i8_shares_depth(F.g.n);
     constexpr int kOwn = 4;
     const int64_t per = share ? 1 : 4 * kOwn, groups = (tiles + per - 1) / per;
     // a workgroup that lays the rows of a out once and walks several groups with them: as many as keep 2 048 workgroups busy
@@ -652,57 +638,32 @@ template <typename X> static int few_rows(FewArgs F, hipStream_t st)
     return launch_status();
 }
 
-// Where rows stream and are not put together to tiles (us, streamed and in tiles): 8 rows unless b has many short ones (16384 x 512 5.3 and 5.2,
-// 28672 x 512 8.0 and 7.0, 65536 x 64 5.8 and 5.0, x 1024 14.7 and 16.3, 16384 x 8192 27 and 32); more where 256 workgroups do, one for each CU, which 64 x 64 tiles
-// would not fill (16 rows: 4096 x 4096 7.0 and 11.0, 8192 x 8192 15.0 and 18.1, 11008 x 8192 26.6 and 21.6; 32: 4096 x 4096 9.1 and 11.2, 8192 x 4096 14.2 and 11.5; 256 x
-// 512 x 8192 13.5 and 18.3, 512 x 512 x 8192 24.3 and 17.7, 189 x 48 x 5391 9.1 and 20.9).
-static int64_t up(int64_t n, int64_t by) { return (n + by - 1) / by; }
-static bool streams(const GemmArgs &G)
-{
-    if (G.m <= 8) return G.k > 11 * kStep || G.n <= 24576;
-    if (G.m <= 16) return G.n <= 8192;
-    return up(G.m, 32) * up(G.n, 16) <= 256;
-}
-static int stream_few(const GemmArgs &G, hipStream_t st)
-{
-    // 32 rows of a a workgroup where 16 would need more than one a CU (64 x 2048 x 4096 8.3 us, 16 rows 10.0; 33 x 1000 x 8192 13.7 and 10.4)
-    if (G.m > 16) return up(G.m, 16) * up(G.n, 16) <= 256 ? stream<1, 1>(G, st) : stream<2, 1>(G, st);
-    // two tiles a workgroup halve the reads of a where there is a workgroup for every CU all the same (16 rows against 8192 x 8192: 15.0 us, one tile 17.2;
-    // 4096 x 8192 14.1 and 10.7; 1 row against 28672 x 8192 46 and 41)
-    return G.m > 4 && G.n > 4096 && G.k >= 2048 ? stream<1, 2>(G, st) : stream<1, 1>(G, st);
-}
-
 static int product(const GemmArgs &G, hipStream_t st)
 {
-    if (streams(G)) return stream_few(G, st);
-    if (G.lda > kMostApart || G.ldb > kMostApart) {              // rows megabytes apart, in whatever number
-        constexpr int64_t kMost = 65535 * 32;                    // of a in a launch
-        const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
-        for (int64_t at = 0; at < G.m; at += kMost) {
-            GemmArgs Q = G;
-            Q.a += at * G.lda;
-            Q.sa += at;
-            Q.y = static_cast<char *>(G.y) + at * G.ldy * size;
-            Q.m = G.m - at < kMost ? G.m - at : kMost;
-            const int rc = stream<2, 1>(Q, st);
-            if (rc != IGCN_OK) return rc;
-        }
-        return IGCN_OK;
+    switch (i8_way(G.m, G.n, G.k, G.lda, G.ldb, G.out == IGCN_DTYPE_F32)) {
+    case I8Way::kStream: return stream<1, 1>(G, st);
+    case I8Way::kStreamTwoTiles: return stream<1, 2>(G, st);
+    case I8Way::kStreamTwoGroups: return stream<2, 1>(G, st);
+    case I8Way::kTiles64x128: return tiles_launch<64, 128, 2, 4, 2>(G, st);
+    case I8Way::kTiles256: return tiles_launch<256, 256, 2, 4, 2>(G, st);
+    case I8Way::kTiles128Deep: return tiles_launch<128, 128, 2, 4, 3>(G, st);
+    case I8Way::kTiles128: return tiles_launch<128, 128, 2, 4, 2>(G, st);
+    case I8Way::kTiles64ByDepth: return tiles_launch<64, 64, 2, 2, 4, true>(G, st);
+    case I8Way::kTiles64: return tiles_launch<64, 64, 2, 2, 4>(G, st);
+    case I8Way::kApart: break;
     }
-    auto tiles = [&](int64_t tm, int64_t tn) { return ((G.m + tm - 1) / tm) * ((G.n + tn - 1) / tn); };
-    // The largest tile that still makes nearly a workgroup for each of 256 CUs: 256 x 256 reads each code half as often as 128 x 128 (8192 x 8192 x
-    // 4096: 258 against 298 us), which with 64 tiles would leave three of four CUs idle (512 x 8192 x 8192: 90 against 47 us; 64 x 64: 57).
-    // One stage of depth: writing y is all there is, and many small waves hide it best (512 x 96421 x 64 to float32: 48 us; 128 x 128 57,
-    // 256 x 256 55; to bfloat16 128 x 128 30, 64 x 128 38).
-    if (G.m > 64) {
-        if (G.k <= kDepth && G.out == IGCN_DTYPE_F32) return tiles_launch<64, 128, 2, 4, 2>(G, st);
-        if (G.k > kDepth && tiles(256, 256) >= 200) return tiles_launch<256, 256, 2, 4, 2>(G, st);
-        // eight waves, two to a SIMD, one reading LDS while the other multiplies (512 x 8192 x 512 6.9 us, four waves 8.1; x 4096 27 and 28); a third stage
-        // where a CU has one workgroup anyway and the depth pays for it (256 x 16384 x 8192 56 and 68, x 1024 10.4 and 10.3; 3000 x 3000 x 4096 69 and 58)
-        const int64_t middle = tiles(128, 128);
-        if (middle >= 200) return middle <= 256 && G.k >= 2048 ? tiles_launch<128, 128, 2, 4, 3>(G, st) : tiles_launch<128, 128, 2, 4, 2>(G, st);
+    constexpr int64_t kMost = 65535 * 32;                        // rows of a in a launch
+    const int64_t size = G.out == IGCN_DTYPE_F32 ? 4 : 2;
+    for (int64_t at = 0; at < G.m; at += kMost) {
+        GemmArgs Q = G;
+        Q.a += at * G.lda;
+        Q.sa += at;
+        Q.y = static_cast<char *>(G.y) + at * G.ldy * size;
+        Q.m = G.m - at < kMost ? G.m - at : kMost;
+        const int rc = stream<2, 1>(Q, st);
+        if (rc != IGCN_OK) return rc;
     }
-    return G.k >= 512 ? tiles_launch<64, 64, 2, 2, 4, true>(G, st) : tiles_launch<64, 64, 2, 2, 4>(G, st);
+    return IGCN_OK;
 }
 
 static int check_product(const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias, int64_t m, int64_t n, int64_t k, const void *y,
@@ -738,7 +699,7 @@ extern "C" int igcn_matmul_i8(const int8_t *a, int64_t lda, const float *sa, con
 extern "C" int64_t igcn_linear_i8_workspace_bytes(int64_t m, int64_t k)
 {
     if (m < 0 || k < 0 || k > IGCN_MAX_I8_DEPTH || m > 0x7fffffff) return -1;
-    return quantises_on_the_way(m, INT64_MAX, k) ? 0 : up16(m * up16(k)) + 4 * m;
+    return i8_quantises_on_the_way(m, INT64_MAX, k) ? 0 : up16(m * up16(k)) + 4 * m;
 }
 
 extern "C" int igcn_linear_i8(const void *x, int32_t x_dtype, int64_t ldx, const int8_t *b, int64_t ldb, const float *sb, const float *bias,
@@ -753,7 +714,7 @@ extern "C" int igcn_linear_i8(const void *x, int32_t x_dtype, int64_t ldx, const
     if (misaligned(x, x_dtype)) return IGCN_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
     GemmArgs G = {nullptr, b, nullptr, sb, bias, y, 0, ldb, ldy, m, n, k, dtype};
-    if (quantises_on_the_way(m, n, k)) {
+    if (i8_quantises_on_the_way(m, n, k)) {
         FewArgs F = {};
         F.g = G;
         F.x = x;

@@ -292,3 +292,76 @@ def test_quantised_values_past_32_bits():
     assert torch.equal(q[-40:], want_q) and torch.equal(s[-40:], want_s) and not bool(s[:-40].any()) and not bool(q[-80:-40].any())
     y = ops.dequantize_rows_i8(q, s, dtype=torch.float16)
     assert torch.equal(y[-40:], (want_q.float() * want_s[:, None]).half()) and not bool(y[-80:-40].any())
+
+
+# Sizes at which the rule of csrc/gemm_i8_rule.h goes to its larger kernels (test_operators_cpu asks it whether every one is met): partial last tiles and
+# stages, rows on and off 16-byte multiples.
+TILE_SIZES = [(3600, 3600, 272), (3600, 3600, 259), (4000, 3400, 131), (513, 1029, 999), (27, 20956, 1381), (300, 700, 2051), (64, 4096, 2053), (300, 700, 2049),
+              (65, 8200, 2064), (2000, 2000, 4099), (700, 4200, 333), (1030, 3300, 1040), (100, 30000, 48), (70, 40000, 13), (9, 30000, 7), (40, 30000, 15), (40, 12000, 2500), (64, 1200, 9)]
+
+
+@pytest.mark.parametrize('m,n,k', TILE_SIZES)
+def test_products_in_the_larger_tiles(m, n, k):
+    g = _rng(m * 31 + n * 7 + k)
+    a, b = _codes((m, k), g), _codes((n, k), g)
+    sa, sb = torch.exp(torch.randn(m, device=DEV, generator=g) - 5), torch.exp(torch.randn(n, device=DEV, generator=g) - 5)
+    bias = torch.randn(n, device=DEV, generator=g)
+    for dtype in (torch.float32, torch.bfloat16):
+        check(a, sa, b, sb, bias if dtype == torch.bfloat16 else None, dtype)
+
+
+def test_rows_of_tiles_apart_and_off_alignment():
+    """As test_rows_apart_and_off_alignment, at sizes that go through LDS: rows that start at any byte, every third row, a depth of one stage, of several and
+    of a few codes."""
+    g = _rng(21)
+    ca, cb = _codes((900, 2200), g), _codes((2110, 2230), g)
+    sa, sb = torch.rand(900, device=DEV, generator=g), torch.rand(2110, device=DEV, generator=g)
+    for off in (0, 1, 2, 3, 4, 8, 15):
+        for k in (1, 15, 16, 31, 64, 100, 129, 256, 380, 600, 2100):
+            for step in (1, 3):
+                a, b = ca[:300 * step:step, off:off + k], cb[off % 3:off % 3 + 700 * step:step, 2 * off:2 * off + k]
+                check(a, sa[:300], b, sb[:700], dtype=torch.bfloat16 if off % 2 else torch.float32)
+
+
+APART_SIZES = [(150, 2000, (1 << 23) + 48, None), (150, 2000, (1 << 23) + 49, None), (2000, 150, None, (1 << 23) + 48), (2000, 150, None, (1 << 23) + 51)]
+
+
+@pytest.mark.parametrize('m,n,lda,ldb', APART_SIZES)
+def test_more_rows_megabytes_apart_than_stream(m, n, lda, ldb):
+    """Leading dimensions over 2^23 where the size asks for tiles: offsets within one would pass 31 bits."""
+    from igcn_cf_amd import ops
+    g, k = _rng(m), 100
+    a, b = _codes((m, k), g), _codes((n, k), g)
+    sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+
+    def spread(t, ld):
+        if ld is None:
+            return t
+        rows = torch.empty((t.shape[0] - 1) * ld + k, dtype=torch.int8, device=DEV).as_strided(t.shape, (ld, 1))
+        return rows.copy_(t)
+    y = check(spread(a, lda), sa, spread(b, ldb), sb)
+    assert torch.equal(y, ops.matmul_i8(a, sa, b, sb))
+
+
+def test_more_rows_than_a_launch_against_two_megabytes_apart():
+    """65535 x 32 rows of a are what one launch is given there."""
+    g, m, k, ld = _rng(23), 65535 * 32 + 2900, 16, (1 << 23) + 16
+    a, b = _codes((m, k), g), torch.empty(ld + k, dtype=torch.int8, device=DEV).as_strided((2, k), (ld, 1))
+    b.copy_(_codes((2, k), g))
+    sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(2, device=DEV, generator=g)
+    check(a, sa, b, sb, dtype=torch.float16)
+
+
+# (m, n, k, type of x, bytes between rows of b past k): the products that quantise on their way, each kernel of them
+FEW_SIZES = [(m, n, k, dtype, past) for dtype in DTYPES for m, n, k, past in
+             ((1, 33, 64, 0), (3, 1000, 130, 0), (8, 500, 77, 0), (2, 1024, 12, 2), (5, 40001, 64, 0), (8, 33000, 200, 1), (1, 50000, 13, 0), (7, 70000, 9, 3))]
+
+
+@pytest.mark.parametrize('m,n,k,dtype,past', FEW_SIZES)
+def test_a_few_short_rows_of_every_type(m, n, k, dtype, past):
+    from igcn_cf_amd import ops
+    g = _rng(m + n + k)
+    x = torch.randn(m, k, device=DEV, generator=g).to(dtype)
+    b, sb = _codes((n, k + past), g)[:, :k], torch.rand(n, device=DEV, generator=g)
+    q, s = _quantized(x)
+    assert torch.equal(ops.linear_i8(x, b, sb, dtype=torch.float32), check(q, s, b, sb))

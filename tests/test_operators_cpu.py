@@ -281,3 +281,47 @@ def test_a_captured_steps_key_names_the_memory_the_optimizer_writes(make):
     if isinstance(trainer.opt, AdamW):
         trainer.opt.state.clear()
         assert trainer._graph_key() != after
+
+
+def test_the_gpu_tests_reach_every_kernel_of_the_8_bit_product(tmp_path):
+    """The rule that chooses among them (csrc/gemm_i8_rule.h, plain C++) is compiled here and asked about every size of the GPU tests: each kernel has to
+    come up in each of its forms — tiles from rows on and off 16-byte multiples, streams of rows on and off 4-byte ones, rows of fewer than 16 codes."""
+    import os
+    import re
+    import subprocess
+    from tests import test_i8_gpu as G
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'igcn_cf_amd', 'csrc')
+    names = re.search(r'enum class I8Way \{(.*?)\};', open(os.path.join(csrc, 'gemm_i8_rule.h')).read(), re.S).group(1)
+    names = re.findall(r'\bk\w+', re.sub(r'//.*', '', names))
+    (tmp_path / 'ask.cpp').write_text('''
+#include "gemm_i8_rule.h"
+#include <cstdio>
+using namespace igcn;
+int main()
+{
+    long long m, n, k, lda, ldb, at;
+    int f32;
+    while (scanf("%lld %lld %lld %lld %lld %lld %d", &m, &n, &k, &lda, &ldb, &at, &f32) == 7)
+        printf("%d %d %d %d %d\\n", (int)i8_way(m, n, k, lda, ldb, f32), i8_direct(at, at, lda, ldb, k), i8_any_byte(at, lda) || i8_any_byte(at, ldb),
+               i8_quantises_on_the_way(m, n, k), i8_shares_depth(n));
+}
+''')
+    subprocess.run(['g++', '-std=c++17', '-O1', '-Wall', '-Werror', '-I', csrc, str(tmp_path / 'ask.cpp'), '-o', str(tmp_path / 'ask')], check=True)
+
+    def ask(rows):
+        got = subprocess.run([str(tmp_path / 'ask')], input='\n'.join(' '.join(map(str, r)) for r in rows), check=True, stdout=subprocess.PIPE, text=True).stdout
+        return [[int(x) for x in line.split()] for line in got.splitlines()]
+    sizes = [s for s in G.SIZES + G.TILE_SIZES if min(s) > 0]
+    rows = [(m, n, k, k, k, 0, f32) for m, n, k in sizes for f32 in (0, 1)]
+    rows += [(300, 700, k, 2200 * step, 2230 * step, off, f32) for off in (0, 1) for k in (1, 15, 64, 380, 2100) for step in (1, 3) for f32 in (0, 1)]
+    rows += [(m, n, 100, lda or 100, ldb or 100, 0, 1) for m, n, lda, ldb in G.APART_SIZES]
+    met = set()
+    for (m, n, k, *_), (way, direct, byte, _, _) in zip(rows, ask(rows)):
+        name = names[way]
+        met.add((name, 'short') if k < 16 else (name, direct) if 'Tiles' in name and 'Stream' not in name else (name, byte))
+    want = {(name, form) for name in names for form in (0, 1)}
+    assert len(names) == 10 and want <= met, sorted(want - met)
+    assert {name for name, form in met if form == 'short'} >= {'kStream', 'kStreamTwoGroups', 'kTiles64x128', 'kTiles128', 'kTiles64'}
+    few = [(m, n, k, k, k + past, 0, 1) for m, n, k, _, past in G.FEW_SIZES]
+    met = {(shares, byte, k < 16, dtype) for (m, n, k, dtype, _), (_, _, byte, fused, shares) in zip(G.FEW_SIZES, ask(few)) if fused}
+    assert {(s, b, t) for s, b, _, t in met} == {(s, b, t) for s in (0, 1) for b in (0, 1) for t in G.DTYPES} and {s for s, _, short, _ in met if short} == {0, 1}
