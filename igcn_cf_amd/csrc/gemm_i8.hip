@@ -74,8 +74,9 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int k, i
 // Bound by the matrix cores (deep sums) or by writing y (shallow ones).  A workgroup makes a TM x TN tile of y, a wave TM / WM x TN / WN of it in
 // 32 x 32 pieces (v_mfma_i32_32x32x32_i8: lane l holds row l % 32, 16 bytes of depth at 16 (l / 32)).  128 codes of depth of either side
 // go to LDS per stage, two stages in turn: the next one is on its way from memory while this one is multiplied, one barrier a stage.
-// DIRECT (rows 16-byte aligned, depth a multiple of 16): memory to LDS without registers (global_load_lds, 1 KiB a wave and
-// instruction, lane after lane); else through registers, AHEAD stages of them under way (13 x 5466 x 1917: 10.9 us; one: 18.1).  A row's eight 16-byte pieces stand in LDS at piece ^ (row / 2 % 8): 16 lanes that read the
+// DIRECT (rows 16-byte aligned, depth a multiple of 16): memory to LDS without registers (global_load_lds, 1 KiB a wave and instruction,
+// lane after lane); else through registers, one stage under way there (300 x 700 x 333 4.9 us, 300 x 700 x 2051 10.6, 512 x 8192 x 4095 37.1;
+// with up to three under way 5.5, 11.2, 36.4).  A row's eight 16-byte pieces stand in LDS at piece ^ (row / 2 % 8): 16 lanes that read the
 // same piece of 16 neighbouring rows hit 64 different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
 // Depth past the end reads a block of zeros, rows past the end the last row (not stored).
 // BY_DEPTH (a 64 x 64 tile of four waves): a wave takes a quarter of the stage's depth for the whole tile instead of all of it for its own piece,
@@ -112,7 +113,6 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     constexpr int kWaves = WM * WN, RT = TM / WM / 32, CT = TN / WN / 32, NA = TM / 8 / kWaves, NB = TN / 8 / kWaves;
     constexpr int kStage = (TM + TN) * kDepth;
     static_assert(!BY_DEPTH || (RT == 1 && CT == 1 && kWaves == kDepth / 32), "a quarter of the depth for each of four waves");
-    constexpr int AHEAD = TM <= 64 ? 3 : TM <= 128 ? 2 : 1;      // stages on their way in registers, where they go that way
     constexpr int AR = BY_DEPTH ? WM : RT, AC = BY_DEPTH ? WN : CT;       // pieces whose sums a wave holds
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     unsigned char *const ring = smem + (TM + 2 * TN) * 4;       // the stages; behind them, the strips of the way out
@@ -135,11 +135,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
     for (int i = 0; i < NB; ++i) ob[i] = (unsigned)min(8 * (wave * NB + i) + (lane >> 3), last_b) * (unsigned)G.ldb + piece(wave * NB + i);
     const int64_t stages = (G.k + kDepth - 1) / kDepth;
-    i32x4 held[DIRECT ? 1 : AHEAD][DIRECT ? 1 : NA + NB];
+    i32x4 held[DIRECT ? 1 : NA + NB];                            // the stage on its way in registers, where it goes that way
     const unsigned lds0 = (unsigned)(uintptr_t)(lds_void *)ring;
 
     const int k = (int)G.k;
-    auto fetch = [&](int64_t s, auto &h) {                       // stage s of both sides: on its way to LDS, or to registers
+    auto fetch = [&](int64_t s) {                                // stage s of both sides: on its way to LDS, or to registers
         const int k0 = (int)s * kDepth;
         if constexpr (DIRECT) {
             const unsigned at = lds0 + (unsigned)(s % STAGES) * kStage + wave * NA * 1024, bt = at + TM * kDepth + wave * (NB - NA) * 1024;
@@ -156,24 +156,24 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
             }
         } else {                                                 // (past the end: the row's last 16 codes, put in place by land())
 #pragma unroll
-            for (int i = 0; i < NA; ++i) h[i] = load16(base_a + (oa[i] - piece(wave * NA + i)) + min(k0 + piece(wave * NA + i), k - 16));
+            for (int i = 0; i < NA; ++i) held[i] = load16(base_a + (oa[i] - piece(wave * NA + i)) + min(k0 + piece(wave * NA + i), k - 16));
 #pragma unroll
-            for (int i = 0; i < NB; ++i) h[NA + i] = load16(base_b + (ob[i] - piece(wave * NB + i)) + min(k0 + piece(wave * NB + i), k - 16));
+            for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + (ob[i] - piece(wave * NB + i)) + min(k0 + piece(wave * NB + i), k - 16));
         }
     };
-    auto land = [&](int64_t s, auto &h) {                        // registers to LDS
+    auto land = [&](int64_t s) {                                 // registers to LDS
         i32x4 *at = reinterpret_cast<i32x4 *>(ring + (s % STAGES) * kStage);
         const int k0 = (int)s * kDepth;
         if (k0 + kDepth > k && k >= 16) {
 #pragma unroll
-            for (int i = 0; i < NA; ++i) h[i] = behind(h[i], max(k0 + piece(wave * NA + i) - (k - 16), 0));
+            for (int i = 0; i < NA; ++i) held[i] = behind(held[i], max(k0 + piece(wave * NA + i) - (k - 16), 0));
 #pragma unroll
-            for (int i = 0; i < NB; ++i) h[NA + i] = behind(h[NA + i], max(k0 + piece(wave * NB + i) - (k - 16), 0));
+            for (int i = 0; i < NB; ++i) held[NA + i] = behind(held[NA + i], max(k0 + piece(wave * NB + i) - (k - 16), 0));
         }
 #pragma unroll
-        for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = h[i];
+        for (int i = 0; i < NA; ++i) at[(wave * NA + i) * 64 + lane] = held[i];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = h[NA + i];
+        for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
     };
 
     // One stage: every tile starts with reads that queue behind the writes of y.  The first row of tiles asks for the rows of b of kSoon tiles on
@@ -195,21 +195,19 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         fc[i] = G.bias && i <= last_b ? G.bias[n0 + i] : 0.f;
     }
     if constexpr (DIRECT) {
-        for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s, held[0]);
+        for (int64_t s = 0; s < STAGES - 1 && s < stages; ++s) fetch(s);
     } else if (k >= 16) {
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d)
-            if (d < stages) fetch(d, held[d]);
-        land(0, held[0]);
-        if (AHEAD < stages) fetch(AHEAD, held[0]);
+        fetch(0);
+        land(0);
+        if (1 < stages) fetch(1);
     } else if (k > 0) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) held[0][i] = load16(base_a + (oa[i] - piece(wave * NA + i)), piece(wave * NA + i), k);
+        for (int i = 0; i < NA; ++i) held[i] = load16(base_a + (oa[i] - piece(wave * NA + i)), piece(wave * NA + i), k);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) held[0][NA + i] = load16(base_b + (ob[i] - piece(wave * NB + i)), piece(wave * NB + i), k);
-        land(0, held[0]);
+        for (int i = 0; i < NB; ++i) held[NA + i] = load16(base_b + (ob[i] - piece(wave * NB + i)), piece(wave * NB + i), k);
+        land(0);
     }
-    auto stage = [&](int64_t s, auto &h) {
+    auto stage = [&](int64_t s) {
         if constexpr (DIRECT) {                                  // stage s is there: all but the STAGES - 2 behind it
             if (s + STAGES - 2 < stages) wait_for_lds<(STAGES - 2) * (NA + NB)>(); else wait_for_lds<0>();
         }
@@ -224,7 +222,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
             for (int c = 0; c < AC; ++c) bv[c] = *reinterpret_cast<const i32x4 *>(sb + c * 32 * kDepth + at);
         };
         read(BY_DEPTH ? wave : 0);                               // (before the next stage is sent for: its addresses take a while)
-        if constexpr (DIRECT) if (s + STAGES - 1 < stages) fetch(s + STAGES - 1, h);
+        if constexpr (DIRECT) if (s + STAGES - 1 < stages) fetch(s + STAGES - 1);
 #pragma unroll
         for (int j = 0; j < (BY_DEPTH ? 1 : kDepth / 32); ++j) {
             if (j) read(j);
@@ -234,16 +232,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
                 for (int c = 0; c < AC; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[c], av[r], acc[r][c], 0, 0, 0);
         }
         if constexpr (!DIRECT) if (s + 1 < stages) {
-            land(s + 1, h);
-            if (s + 1 + AHEAD < stages) fetch(s + 1 + AHEAD, h);
+            land(s + 1);
+            if (s + 2 < stages) fetch(s + 2);
         }
     };
-    if constexpr (DIRECT) for (int64_t s = 0; s < stages; ++s) stage(s, held[0]);
-    else for (int64_t s = 0; s < stages; s += AHEAD) {
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d)
-            if (s + d < stages) stage(s + d, held[(d + 1) % AHEAD]);
-    }
+    for (int64_t s = 0; s < stages; ++s) stage(s);
     __syncthreads();
     if constexpr (BY_DEPTH) {                                    // piece q of the tile goes to wave q: [piece][the three other waves][4 sums a lane and quarter]
         i32x4 *const sums = reinterpret_cast<i32x4 *>(ring);
