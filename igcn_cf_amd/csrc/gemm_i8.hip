@@ -80,8 +80,7 @@ __device__ __forceinline__ i32x4 load16(const int8_t *__restrict__ row, int k, i
 // same piece of 16 neighbouring rows hit 64 different banks; memory-to-LDS writes linearly, so it is the lane's source that is permuted.
 // Depth past the end reads a block of zeros, rows past the end the last row (not stored).
 // BY_DEPTH (a 64 x 64 tile of four waves): a wave takes a quarter of the stage's depth for the whole tile instead of all of it for its own piece,
-// and they exchange sums in the end: LDS is read half as often and no product waits for the one before it (64 x 1000 x 8192: 23.6 -> 18.1 us;
-// 64 x 96421 x 64: 8.2 -> 11.4, so only where the depth pays for the exchange).
+// and they exchange sums in the end: LDS is read half as often and no product waits for the one before it.
 // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, 4 tiles of a deep at a time, so that the tiles under way there
 // share their rows in its L2 (512 x 96421 x 64, whose rows of y end inside a line, without: 47 -> 74 us).
 __device__ const i32x4 g_zeros = {0, 0, 0, 0};

@@ -51,7 +51,10 @@ inline I8Way i8_way(int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, b
         const int64_t middle = pieces(m, 128) * pieces(n, 128);
         if (middle >= 200) return middle <= 256 && k >= 2048 ? I8Way::kTiles128Deep : I8Way::kTiles128;
     }
-    return k >= 512 ? I8Way::kTiles64ByDepth : I8Way::kTiles64;
+    // Waves that share the depth of a 64 x 64 tile pay where a CU has one workgroup, which waits for its own products, and the depth is worth the exchange
+    // (300 x 700 x 2048 7.7 / 8.5, x 4096 11.2 / 13.5, x 1024 6.1 / 6.1, x 512 5.2 / 4.8; 180 x 3000 x 2048 7.9 / 8.6, x 8192 18.7 / 23.3; more tiles: 64 x 16384 x
+    // 2048 9.1 / 9.6, x 4096 14.9 / 14.7, 40 x 30000 x 2048 14.0 / 13.6; b not in a cache: 64 x 12000 x 2048 10.6 / 10.2, x 8192 26.2 / 26.7).
+    return k >= 2048 && pieces(m, 64) * pieces(n, 64) <= 200 ? I8Way::kTiles64ByDepth : I8Way::kTiles64;
 }
 
 // Rows that start at, and are apart by, multiples of 16 bytes, a depth of whole 16-byte pieces: memory to LDS without registers
