@@ -102,7 +102,7 @@ __device__ __forceinline__ void to_lds(const void *p, unsigned lds)
 #pragma clang diagnostic pop
 template <int LEFT> __device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory"); }      // all but the last LEFT are there
 
-struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; };
+struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; bool asks_ahead; };
 
 constexpr size_t kExchanged = 3 * 4 * 4096;                      // of LDS: three waves' sums of four pieces
 
@@ -175,14 +175,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
     };
 
-    // One stage: every tile starts with reads that queue behind the writes of y.  The first row of tiles asks for the rows of b of kSoon tiles on
-    // (twice what an XCD has under way), so that those find them in a cache (512 x 96421 x 64, b not there before: 60 us, this way 55; to bfloat16 35 and 32).
+    // Where every tile starts with reads that queue behind the writes of y (i8_asks_ahead): the first row of tiles of a band asks for the rows of b of kSoon
+    // tiles on, twice what an XCD has under way, so that those find them in a cache.
     constexpr int kSoon = 64;
     i32x4 soon = {0, 0, 0, 0};
     if constexpr (DIRECT && !BY_DEPTH && TM < 256) {
         static_assert(64 * kWaves == 4 * TN, "four lanes a row");
         const int64_t r = n0 + kSoon * TN + threadIdx.x / 4;
-        if (stages == 1 && in % high == 0 && r < G.n) soon = load16(G.b + r * G.ldb + ((threadIdx.x & 3) * k / 4 & ~15));
+        if (T.asks_ahead && in % high == 0 && r < G.n) soon = load16(G.b + r * G.ldb + ((threadIdx.x & 3) * k / 4 & ~15));
     }
     i32x16 acc[AR][AC] = {};
     const int wm = wave / WN, wn = wave % WN;
@@ -318,6 +318,7 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
     constexpr int64_t kMostTiles = ((int64_t)1 << 32) / (64 * WM * WN) - 8;      // a launch has fewer than 2^32 threads
     if (T.tiles_m > kMostTiles / T.tiles_n) return IGCN_E_SHAPE;
     T.per_xcd = (T.tiles_m * T.tiles_n + 7) / 8;
+    T.asks_ahead = i8_asks_ahead(G.m, G.n, G.k, G.out == IGCN_DTYPE_F32);
     const bool direct = i8_direct(reinterpret_cast<uintptr_t>(G.a), reinterpret_cast<uintptr_t>(G.b), G.lda, G.ldb, G.k);
     auto launch = [&](auto *kernel, int most) {
         int64_t stages = (G.k + kDepth - 1) / kDepth;

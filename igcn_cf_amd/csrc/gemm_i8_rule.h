@@ -57,6 +57,12 @@ inline I8Way i8_way(int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, b
     return k >= 2048 && pieces(m, 64) * pieces(n, 64) <= 200 ? I8Way::kTiles64ByDepth : I8Way::kTiles64;
 }
 
+// One stage of depth and 32 MB of y and more, more than the L2s hold: a tile's reads of b then queue behind the writes of y, and the first row of tiles
+// asks for later rows of b ahead (asked / not; b not in a cache, then there.  To float32: 128 x 96421 x 64, 49 MB of y, 14.4 / 16.9, 13.1 / 12.6; 512 x 96421 x 64
+// 46 / 53, 38 / 36; 2048 x 96421 x 64 191 / 211, 191 / 214.  To bfloat16: 200 x 96421 x 64, 39 MB, 15.5 / 17.2, 14.5 / 14.0; 512 x 96421 x 64 30 / 33, 27 / 27.
+// Smaller ones: 64 x 96421 x 128 to float32, 25 MB, 10.9 / 11.0, 9.2 / 9.1, to bfloat16 9.5 / 8.4, 7.9 / 7.4; 9 x 20956 x 128 4.8 / 4.0, 4.1 / 4.1).
+inline bool i8_asks_ahead(int64_t m, int64_t n, int64_t k, bool out_f32) { return k > 0 && k <= kDepth && m * n >= (out_f32 ? 1 << 23 : 1 << 24); }
+
 // Rows that start at, and are apart by, multiples of 16 bytes, a depth of whole 16-byte pieces: memory to LDS without registers
 inline bool i8_direct(uintptr_t a, uintptr_t b, int64_t lda, int64_t ldb, int64_t k) { return ((a | b | (uintptr_t)lda | (uintptr_t)ldb | (uintptr_t)k) & 15) == 0; }
 inline bool i8_any_byte(uintptr_t p, int64_t ld) { return ((p | (uintptr_t)ld) & 3) != 0; }

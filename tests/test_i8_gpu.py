@@ -297,7 +297,8 @@ def test_quantised_values_past_32_bits():
 # Sizes at which the rule of csrc/gemm_i8_rule.h goes to its larger kernels (test_operators_cpu asks it whether every one is met): partial last tiles and
 # stages, rows on and off 16-byte multiples.
 TILE_SIZES = [(3600, 3600, 272), (3600, 3600, 259), (4000, 3400, 131), (513, 1029, 999), (27, 20956, 1381), (300, 700, 2051), (64, 4096, 2053), (300, 700, 2049),
-              (65, 8200, 2064), (2000, 2000, 4099), (700, 4200, 333), (1030, 3300, 1040), (100, 30000, 48), (70, 40000, 13), (9, 30000, 7), (40, 30000, 15), (40, 12000, 2500), (64, 1200, 9)]
+              (65, 8200, 2064), (2000, 2000, 4099), (700, 4200, 333), (1030, 3300, 1040), (100, 30000, 48), (70, 40000, 13), (9, 30000, 7), (40, 30000, 15), (40, 12000, 2500), (64, 1200, 9), (128, 96421, 64),
+              (300, 60001, 112), (33, 530001, 16)]
 
 
 @pytest.mark.parametrize('m,n,k', TILE_SIZES)

@@ -302,8 +302,9 @@ int main()
     long long m, n, k, lda, ldb, at;
     int f32;
     while (scanf("%lld %lld %lld %lld %lld %lld %d", &m, &n, &k, &lda, &ldb, &at, &f32) == 7)
-        printf("%d %d %d %d %d\\n", (int)i8_way(m, n, k, lda, ldb, f32), i8_direct(at, at, lda, ldb, k), i8_any_byte(at, lda) || i8_any_byte(at, ldb),
-               i8_quantises_on_the_way(m, n, k), i8_shares_depth(n));
+        printf("%d %d %d %d %d %d\\n", (int)i8_way(m, n, k, lda, ldb, f32), i8_direct(at, at, lda, ldb, k), i8_any_byte(at, lda) || i8_any_byte(at, ldb),
+               i8_quantises_on_the_way(m, n, k), i8_shares_depth(n),
+               i8_asks_ahead(m, n, k, f32));
 }
 ''')
     subprocess.run(['g++', '-std=c++17', '-O1', '-Wall', '-Werror', '-I', csrc, str(tmp_path / 'ask.cpp'), '-o', str(tmp_path / 'ask')], check=True)
@@ -315,13 +316,15 @@ int main()
     rows = [(m, n, k, k, k, 0, f32) for m, n, k in sizes for f32 in (0, 1)]
     rows += [(300, 700, k, 2200 * step, 2230 * step, off, f32) for off in (0, 1) for k in (1, 15, 64, 380, 2100) for step in (1, 3) for f32 in (0, 1)]
     rows += [(m, n, 100, lda or 100, ldb or 100, 0, 1) for m, n, lda, ldb in G.APART_SIZES]
-    met = set()
-    for (m, n, k, *_), (way, direct, byte, _, _) in zip(rows, ask(rows)):
+    met, ahead = set(), set()
+    for (m, n, k, *_), (way, direct, byte, _, _, asks) in zip(rows, ask(rows)):
         name = names[way]
+        ahead |= {(name, asks)} if direct else set()
         met.add((name, 'short') if k < 16 else (name, direct) if 'Tiles' in name and 'Stream' not in name else (name, byte))
     want = {(name, form) for name in names for form in (0, 1)}
     assert len(names) == 10 and want <= met, sorted(want - met)
     assert {name for name, form in met if form == 'short'} >= {'kStream', 'kStreamTwoGroups', 'kTiles64x128', 'kTiles128', 'kTiles64'}
+    assert ahead >= {(name, asks) for name in ('kTiles64x128', 'kTiles128', 'kTiles64') for asks in (0, 1)}
     few = [(m, n, k, k, k + past, 0, 1) for m, n, k, _, past in G.FEW_SIZES]
-    met = {(shares, byte, k < 16, dtype) for (m, n, k, dtype, _), (_, _, byte, fused, shares) in zip(G.FEW_SIZES, ask(few)) if fused}
+    met = {(shares, byte, k < 16, dtype) for (m, n, k, dtype, _), (_, _, byte, fused, shares, _) in zip(G.FEW_SIZES, ask(few)) if fused}
     assert {(s, b, t) for s, b, _, t in met} == {(s, b, t) for s in (0, 1) for b in (0, 1) for t in G.DTYPES} and {s for s, _, short, _ in met if short} == {0, 1}
