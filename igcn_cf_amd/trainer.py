@@ -225,7 +225,8 @@ class BasicTrainer:
                self.batch_size, getattr(m, 'dropout', None), bool(m.training), getattr(self, 'l2_reg', None),
                getattr(self, 'aux_reg', None)]
         for g in opt.param_groups:
-            key.append(float(g['lr']))
+            lr = g['lr']                   # (on the GPU: read by the replays, its address is what is baked in)
+            key.append(('lr', lr.data_ptr()) if torch.is_tensor(lr) and lr.is_cuda else float(lr))
             if isinstance(opt, AdamW):
                 key += [*g['betas'], g['eps'], g['weight_decay']]
             for p in g['params']:

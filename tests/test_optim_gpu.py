@@ -845,3 +845,26 @@ def test_captured_steps_follow_a_state_that_is_loaded_between_them(name, bits):
                      for p in model.parameters()])
     for a, b in zip(*ends):
         assert float((a - b).abs().mean()) <= 1e-2 * float(b.abs().max())
+
+
+def test_a_captured_step_reads_a_device_rate_anew():
+    """A learning rate on the GPU is read by the replays: changing it neither captures again nor waits for the GPU, another tensor in its place does
+    capture.  Rate 0 moves nothing (no decay at that rate either)."""
+    ds, model, trainer = _trainer('MF', True, 32)
+    lr = torch.full((), 1e-2, device=DEV)
+    trainer.opt.param_groups[0]['lr'] = lr
+    model.train()
+    batch = next(iter(trainer.sampler.epoch_node_batches(1024, 0))).clone()
+    trainer.flat_step(batch)
+    first, key = trainer._graph, trainer._graph_key()
+    lr.zero_()
+    assert trainer._graph_key() == key and all(type(k) is not torch.Tensor for k in key)
+    before = [p.detach().clone() for p in model.parameters()]
+    trainer.flat_step(batch)
+    assert trainer._graph is first and all(torch.equal(p, b) for p, b in zip(model.parameters(), before))
+    lr.fill_(1e-2)
+    trainer.flat_step(batch)
+    assert trainer._graph is first and not any(torch.equal(p, b) for p, b in zip(model.parameters(), before))
+    trainer.opt.param_groups[0]['lr'] = torch.full((), 1e-3, device=DEV)
+    trainer.flat_step(batch)
+    assert trainer._graph is not first
