@@ -13,7 +13,8 @@
 // 8-bit moments: blocks of 128 consecutive elements share s_m = max |m| / 448 and s_v = max v / 57344 (float32); m / s_m is held as
 // e4m3, v / s_v as e5m2.  An average that moves by 0.1 % a step would stand still under a code step of 12-25 % rounded to nearest, so
 // the codes are rounded stochastically: code = floor(x + u), u of 16 bits from a hash of (seed, tensor, step, element) — right in the
-// mean, the same on every replay and every machine.  v > 0 is never held as 0 (m / sqrt(0)).  The averages and codes are formed in
+// mean, the same on every replay and every machine (the float32 step count ends at 2^24: from there on every step draws the same u).
+// v > 0 is not held as 0 (m / sqrt(0)) unless it is under 2^-165 of its block's largest.  The averages and codes are formed in
 // float32 with every operation rounded once, in the order written (no fused multiply-add): elementary float32 operations in any other
 // program give the same codes, bit for bit.
 #include "dtypes.h"
@@ -348,10 +349,11 @@ __global__ __launch_bounds__(kBlock) void adamw_step_kernel(const TensorTable T,
 
 // A call of small tensors is its launches: here one does all of it.  A workgroup of kSmallBlock threads per tensor, so that nobody else
 // reads the step it counts; the norm over all tensors, where there is one, every workgroup adds up for itself, in the same order.
-// On the device alone (captured) 4 chunks take 4.4 us this way and 4.3 the other, 12 take 9.3 (float32; 8-bit 6.7 and 6.2, 15.4); from the host a
-// launch less is 2.5 us less.
+// us of a captured call, one launch / two: a tensor of 4 chunks 4.4 / 4.3 (8-bit moments 6.7 / 6.2); of 12 chunks, three rounds of the workgroup,
+// one launch would take 9.3 (15.4).  From the host a launch less is 2.5 us less.
 constexpr int kSmallBlock = 1024;
-constexpr int64_t kSmallChunks = kSmallBlock / kBlock, kSmallNormChunks = 16;        // of a tensor; of the call, where every workgroup reads all gradients
+constexpr int64_t kSmallChunks = kSmallBlock / kBlock;           // of a tensor
+constexpr int64_t kSmallNormChunks = 16;                         // of the call, where every workgroup reads all gradients
 template <int BITS, bool SMALL>
 __global__ __launch_bounds__(kSmallBlock) void adamw_small_kernel(const TensorTable T, const Hyper H, const float *norm_in, float *norm_out)
 {
@@ -482,8 +484,11 @@ extern "C" int64_t igcn_adamw_workspace_bytes(const igcn_adamw_tensor *tensors_h
 {
     if (check_tensors(tensors_host, n_tensors, 0) != IGCN_OK) return -1;
     int64_t partials = 0;
-    if (for_tables(tensors_host, n_tensors, [&](const TensorTable &T, int) { partials += T.first[T.n] < kNormBlocks ? T.first[T.n] : kNormBlocks; return (int)IGCN_OK; }) != IGCN_OK)
-        return -1;
+    const int rc = for_tables(tensors_host, n_tensors, [&](const TensorTable &T, int) {
+        partials += std::min(T.first[T.n], kNormBlocks);
+        return (int)IGCN_OK;
+    });
+    if (rc != IGCN_OK) return -1;
     return n_tensors * (int64_t)sizeof(Prepared) + partials * 8 + 16;
 }
 
@@ -502,20 +507,20 @@ extern "C" int igcn_grad_norm(const igcn_adamw_tensor *tensors_host, int64_t n_t
     return launch_status();
 }
 
-extern "C" int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, int32_t moment_bits, double lr, const float *lr_dev, double beta1, double beta2,
-                               double eps, double weight_decay, double max_norm, const float *norm_in, float *norm_out, uint64_t seed,
-                               void *workspace, void *stream)
+extern "C" int igcn_adamw_step(const igcn_adamw_tensor *tensors_host, int64_t n_tensors, int32_t moment_bits, double lr, const float *lr_dev,
+                               double beta1, double beta2, double eps, double weight_decay, double max_norm, const float *norm_in,
+                               float *norm_out, uint64_t seed, void *workspace, void *stream)
 {
     if (moment_bits != 8 && moment_bits != 32) return IGCN_E_RANGE;
     const bool clipped = max_norm > 0.0;
     const int rc = check_tensors(tensors_host, n_tensors, moment_bits, lr_dev, clipped ? norm_in : nullptr, clipped ? norm_out : nullptr);
     if (rc != IGCN_OK) return rc;
-    if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(max_norm >= 0.0))
-        return IGCN_E_RANGE;
+    if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) return IGCN_E_RANGE;
+    if (!(eps >= 0.0) || !(weight_decay >= 0.0) || !(max_norm >= 0.0)) return IGCN_E_RANGE;
     if (n_tensors > 0 && !workspace) return IGCN_E_NULL;
     if (max_norm > 0.0 && !norm_in && !norm_out) return IGCN_E_NULL;
-    if ((reinterpret_cast<uintptr_t>(workspace) & 15) || ((reinterpret_cast<uintptr_t>(norm_in) | reinterpret_cast<uintptr_t>(norm_out) | reinterpret_cast<uintptr_t>(lr_dev)) & 3))
-        return IGCN_E_ALIGN;
+    const uintptr_t numbers = reinterpret_cast<uintptr_t>(norm_in) | reinterpret_cast<uintptr_t>(norm_out) | reinterpret_cast<uintptr_t>(lr_dev);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) || (numbers & 3)) return IGCN_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
     Prepared *prep = static_cast<Prepared *>(workspace);
     double *partial = reinterpret_cast<double *>(prep + n_tensors);

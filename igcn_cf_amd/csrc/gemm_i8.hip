@@ -4,8 +4,9 @@
 //
 // The sum is exact (int32: K <= 131 071); the scales are applied once, in float32, before the one rounding to the output's type.
 //
-// Measured: 8192 x 8192 x 4096 to bfloat16 264 us = 2.1 POP/s (a library's bare int8 product: 306 us), 512 x 96421 x 64 to float32 45-54 us = 3.7-4.4
-// TB/s of y (the same stores alone 45), 4 x 16384 x 8192 28 us = 4.8 TB/s of b, 16 x 4096 x 4096 7 us, 1 x 96421 x 64 from float32 7.1 us.
+// Measured: 8192 x 8192 x 4096 to bfloat16 262 us = 2.1 POP/s (a library's bare int8 product: 306 us; matrix pipes busy 52 % of the cycles, LDS
+// 1.6 M conflict cycles of 30 M), 512 x 96421 x 64 to float32 46-54 us = 3.7-4.3 TB/s of y (the same stores alone 45), 4 x 16384 x 8192 28 us =
+// 4.8 TB/s of b, 16 x 4096 x 4096 7 us, 1 x 96421 x 64 from float32 7.1 us.
 #include "gemm_i8_rule.h"
 #include "quant_i8.h"
 #include <type_traits>
@@ -100,7 +101,8 @@ __device__ __forceinline__ void to_lds(const void *p, unsigned lds)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
-template <int LEFT> __device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory"); }      // all but the last LEFT are there
+// all but the last LEFT are there
+template <int LEFT> __device__ __forceinline__ void wait_for_lds() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory"); }
 
 struct TileArgs { GemmArgs g; int64_t tiles_m, tiles_n, per_xcd; bool asks_ahead; };
 
@@ -124,7 +126,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     const int64_t band = t / (bd * T.tiles_n), in = t - band * bd * T.tiles_n, high = T.tiles_m - bd * band < bd ? T.tiles_m - bd * band : bd;
     const int64_t m0 = (bd * band + in % high) * TM, n0 = in / high * TN;
 
-    // this lane's pieces: rows 8 (wave NA + i) + lane / 8 of the tile, piece (lane % 8) ^ (row / 2 % 8); offsets from the tile's first row fit 32 bits
+    // this lane's pieces: rows 8 (wave NA + i) + lane / 8 of the tile, piece (lane % 8) ^ (row / 2 % 8); offsets from the tile's first row fit
+    // 32 bits
     auto piece = [&](int i) { return ((lane & 7) ^ ((4 * i + (lane >> 4)) & 7)) * 16; };       // ... of rows 8 i ... 8 i + 7
     const int8_t *const base_a = G.a + m0 * G.lda, *const base_b = G.b + n0 * G.ldb;
     const int last_a = (int)(G.m - m0 < TM ? G.m - m0 : TM) - 1, last_b = (int)(G.n - n0 < TN ? G.n - n0 : TN) - 1;
@@ -148,10 +151,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
                 for (int i = 0; i < NB; ++i) to_lds(base_b + k0, ob[i], bt + 1024 * i);
             } else {                                             // (pieces are whole: the depth is a multiple of 16)
+                const void *const zeros = &g_zeros;
 #pragma unroll
-                for (int i = 0; i < NA; ++i) to_lds(k0 + piece(wave * NA + i) < k ? (const void *)(base_a + k0 + oa[i]) : (const void *)&g_zeros, at + 1024 * i);
+                for (int i = 0; i < NA; ++i) to_lds(k0 + piece(wave * NA + i) < k ? (const void *)(base_a + k0 + oa[i]) : zeros, at + 1024 * i);
 #pragma unroll
-                for (int i = 0; i < NB; ++i) to_lds(k0 + piece(wave * NB + i) < k ? (const void *)(base_b + k0 + ob[i]) : (const void *)&g_zeros, bt + 1024 * i);
+                for (int i = 0; i < NB; ++i) to_lds(k0 + piece(wave * NB + i) < k ? (const void *)(base_b + k0 + ob[i]) : zeros, bt + 1024 * i);
             }
         } else {                                                 // (past the end: the row's last 16 codes, put in place by land())
 #pragma unroll
@@ -175,8 +179,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
         for (int i = 0; i < NB; ++i) at[TM * kDepth / 16 + (wave * NB + i) * 64 + lane] = held[NA + i];
     };
 
-    // Where every tile starts with reads that queue behind the writes of y (i8_asks_ahead): the first row of tiles of a band asks for the rows of b of kSoon
-    // tiles on, twice what an XCD has under way, so that those find them in a cache.
+    // Where every tile starts with reads that queue behind the writes of y (i8_asks_ahead): the first row of tiles of a band asks for the rows
+    // of b of kSoon tiles on, twice what an XCD has under way, so that those find them in a cache.
     constexpr int kSoon = 64;
     i32x4 soon = {0, 0, 0, 0};
     if constexpr (DIRECT && !BY_DEPTH && TM < 256) {
@@ -186,7 +190,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     }
     i32x16 acc[AR][AC] = {};
     const int wm = wave / WN, wn = wave % WN;
-    const int ra = (BY_DEPTH ? 0 : wm * (TM / WM)) + (lane & 31), rb = (BY_DEPTH ? 0 : wn * (TN / WN)) + (lane & 31), half = lane >> 5, turn = (lane >> 1) & 7;
+    const int half = lane >> 5, turn = (lane >> 1) & 7;
+    const int ra = (BY_DEPTH ? 0 : wm * (TM / WM)) + (lane & 31), rb = (BY_DEPTH ? 0 : wn * (TN / WN)) + (lane & 31);
     float *const fa = reinterpret_cast<float *>(smem), *const fb = fa + TM, *const fc = fb + TN;       // the tile's scales and bias, for the way out
     for (int i = threadIdx.x; i < TM; i += 64 * kWaves) fa[i] = i <= last_a ? G.sa[m0 + i] : 0.f;
     for (int i = threadIdx.x; i < TN; i += 64 * kWaves) {
@@ -237,14 +242,17 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     };
     for (int64_t s = 0; s < stages; ++s) stage(s);
     __syncthreads();
-    if constexpr (BY_DEPTH) {                                    // piece q of the tile goes to wave q: [piece][the three other waves][4 sums a lane and quarter]
+    if constexpr (BY_DEPTH) {                                    // piece q of the tile goes to wave q: [piece][three other waves][quarter][lane], 4 sums each
         i32x4 *const sums = reinterpret_cast<i32x4 *>(ring);
 #pragma unroll
         for (int q = 0; q < kWaves; ++q)
             if (q != wave) {
                 i32x4 *to = sums + ((q * 3 + (wave - (wave > q))) * 4) * 64 + lane;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) to[64 * i] = i32x4{acc[q / WN][q % WN][4 * i], acc[q / WN][q % WN][4 * i + 1], acc[q / WN][q % WN][4 * i + 2], acc[q / WN][q % WN][4 * i + 3]};
+                for (int i = 0; i < 4; ++i) {
+                    const i32x16 &part = acc[q / WN][q % WN];
+                    to[64 * i] = i32x4{part[4 * i], part[4 * i + 1], part[4 * i + 2], part[4 * i + 3]};
+                }
             }
         __syncthreads();
         i32x16 all = acc[0][0];
@@ -268,7 +276,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
     // lines: 16 bytes a lane, neighbouring lanes along the row.
     auto put = [&](auto *y) {
         using Y = std::remove_pointer_t<decltype(y)>;
-        constexpr int kCols = CT * 32, kRow = kCols * sizeof(Y) + 16, kLanes = kCols * sizeof(Y) / 16, kRows = 64 / kLanes, kE = 16 / sizeof(Y);       // (16 bytes more a row: other banks)
+        constexpr int kE = 16 / sizeof(Y), kCols = CT * 32, kLanes = kCols / kE, kRows = 64 / kLanes;
+        constexpr int kRow = kCols * sizeof(Y) + 16;             // (16 bytes more a row: other banks)
         unsigned char *const strip = ring + wave * 32 * (kCols * 4 + 16);
         const bool biased = G.bias != nullptr;
         const int n1 = wn * (TN / WN) + lane % kLanes * kE;      // of the tile: this lane's columns on the way out
@@ -280,9 +289,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tiles_i8_kernel(const TileArg
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int at = c * 32 + 8 * q + 4 * half;
-                    const float4 sb4 = *reinterpret_cast<const float4 *>(fb + wn * (TN / WN) + at), bi4 = *reinterpret_cast<const float4 *>(fc + wn * (TN / WN) + at);
-                    Y v[4] = {from_float<Y>(scaled(acc[r][c][4 * q], s, sb4.x, biased, bi4.x)), from_float<Y>(scaled(acc[r][c][4 * q + 1], s, sb4.y, biased, bi4.y)),
-                              from_float<Y>(scaled(acc[r][c][4 * q + 2], s, sb4.z, biased, bi4.z)), from_float<Y>(scaled(acc[r][c][4 * q + 3], s, sb4.w, biased, bi4.w))};
+                    const float4 sb4 = *reinterpret_cast<const float4 *>(fb + wn * (TN / WN) + at);
+                    const float4 bi4 = *reinterpret_cast<const float4 *>(fc + wn * (TN / WN) + at);
+                    auto out = [&](int e, float sb, float bias) { return from_float<Y>(scaled(acc[r][c][4 * q + e], s, sb, biased, bias)); };
+                    Y v[4] = {out(0, sb4.x, bi4.x), out(1, sb4.y, bi4.y), out(2, sb4.z, bi4.z), out(3, sb4.w, bi4.w)};
                     __builtin_memcpy(__builtin_assume_aligned(strip + (lane & 31) * kRow + at * sizeof(Y), 8), v, sizeof(v));
                 }
             const int m1 = wm * (TM / WM) + r * 32 + lane / kLanes;
@@ -335,16 +345,20 @@ template <int TM, int TN, int WM, int WN, int STAGES, bool BY_DEPTH = false> sta
         hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * T.per_xcd)), dim3(64 * WM * WN), lds, st, T);
         return launch_status();
     };
-    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true, BY_DEPTH>, STAGES) : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false, BY_DEPTH>, 2);
+    return direct ? launch(tiles_i8_kernel<TM, TN, WM, WN, STAGES, true, BY_DEPTH>, STAGES)
+                  : launch(tiles_i8_kernel<TM, TN, WM, WN, 2, false, BY_DEPTH>, 2);
 }
 
 // ---- a few rows of a ------------------------------------------------------------------------------------------------------------------
-// Bound by the bytes of b, each used once, or by the way through the depth where neither side has many: no tile is worth staging.  A wave takes 16 rows of b as the matrix instruction's first operand straight
-// from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes of depth at 16 (l / 16)) and up to 16 rows of a, which stay in L2, as the
-// second.  KEEP steps' loads are under way while the ones before are multiplied.
-// A lane's row of either side.  BYTES: rows at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from elsewhere at half of it
-// (1 row against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them into place; the first
-// and the last row of b, whose words may reach over its ends, are loaded as they are.  What is behind a row's end meets zeros of a.
+// Bound by the bytes of b, each used once, or by the way through the depth where neither side has many: no tile is worth staging.  A wave
+// takes 16 rows of b as the matrix instruction's first operand straight from memory (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, 16 bytes
+// of depth at 16 (l / 16)) and up to 16 rows of a, which stay in L2, as the second.  KEEP steps' loads are under way while the ones before are
+// multiplied.
+
+// A lane's row of either side.  BYTES: rows at any byte.  The memory system takes 16 bytes from a multiple of 4 at full speed, from
+// elsewhere at half of it (1 row against 16384 x 4095: 31 us, this way 15): a lane loads the five words around its 16 bytes and shifts them
+// into place; the first and the last row of b, whose words may reach over its ends, are loaded as they are.  What is behind a row's end
+// meets zeros of a.
 template <bool BYTES> struct Row {
     const int8_t *p;
     int off, last, more;                                         // of the row behind a multiple of 4; the last piece's place; to the fifth word
@@ -606,7 +620,8 @@ __global__ __launch_bounds__(kBlock) void few_rows_i8_kernel(const FewArgs F)
                 const int64_t n0 = (tile0 + t) * 16 + 4 * quarter;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (r < m && n0 + i < G.n) store_out(G, r, n0 + i, scaled(acc[t][i], sx[r], G.sb[n0 + i], G.bias != nullptr, G.bias ? G.bias[n0 + i] : 0.f));
+                    if (r < m && n0 + i < G.n)
+                        store_out(G, r, n0 + i, scaled(acc[t][i], sx[r], G.sb[n0 + i], G.bias != nullptr, G.bias ? G.bias[n0 + i] : 0.f));
             }
         }
     }
@@ -659,15 +674,16 @@ static int product(const GemmArgs &G, hipStream_t st)
     return IGCN_OK;
 }
 
-static int check_product(const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias, int64_t m, int64_t n, int64_t k, const void *y,
-                         int32_t dtype, int64_t ldy)
+static int check_product(const float *sa, const int8_t *b, int64_t ldb, const float *sb, const float *bias, int64_t m, int64_t n, int64_t k,
+                         const void *y, int32_t dtype, int64_t ldy)
 {
     if (!dtype_ok(dtype)) return IGCN_E_RANGE;
     if (m < 0 || n < 0 || k < 0 || ldb < k || ldy < n) return IGCN_E_SHAPE;
     if (k > IGCN_MAX_I8_DEPTH) return IGCN_E_RANGE;
     if (m == 0 || n == 0) return IGCN_OK;
     if (!sb || !y || (k > 0 && !b)) return IGCN_E_NULL;
-    if (misaligned(y, dtype) || ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sb) | reinterpret_cast<uintptr_t>(bias)) & 3)) return IGCN_E_ALIGN;
+    const uintptr_t vectors = reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sb) | reinterpret_cast<uintptr_t>(bias);
+    if (misaligned(y, dtype) || (vectors & 3)) return IGCN_E_ALIGN;
     return IGCN_OK;
 }
 

@@ -7,7 +7,8 @@
 // power of two that makes I one, up to a wave; from 129 pieces on more waves share the row, at most two pieces a lane until it is long
 // (2048 rows of 8192 bfloat16: two pieces on 512 lanes 13.7 us, four on 256 16.7).  Short rows: each lane group takes R rows at once, R loads
 // in flight before the first maximum.  Rows over kHeldPieces do not fit: they are read a second time (from L2).
-// Measured: 206151 x 64 float32 12.7 us = 5.3 TB/s (and back 11.6 = 5.8), 2048 x 8191 bfloat16, rows at any multiple of 2, 14.2 us = 3.5 (back to float32 16).
+// Measured: 206151 x 64 float32 12.7 us = 5.3 TB/s (and back 11.8 = 5.7), 2048 x 8191 bfloat16, rows at any multiple of 2, 14.3 us = 3.5
+// (back to float32 16).
 #include "quant_i8.h"
 
 namespace igcn {

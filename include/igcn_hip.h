@@ -504,7 +504,8 @@ typedef struct igcn_adamw_tensor {
  * lr_dev: NULL, or a device float read instead of lr (a captured step whose rate changes).
  * moment_bits 32: float32 moments.  8: a block of IGCN_ADAMW_BLOCK elements is held as e4m3 codes of m / s_m and e5m2 codes of v / s_v,
  * s_m = max|m| / 448, s_v = max v / 57344, rounded stochastically with 16 bits of a hash of (seed, tensor's place in the list, step,
- * element); v > 0 is never held as 0; a block below 2^-100 is held as zeros, one with a NaN or an infinity gets a NaN scale.
+ * element; the float32 step count ends at 2^24).  v > 0 is not held as 0 unless under 2^-165 of its block's largest; a block below 2^-100
+ * is held as zeros, one with a NaN or an infinity gets a NaN scale.
  * The averages themselves are formed unrounded before the parameter is updated.
  * workspace: igcn_adamw_workspace_bytes(...) bytes, 16-byte aligned; one call's own.  Memory that the call rewrites stands in one
  * place of the list only, gradients, lr_dev and the norm included (IGCN_E_OVERLAP); a tensor has at most (2^24 - 1) * 2048 elements. */
