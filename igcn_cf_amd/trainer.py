@@ -185,11 +185,14 @@ class BasicTrainer:
 
     def _norm_reduce_fn(self):
         """Where the parameters are a rank's share of a model: what sums over its ranks; else None."""
-        return getattr(self.model, 'slice_reduce_fn', None) or getattr(self.model, 'all_reduce', None)
+        reduce_fn = getattr(self.model, 'slice_reduce_fn', None)
+        if reduce_fn is None and any(getattr(p, 'is_share', False) for p in self.model.parameters()):
+            reduce_fn = getattr(self.model, 'all_reduce', None)
+        return reduce_fn
 
     def _optimizer_step(self):
-        if isinstance(self.opt, AdamW):
-            self.opt.norm_reduce_fn = self._norm_reduce_fn() or self.opt.norm_reduce_fn      # (the model's may have been replaced)
+        if isinstance(self.opt, AdamW):            # (a model's slice_reduce_fn may have been replaced since)
+            self.opt.norm_reduce_fn = getattr(self.model, 'slice_reduce_fn', None) or self.opt.norm_reduce_fn
         self.opt.step()
 
     # ---- one optimisation step as ONE captured HIP graph (config key 'hip_graph', default True) -----------------

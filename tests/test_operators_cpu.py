@@ -328,3 +328,23 @@ int main()
     few = [(m, n, k, k, k + past, 0, 1) for m, n, k, _, past in G.FEW_SIZES]
     met = {(shares, byte, k < 16, dtype) for (m, n, k, dtype, _), (_, _, byte, fused, shares, _) in zip(G.FEW_SIZES, ask(few)) if fused}
     assert {(s, b, t) for s, b, _, t in met} == {(s, b, t) for s in (0, 1) for b in (0, 1) for t in G.DTYPES} and {s for s, _, short, _ in met if short} == {0, 1}
+
+
+def test_a_trainer_takes_the_sum_over_ranks_of_shares_only():
+    """A model's all_reduce is the clipped norm's where its parameters are marked as shares (dist's models mark them), not where every rank has all of
+    them and the method means something else; a slice_reduce_fn that is replaced later is followed."""
+    from igcn_cf_amd.trainer import BPRTrainer
+    trainer = BPRTrainer.__new__(BPRTrainer)
+    trainer.model = torch.nn.Linear(3, 3)
+    trainer.model.all_reduce = lambda t: t
+    trainer.config = {'optimizer': 'AdamW', 'lr': 0.1, 'max_grad_norm': 1.}
+    trainer.initialize_optimizer()
+    assert trainer.opt.norm_reduce_fn is None
+    for p in trainer.model.parameters():
+        p.is_share = True
+    trainer.initialize_optimizer()
+    assert trainer.opt.norm_reduce_fn is trainer.model.all_reduce
+    trainer.opt.step = lambda: None
+    trainer.model.slice_reduce_fn = lambda t: t
+    trainer._optimizer_step()
+    assert trainer.opt.norm_reduce_fn is trainer.model.slice_reduce_fn
